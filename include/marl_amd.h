@@ -549,6 +549,66 @@ int ec_bn_relu_dropout_bwd_dx(const float* dout, const float* x, const float* sc
                               uint64_t seed, float p, const float* a, const float* b, const float* c, int64_t rows, int32_t C,
                               float* dx, void* stream);
 
+/* --- operators of a policy's training step, for any width and any number of tokens / actions ------------------
+ * Element types of the tensors they take (every sum, norm and softmax statistic is fp32 or wider): */
+#define EC_F32 0
+#define EC_BF16 1
+#define EC_F16 2
+
+/* Layer norm over the last dimension.  x [rows][cols] of `dtype` with row stride x_stride (elements, >= 0; the columns are
+ * contiguous, any alignment); weight, bias [cols] of wdtype (EC_F32 or dtype), each optional (1 and 0).
+ *   y = (x - mean) / sqrt(var + eps) * weight + bias, var = mean (x - mean)^2;  y [rows][cols] contiguous;
+ *   mean, rstd [rows] f32, each optional.  1 <= cols <= 2^24. */
+int ec_layer_norm_fwd(const void* x, int64_t x_stride, const void* weight, const void* bias, int32_t dtype, int32_t wdtype,
+                      int64_t rows, int64_t cols, double eps, void* y, float* mean, float* rstd, void* stream);
+/* Its gradients: dx [rows][cols] of dtype, dweight / dbias [cols] of wdtype, each optional; rows >= 1.  partials: scratch
+ * f32 [n_partials][2][cols], n_partials = ec_layer_norm_bwd_partials(rows, cols, dtype) (NULL and 0 when neither dweight
+ * nor dbias is asked for).  The sums over rows are added in a fixed order: the same bits every run. */
+int64_t ec_layer_norm_bwd_partials(int64_t rows, int64_t cols, int32_t dtype);
+int ec_layer_norm_bwd(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const float* mean, const float* rstd,
+                      const void* weight, int32_t dtype, int32_t wdtype, int64_t rows, int64_t cols, void* dx, float* partials,
+                      int64_t n_partials, void* dweight, void* dbias, void* stream);
+
+/* Log-probs of given tokens (actions) under softmax(logits), the entropy, and the top_k likeliest entries.
+ * logits [rows][vocab] of dtype: row r lies at (r / inner) * s_outer + (r % inner) * s_inner elements, its columns are
+ * contiguous; tokens [rows] i64.  avail: entries with 0 are excluded (so are logits of -inf); mask_dtype 0: none (NULL),
+ * 1: bytes, 2: i32; laid out as logits, with strides a_outer, a_inner.  What an excluded entry's logit holds does not matter.
+ *   logp [rows]: log p(token); 0 for a token below 0 (a padded row), NaN for one >= vocab, -inf for an excluded one
+ *   entropy [rows];  lse [rows][2]: the largest logit and log(sum exp(logit - largest)), their sum is the log-sum-exp
+ *   top_logp f32, top_index i64 [rows][top_k]: in falling order, equal ones by index; -inf / -1 where there are fewer
+ * A row with everything excluded: logp -inf, entropy 0, lse (-inf, 0).  A NaN or +inf among the entries makes the row NaN
+ * (top_index -1).  Outputs are optional; top_k <= 64.  work: scratch, ec_token_logprobs_workspace bytes, 8-byte aligned. */
+#define EC_TOKEN_LOGPROBS_MAX_TOP 64
+int64_t ec_token_logprobs_workspace(int64_t rows, int64_t vocab, int32_t dtype, int32_t top_k);
+int ec_token_logprobs_fwd(const void* logits, int64_t inner, int64_t s_outer, int64_t s_inner, const int64_t* tokens,
+                          const void* avail, int32_t mask_dtype, int64_t a_outer, int64_t a_inner, int32_t dtype, int64_t rows,
+                          int64_t vocab, int32_t top_k, float* logp, float* entropy, float* lse, float* top_logp,
+                          int64_t* top_index, void* work, int64_t work_bytes, void* stream);
+/* d logits [rows][vocab] (contiguous, of dtype) from the forward's lse and entropy and from dlogp, dentropy [rows] (each
+ * optional: 0): dlogp (1[v = token] - p_v) - dentropy p_v (log p_v + entropy), 0 at excluded entries and in rows with
+ * nothing else; a token below 0 takes no dlogp. */
+int ec_token_logprobs_bwd(const void* logits, int64_t inner, int64_t s_outer, int64_t s_inner, const int64_t* tokens,
+                          const void* avail, int32_t mask_dtype, int64_t a_outer, int64_t a_inner, int32_t dtype, int64_t rows,
+                          int64_t vocab, const float* lse, const float* entropy, const float* dlogp, const float* dentropy,
+                          void* dlogits, void* stream);
+
+/* coef <- min(1, max_norm / (norm + 1e-6)) with norm = sqrt(sum g^2) over `count` gradients of types dtypes[i], max_norm > 0
+ * (clip_grad_norm_'s factor, left on the device for ec_adamw_step; the gradients are only read); *norm <- norm, optional.
+ * work: ec_grad_clip_workspace bytes, 8-byte aligned.  Sums in double, in a fixed order. */
+int64_t ec_grad_clip_workspace(int32_t count, const int64_t* numel);
+int ec_grad_clip_coef(int32_t count, const void* const* grads, const int64_t* numel, const int32_t* dtypes, double max_norm,
+                      float* norm, float* coef, void* work, int64_t work_bytes, void* stream);
+/* One AdamW step (decoupled weight decay) over `count` tensors of any size; dtypes[i]: the type of params[i] and grads[i].
+ * state_bits 32: exp_avg, exp_avg_sq f32 (scales NULL).  state_bits 8: exp_avg [numel] e4m3 with exp_avg_scale
+ * [ceil(numel / 256)] f32: m = q * scale over each 256 consecutive elements; exp_avg_sq likewise holds sqrt(v).
+ * coef (optional, on the device) scales the gradients as they are read.  The step count is step_host (this step's, from 1
+ * on), or *step_dev f32, which the call advances (dyn: scratch of 3 f32); with it lr may come from *lr_dev.  Pointers need
+ * no alignment beyond their element's. */
+int ec_adamw_step(int32_t count, void* const* params, const void* const* grads, void* const* exp_avg, void* const* exp_avg_sq,
+                  float* const* exp_avg_scale, float* const* exp_avg_sq_scale, const int64_t* numel, const int32_t* dtypes,
+                  int32_t state_bits, const float* coef, double step_host, float* step_dev, float* dyn, double lr,
+                  const float* lr_dev, double beta1, double beta2, double eps, double weight_decay, void* stream);
+
 const char* ec_last_error(void);
 const char* ec_version(void);
 

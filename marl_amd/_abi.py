@@ -189,13 +189,26 @@ def lib():
     L.ec_store_episode_static.argtypes = [vp] * 9 + [i64, i32, i32, i32, i64] + [vp] * 8
     L.ec_debug_store_episode_static_scratch.argtypes = [i32, C.POINTER(vp), C.POINTER(i64), vp]
     L.ec_debug_store_episode_static_scratch.restype = C.c_int
+    f64 = C.c_double
+    L.ec_layer_norm_fwd.argtypes = [vp, i64, vp, vp, i32, i32, i64, i64, f64, vp, vp, vp, vp]
+    L.ec_layer_norm_bwd.argtypes = [vp, i64, vp, i64, vp, vp, vp, i32, i32, i64, i64, vp, vp, i64, vp, vp, vp]
+    L.ec_layer_norm_bwd_partials.argtypes = [i64, i64, i32]
+    L.ec_token_logprobs_fwd.argtypes = [vp, i64, i64, i64, vp, vp, i32, i64, i64, i32, i64, i64, i32] + [vp] * 6 + [i64, vp]
+    L.ec_token_logprobs_bwd.argtypes = [vp, i64, i64, i64, vp, vp, i32, i64, i64, i32, i64, i64] + [vp] * 6
+    L.ec_token_logprobs_workspace.argtypes = [i64, i64, i32, i32]
+    L.ec_grad_clip_workspace.argtypes = [i32, vp]
+    L.ec_grad_clip_coef.argtypes = [i32, vp, vp, vp, f64, vp, vp, vp, i64, vp]
+    L.ec_adamw_step.argtypes = [i32] + [vp] * 8 + [i32, vp, f64, vp, vp, f64, vp, f64, f64, f64, f64, vp]
+    for fn in ("ec_layer_norm_bwd_partials", "ec_token_logprobs_workspace", "ec_grad_clip_workspace"):
+        getattr(L, fn).restype = i64
     for fn in ("ec_create", "ec_destroy", "ec_reset", "ec_observe", "ec_step", "ec_random_policy", "ec_status",
                "ec_debug_dump", "ec_debug_rng_cursors", "ec_debug_live_tasks", "ec_info", "ec_gae",
                "ec_policy_forward", "ec_gail_reward", "ec_diffusion_reward", "ec_diffusion_grad", "ec_expert_policy",
                "ec_ppo_actor_grad", "ec_ppo_critic_grad", "ec_ppo_actor_grad_ex", "ec_ppo_critic_grad_ex", "ec_gail_disc_grad", "ec_store_transition", "ec_bn_relu_dropout_fwd", "ec_bn_relu_dropout_bwd_sums", "ec_bn_relu_dropout_bwd_dx", "ec_expert_mix", "ec_store_episode", "ec_store_episode_static",
                "ec_step_random_policy", "ec_rollout_random_policy", "ec_rollout_mlp_policy",
                "ec_rollout_mlp_expert_policy", "ec_expert_append_episode", "ec_adam_clip_step", "ec_bn_col_stats", "ec_diffusion_grad_bce", "ec_linear_wgrad", "ec_bn_finalize", "ec_bn_bwd_coeffs", "ec_linear_fwd", "ec_linear_fwd_bn", "ec_linear2_fwd_bn", "ec_row_moments", "ec_disc_rows", "ec_linear_fwd_stats",
-               "ec_diffusion_reward_from_loss"):
+               "ec_diffusion_reward_from_loss", "ec_layer_norm_fwd", "ec_layer_norm_bwd", "ec_token_logprobs_fwd",
+               "ec_token_logprobs_bwd", "ec_grad_clip_coef", "ec_adamw_step"):
         getattr(L, fn).restype = C.c_int
     L.ec_last_error.restype = C.c_char_p
     L.ec_version.restype = C.c_char_p

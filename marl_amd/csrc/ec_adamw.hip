@@ -1,0 +1,370 @@
+// ec_adamw.hip -- one AdamW step over many tensors of any size, with moments in fp32 or in 8 bits.
+//
+//   norm = sqrt(sum g^2) over all tensors;  coef = min(1, max_norm / (norm + 1e-6));  g' = coef g
+//   m' = m + (g' - m)(1 - b1);  v' = v b2 + (1 - b2) g' g'
+//   p' = p (1 - lr wd) - lr / (1 - b1^t) m' / (sqrt(v') / sqrt(1 - b2^t) + eps)
+//
+// 8 bits: each 256 consecutive elements of a tensor share two fp32 scales; m is held as q s with q in e4m3 and
+// s = max |m| / 448, and v as (q s)^2, the root being what the step divides by and having half the range of v in exponents.
+// q is rounded to the nearest e4m3 value (relative step 2^-3 .. 2^-4, the states' only loss: the step itself uses m' and v'
+// before they are rounded), except that the q of a v' > 0 is never 0, which would turn a rounding into a step of lr m / eps.
+//
+// Bound by HBM: every operand once, 28 bytes an element in fp32 (16 with 8-bit moments), no intermediate.  A launch takes
+// up to MAX_TENSORS tensors in its argument block, so nothing is copied to the device; a block finds its tensor by the
+// first block of each.  The clip reads g once more: per-block sums in double, added in a fixed order by one block, so that
+// the coefficient is the same every run; it stays on the device.
+#include <cmath>
+
+#include "ec_stream.h"
+
+namespace {
+
+using namespace ecs;
+
+constexpr int MAX_TENSORS = 48;          // (the argument block stays under the 4 KB a launch can carry)
+constexpr int CHUNK = 4096;              // elements a block
+constexpr int QBLOCK = 256;              // elements that share a scale: a wave, four each
+constexpr float QMAX = 448.0f, QMIN = 0.001953125f;
+
+struct Tensor {
+    void *p, *m, *v;
+    const void* g;
+    float *ms, *vs;
+    int64_t n;
+};
+struct Group {
+    Tensor t[MAX_TENSORS];
+    uint32_t first[MAX_TENSORS + 1];     // first block of each tensor
+    int count;
+};
+struct Hyper {
+    float omb1, b2, omb2, eps;           // 1 - beta, rounded once from double
+    float step_size, bc2_sqrt, keep;     // lr / (1 - b1^t), sqrt(1 - b2^t), 1 - lr wd
+    const float* coef;                   // of the gradients, on the device, or NULL: 1
+    const float* dyn;                    // {step_size, bc2_sqrt, keep} on the device, or NULL
+};
+static_assert(sizeof(Group) + sizeof(Hyper) + 64 <= 4096, "argument block");
+
+__device__ __forceinline__ int tensor_of(const Group& a, uint32_t block) {
+    int lo = 0, hi = a.count;            // first[lo] <= block < first[hi]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a.first[mid] <= block) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ void read_hyper(Hyper& h, float& coef) {
+    coef = h.coef ? *h.coef : 1.0f;
+    if (h.dyn) h.step_size = h.dyn[0], h.bc2_sqrt = h.dyn[1], h.keep = h.dyn[2];
+}
+
+// m, v -> m', v' and p -> p'; root: sqrt(v').  One rounding per operation, in the order of the formulas above
+__device__ __forceinline__ void adam(const Hyper& h, float coef, float g, float& p, float& m, float& v, float& root) {
+    g *= coef;
+    m = m + (g - m) * h.omb1;
+    v = v * h.b2 + h.omb2 * g * g;
+    root = sqrtf(v);
+    p = p * h.keep - h.step_size * m / (root / h.bc2_sqrt + h.eps);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) k_adamw32(Group a, Hyper h) {
+    const int k = tensor_of(a, blockIdx.x);
+    const Tensor t = a.t[k];
+    float coef;
+    read_hyper(h, coef);
+    const int64_t e0 = (int64_t)(blockIdx.x - a.first[k]) * CHUNK;
+#pragma unroll 4
+    for (int i = 0; i < CHUNK / 1024; i++) {
+        const int64_t e = e0 + i * 1024 + threadIdx.x * 4, n = t.n - e;
+        float p[4], g[4], m[4], v[4], root;
+        load_upto((const T*)t.p + e, n, 0.0f, p);
+        load_upto((const T*)t.g + e, n, 0.0f, g);
+        load_upto((const float*)t.m + e, n, 0.0f, m);
+        load_upto((const float*)t.v + e, n, 0.0f, v);
+#pragma unroll
+        for (int j = 0; j < 4; j++) adam(h, coef, g[j], p[j], m[j], v[j], root);
+        store_upto((T*)t.p + e, n, p);
+        store_upto((float*)t.m + e, n, m);
+        store_upto((float*)t.v + e, n, v);
+    }
+}
+
+// four e4m3 values of a dword
+__device__ __forceinline__ void unpack8(uint32_t q, float (&f)[4]) {
+    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)q, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)q, true);
+    f[0] = lo[0], f[1] = lo[1], f[2] = hi[0], f[3] = hi[1];
+}
+__device__ __forceinline__ uint32_t pack8(const float (&f)[4]) {
+    int q = __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], q, true);
+}
+typedef uint32_t u32_any __attribute__((aligned(1)));
+__device__ __forceinline__ uint32_t load8(const uint8_t* q, int64_t n) {
+    if (n >= 4) return *reinterpret_cast<const u32_any*>(q);
+    uint32_t x = 0;
+#pragma unroll
+    for (int j = 0; j < 3; j++)
+        if (j < n) x |= (uint32_t)q[j] << (8 * j);
+    return x;
+}
+__device__ __forceinline__ void store8(uint8_t* q, int64_t n, uint32_t x) {
+    if (n >= 4) {
+        *reinterpret_cast<u32_any*>(q) = x;
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 3; j++)
+        if (j < n) q[j] = (uint8_t)(x >> (8 * j));
+}
+// the scale of a block whose largest magnitude has these bits (a NaN's are larger than any number's: it marks the whole
+// block), and its inverse; a block of zeros, or of what is too small for 1 / s, is held as zeros
+__device__ __forceinline__ float scale_of(uint32_t most, float& inv) {
+    float s = bitsf(most) / QMAX;
+    s = s < 1.17549435e-38f ? 0.0f : s;
+    inv = s != 0.0f ? 1.0f / s : 0.0f;
+    return s;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) k_adamw8(Group a, Hyper h) {
+    const int k = tensor_of(a, blockIdx.x), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const Tensor t = a.t[k];
+    float coef;
+    read_hyper(h, coef);
+    const int64_t b0 = (int64_t)(blockIdx.x - a.first[k]) * (CHUNK / QBLOCK);
+#pragma unroll 4
+    for (int i = 0; i < CHUNK / QBLOCK / 4; i++) {
+        const int64_t b = b0 + i * 4 + wave, e = b * QBLOCK + lane * 4, n = t.n - e;
+        if (b * QBLOCK >= t.n) break;  // (the same for all lanes of the wave)
+        float p[4], g[4], m[4], v[4], root[4];
+        load_upto((const T*)t.p + e, n, 0.0f, p);
+        load_upto((const T*)t.g + e, n, 0.0f, g);
+        unpack8(load8((const uint8_t*)t.m + e, n), m);
+        unpack8(load8((const uint8_t*)t.v + e, n), v);
+        const float ms = t.ms[b], vs = t.vs[b];
+        uint32_t most_m = 0, most_v = 0;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            m[j] *= ms;
+            v[j] *= vs;
+            v[j] *= v[j];
+            adam(h, coef, g[j], p[j], m[j], v[j], root[j]);
+            const uint32_t am = fbits(m[j]) & 0x7fffffffu, av = fbits(root[j]) & 0x7fffffffu;
+            most_m = am > most_m ? am : most_m;
+            most_v = av > most_v ? av : most_v;
+        }
+        float im, iv;
+        const float sm = scale_of(lanes_umax<64>(most_m), im), sv = scale_of(lanes_umax<64>(most_v), iv);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            m[j] *= im;
+            const float q = root[j] * iv;
+            v[j] = root[j] > 0.0f && sv > 0.0f && q < QMIN ? QMIN : q;
+        }
+        store_upto((T*)t.p + e, n, p);
+        store8((uint8_t*)t.m + e, n, pack8(m));
+        store8((uint8_t*)t.v + e, n, pack8(v));
+        if (lane == 0) t.ms[b] = sm, t.vs[b] = sv;
+    }
+}
+
+// partial[blockIdx.x] = sum g^2 over `chunk` elements of a tensor, in double
+template <typename T>
+__global__ void __launch_bounds__(256) k_sumsq(Group a, int64_t chunk, double* partial) {
+    __shared__ double s[4];
+    const int k = tensor_of(a, blockIdx.x);
+    const T* g = (const T*)a.t[k].g;
+    const int64_t e0 = (int64_t)(blockIdx.x - a.first[k]) * chunk;
+    const int64_t e1 = e0 + chunk < a.t[k].n ? e0 + chunk : a.t[k].n;
+    double x = 0.0;
+    for (int64_t e = e0 + threadIdx.x * 4; e < e1; e += 1024) {
+        float f[4];
+        load_upto(g + e, e1 - e, 0.0f, f);
+#pragma unroll
+        for (int j = 0; j < 4; j++) x = fma((double)f[j], (double)f[j], x);
+    }
+    for (int o = 32; o >= 1; o >>= 1) x += __shfl_xor(x, o);
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = x;
+    __syncthreads();
+    if (threadIdx.x == 0) partial[blockIdx.x] = s[0] + s[1] + s[2] + s[3];
+}
+
+// norm and coefficient from the partial sums: one block, a fixed order
+__global__ void __launch_bounds__(1024) k_clip_coef(const double* partial, int64_t n, float max_norm, float* norm, float* coef) {
+    __shared__ double s[16];
+    double x = 0.0;
+    for (int64_t i = threadIdx.x; i < n; i += 1024) x += partial[i];
+    for (int o = 32; o >= 1; o >>= 1) x += __shfl_xor(x, o);
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = x;
+    __syncthreads();
+    if (threadIdx.x) return;
+    x = 0.0;
+    for (int w = 0; w < 16; w++) x += s[w];
+    const float total = (float)sqrt(x), c = max_norm / (total + 1e-6f);
+    if (norm) *norm = total;
+    *coef = c < 1.0f || c != c ? c : 1.0f;  // (a NaN norm reaches every gradient, as in clip_grad_norm_)
+}
+
+// what follows from a step count (and a learning rate) on the device: dyn = {step_size, bc2_sqrt, keep}
+__global__ void __launch_bounds__(64) k_count_step(float* step, const float* lr_dev, double lr, double b1, double b2, double wd,
+                                                   float* dyn) {
+    if (threadIdx.x) return;
+    const double t = (double)*step + 1.0, rate = lr_dev ? (double)*lr_dev : lr;
+    *step = (float)t;
+    dyn[0] = (float)(rate / (1.0 - pow(b1, t)));
+    dyn[1] = (float)sqrt(1.0 - pow(b2, t));
+    dyn[2] = (float)(1.0 - rate * wd);
+}
+
+// elements a block of k_sumsq takes: about 4096 blocks in all
+int64_t norm_chunk(int64_t total) { return cdiv(cdiv(total, 4096), CHUNK) * CHUNK; }
+
+int64_t norm_parts(int32_t count, const int64_t* numel) {
+    int64_t total = 0, parts = 0;
+    for (int i = 0; i < count; i++) total += numel[i];
+    if (total == 0) return 0;
+    const int64_t chunk = norm_chunk(total);
+    for (int i = 0; i < count; i++) parts += cdiv(numel[i], chunk);
+    return parts;
+}
+
+const char* bad_tensors(const char* who, int32_t count, const void* const* grads, const int64_t* numel, const int32_t* dtypes,
+                        int64_t& total) {
+    static thread_local char msg[160];
+    total = 0;
+    if (count < 0 || (count && (!grads || !numel || !dtypes))) {
+        snprintf(msg, sizeof msg, "%s: null argument", who);
+        return msg;
+    }
+    for (int i = 0; i < count; i++) {
+        if (!dtype_ok(dtypes[i]) || numel[i] < 0 || numel[i] > ((int64_t)1 << 40) || (numel[i] && !grads[i])) {
+            snprintf(msg, sizeof msg, "%s: tensor %d: type %d, %lld elements%s", who, i, dtypes[i], (long long)numel[i],
+                     grads[i] ? "" : ", no gradient");
+            return msg;
+        }
+        total += numel[i];
+    }
+    if (cdiv(total, CHUNK) + count > INT32_MAX) {
+        snprintf(msg, sizeof msg, "%s: %lld elements", who, (long long)total);
+        return msg;
+    }
+    return nullptr;
+}
+
+// tensors of one type, up to MAX_TENSORS at a time: fill(i) makes the i-th, go(type, group, blocks) launches
+template <typename Fill, typename Go>
+void each_group(int32_t count, const int64_t* numel, const int32_t* dtypes, int64_t chunk, Fill fill, Go go) {
+    for (int type = EC_F32; type <= EC_F16; type++) {
+        Group a;
+        a.count = 0;
+        uint32_t blocks = 0;
+        for (int i = 0; i < count; i++) {
+            if (!numel[i] || dtypes[i] != type) continue;
+            if (a.count == MAX_TENSORS) {
+                a.first[a.count] = blocks;
+                go(type, a, blocks);
+                a.count = 0;
+                blocks = 0;
+            }
+            a.t[a.count] = fill(i);
+            a.first[a.count++] = blocks;
+            blocks += (uint32_t)cdiv(numel[i], chunk);
+        }
+        if (a.count) {
+            a.first[a.count] = blocks;
+            go(type, a, blocks);
+        }
+    }
+}
+
+}  // namespace
+
+extern "C" int64_t ec_grad_clip_workspace(int32_t count, const int64_t* numel) {
+    if (count < 1 || !numel) return 0;
+    for (int i = 0; i < count; i++)
+        if (numel[i] < 0) return 0;
+    return 8 * norm_parts(count, numel);
+}
+
+extern "C" int ec_grad_clip_coef(int32_t count, const void* const* grads, const int64_t* numel, const int32_t* dtypes,
+                                 double max_norm, float* norm, float* coef, void* work, int64_t work_bytes, void* stream) {
+    int64_t total;
+    if (const char* m = bad_tensors("ec_grad_clip_coef", count, grads, numel, dtypes, total)) return ec::fail(EC_EINVAL, "%s", m);
+    if (!coef || !(max_norm > 0)) return ec::fail(EC_EINVAL, "ec_grad_clip_coef: no output, or a largest norm of %g", max_norm);
+    const int64_t need = ec_grad_clip_workspace(count, numel);
+    if (work_bytes < need || (need && (!work || (uintptr_t)work % 8)))
+        return ec::fail(EC_EINVAL, "ec_grad_clip_coef: workspace of %lld bytes (%lld are needed, at a multiple of 8)",
+                        (long long)work_bytes, (long long)need);
+    const hipStream_t st = (hipStream_t)stream;
+    const int64_t chunk = total ? norm_chunk(total) : CHUNK;
+    double* partial = (double*)work;
+    each_group(count, numel, dtypes, chunk,
+               [&](int i) {
+                   Tensor t{};
+                   t.g = grads[i], t.n = numel[i];
+                   return t;
+               },
+               [&](int type, const Group& a, uint32_t blocks) {
+                   if (type == EC_F32) hipLaunchKernelGGL(k_sumsq<float>, dim3(blocks), dim3(256), 0, st, a, chunk, partial);
+                   if (type == EC_BF16) hipLaunchKernelGGL(k_sumsq<bf16>, dim3(blocks), dim3(256), 0, st, a, chunk, partial);
+                   if (type == EC_F16) hipLaunchKernelGGL(k_sumsq<f16>, dim3(blocks), dim3(256), 0, st, a, chunk, partial);
+                   partial += blocks;
+               });
+    hipLaunchKernelGGL(k_clip_coef, dim3(1), dim3(1024), 0, st, (const double*)work, (int64_t)(partial - (double*)work),
+                       (float)max_norm, norm, coef);
+    EC_HIP(hipGetLastError());
+    return EC_OK;
+}
+
+extern "C" int ec_adamw_step(int32_t count, void* const* params, const void* const* grads, void* const* exp_avg,
+                             void* const* exp_avg_sq, float* const* exp_avg_scale, float* const* exp_avg_sq_scale,
+                             const int64_t* numel, const int32_t* dtypes, int32_t state_bits, const float* coef, double step_host,
+                             float* step_dev, float* dyn, double lr, const float* lr_dev, double beta1, double beta2, double eps,
+                             double weight_decay, void* stream) {
+    int64_t total;
+    if (const char* m = bad_tensors("ec_adamw_step", count, grads, numel, dtypes, total)) return ec::fail(EC_EINVAL, "%s", m);
+    const bool q = state_bits == 8;
+    if ((state_bits != 32 && !q) || (count && (!params || !exp_avg || !exp_avg_sq || (q && (!exp_avg_scale || !exp_avg_sq_scale)))))
+        return ec::fail(EC_EINVAL, "ec_adamw_step: null argument, or states of %d bits (32, or 8 with scales)", state_bits);
+    for (int i = 0; i < count; i++)
+        if (numel[i] && (!params[i] || !exp_avg[i] || !exp_avg_sq[i] || (q && (!exp_avg_scale[i] || !exp_avg_sq_scale[i]))))
+            return ec::fail(EC_EINVAL, "ec_adamw_step: tensor %d: null pointer", i);
+    if (!(lr >= 0) || !(beta1 >= 0 && beta1 < 1) || !(beta2 >= 0 && beta2 < 1) || !(eps >= 0) || !(weight_decay >= 0))
+        return ec::fail(EC_EINVAL, "ec_adamw_step: lr %g, betas %g and %g, eps %g, weight decay %g", lr, beta1, beta2, eps, weight_decay);
+    if (step_dev ? !dyn : (!(step_host >= 1.0) || lr_dev))
+        return ec::fail(EC_EINVAL, "ec_adamw_step: step count %g (from 1 on, or one on the device, with scratch)", step_host);
+    if (total == 0 && !step_dev) return EC_OK;
+    const hipStream_t st = (hipStream_t)stream;
+    Hyper h{};
+    h.omb1 = (float)(1.0 - beta1), h.b2 = (float)beta2, h.omb2 = (float)(1.0 - beta2), h.eps = (float)eps;
+    h.coef = coef, h.dyn = step_dev ? dyn : nullptr;
+    if (step_dev) {
+        hipLaunchKernelGGL(k_count_step, dim3(1), dim3(64), 0, st, step_dev, lr_dev, lr, beta1, beta2, weight_decay, dyn);
+    } else {
+        h.step_size = (float)(lr / (1.0 - pow(beta1, step_host)));
+        h.bc2_sqrt = (float)sqrt(1.0 - pow(beta2, step_host));
+        h.keep = (float)(1.0 - lr * weight_decay);
+    }
+    each_group(count, numel, dtypes, CHUNK,
+               [&](int i) {
+                   return Tensor{params[i], exp_avg[i], exp_avg_sq[i], grads[i], q ? exp_avg_scale[i] : nullptr,
+                                 q ? exp_avg_sq_scale[i] : nullptr, numel[i]};
+               },
+               [&](int type, const Group& a, uint32_t blocks) {
+                   const dim3 g(blocks), b(256);
+                   if (q) {
+                       if (type == EC_F32) hipLaunchKernelGGL(k_adamw8<float>, g, b, 0, st, a, h);
+                       if (type == EC_BF16) hipLaunchKernelGGL(k_adamw8<bf16>, g, b, 0, st, a, h);
+                       if (type == EC_F16) hipLaunchKernelGGL(k_adamw8<f16>, g, b, 0, st, a, h);
+                   } else {
+                       if (type == EC_F32) hipLaunchKernelGGL(k_adamw32<float>, g, b, 0, st, a, h);
+                       if (type == EC_BF16) hipLaunchKernelGGL(k_adamw32<bf16>, g, b, 0, st, a, h);
+                       if (type == EC_F16) hipLaunchKernelGGL(k_adamw32<f16>, g, b, 0, st, a, h);
+                   }
+               });
+    EC_HIP(hipGetLastError());
+    return EC_OK;
+}

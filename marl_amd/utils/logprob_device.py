@@ -1,0 +1,139 @@
+"""Host side of ec_token_logprobs_fwd / _bwd (include/marl_amd.h): log-probs of given tokens (or actions) under
+softmax(logits), the entropy, and the likeliest alternatives, for any number of tokens.
+
+`token_logprobs` is the autograd form; `token_logprobs_fwd` and `token_logprobs_bwd` are the two passes by hand, for update
+steps that keep no autograd graph and for recording into a HIP graph."""
+from collections import namedtuple
+
+import torch as th
+
+from marl_amd import _abi
+from marl_amd.utils.mlp_device import _p, _stream
+from marl_amd.utils.norm_device import need_device, need_dtype, refuse_capture
+
+MAX_TOP = 64  # EC_TOKEN_LOGPROBS_MAX_TOP
+
+TokenLogprobs = namedtuple("TokenLogprobs", "logp entropy top_logp top_index lse")
+
+
+def _layout(t, vocab):
+    """(tensor, inner, outer stride, inner stride): the rows of t [..., vocab] as [outer, inner] of them, a view where the
+    strides allow one (a slice of steps out of [batch, steps, vocab] does)"""
+    lead = t.shape[:-1]
+    inner = lead[-1] if len(lead) >= 2 else 1
+    outer = lead[:-1].numel() if len(lead) >= 2 else lead.numel()
+    t = t.reshape(outer, inner, vocab)
+    if vocab > 1 and t.stride(2) != 1:
+        t = t.contiguous()
+    return t, max(1, inner), t.stride(0), t.stride(1)
+
+
+def _inputs(who, logits, tokens, avail):
+    """checked arguments, as both passes of the C entry points take them first"""
+    dev = need_device(who, logits, tokens, avail)
+    code = need_dtype(who, logits)
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError("%s: logits of shape %s" % (who, tuple(logits.shape)))
+    if tokens.shape != logits.shape[:-1]:
+        raise ValueError("%s: tokens of shape %s for logits of shape %s" % (who, tuple(tokens.shape), tuple(logits.shape)))
+    if tokens.dtype not in (th.int64, th.int32):
+        raise TypeError("%s: tokens of type %s" % (who, tokens.dtype))
+    vocab = logits.shape[-1]
+    kind = 0
+    if avail is not None:
+        if avail.is_floating_point() or avail.is_complex():
+            raise TypeError("%s: avail of type %s (bool or integers)" % (who, avail.dtype))
+        try:
+            avail = avail.expand(logits.shape)
+        except RuntimeError:
+            raise ValueError("%s: avail of shape %s for logits of shape %s" % (who, tuple(avail.shape), tuple(logits.shape))) from None
+        if avail.dtype not in (th.bool, th.uint8, th.int8, th.int32):
+            avail = avail != 0
+        kind = 2 if avail.dtype == th.int32 else 1
+        avail, _, ao, ai = _layout(avail, vocab)
+    else:
+        ao = ai = 0
+    logits, inner, so, si = _layout(logits, vocab)
+    tokens = tokens.to(th.int64).contiguous()
+    # (the tensors are kept by the caller until the launch is made)
+    head = (_p(logits), inner, so, si, _p(tokens), _p(avail), kind, ao, ai, code, tokens.numel(), vocab)
+    return dev, head, (logits, tokens, avail)
+
+
+def token_logprobs_fwd(logits, tokens, avail=None, top_k=0):
+    """TokenLogprobs(logp, entropy, top_logp, top_index, lse) for logits [..., V] (float32, bfloat16, float16; any V) and
+    tokens [...] (int64 or int32).  avail (bool or integers, broadcastable to logits; the env's avail_actions): entries
+    with 0 are excluded, whatever their logit holds; so are logits of -inf.
+      logp [...]: log-prob of the token; 0 for a token below 0 (a padded row), NaN for one >= V, -inf for an excluded one
+      entropy [...] of the distribution
+      top_logp, top_index [..., top_k] (top_k <= 64; None for 0): the likeliest entries, equal ones by index; -inf and -1
+        where there are fewer
+      lse [..., 2]: largest logit and log-sum-exp above it, for token_logprobs_bwd
+    all float32 (top_index int64).  A row with everything excluded has logp -inf, entropy 0 and gradient 0."""
+    dev, head, keep = _inputs("token_logprobs_fwd", logits, tokens, avail)
+    top_k = int(top_k)
+    if not 0 <= top_k <= MAX_TOP:
+        raise ValueError("token_logprobs_fwd: top_k %d (0 .. %d)" % (top_k, MAX_TOP))
+    lead = tuple(tokens.shape)
+    rows, vocab, code = head[-2], head[-1], head[-3]
+    f32 = lambda *s: th.empty(s, dtype=th.float32, device=dev)
+    logp, entropy, lse = f32(*lead), f32(*lead), f32(*lead, 2)
+    top_logp = f32(*lead, top_k) if top_k else None
+    top_index = th.empty(lead + (top_k,), dtype=th.int64, device=dev) if top_k else None
+    L = _abi.lib()
+    nbytes = L.ec_token_logprobs_workspace(rows, vocab, code, top_k)
+    work = th.empty(nbytes, dtype=th.uint8, device=dev) if nbytes else None
+    with th.cuda.device(dev):
+        _abi.check(L.ec_token_logprobs_fwd(*head, top_k, _p(logp), _p(entropy), _p(lse), _p(top_logp), _p(top_index), _p(work),
+                                           nbytes, _stream(dev)), "ec_token_logprobs_fwd")
+    del keep
+    return TokenLogprobs(logp, entropy, top_logp, top_index, lse)
+
+
+def token_logprobs_bwd(logits, tokens, lse, entropy, dlogp=None, dentropy=None, avail=None):
+    """d loss / d logits [..., V], contiguous and of logits' type, for dlogp = d loss / d logp and dentropy = d loss / d
+    entropy [...] (None: 0), with token_logprobs_fwd's inputs and its lse and entropy:
+      dlogp (1[v = token] - p_v) - dentropy p_v (log p_v + entropy),
+    0 at excluded entries; a token below 0 takes no dlogp."""
+    dev, head, keep = _inputs("token_logprobs_bwd", logits, tokens, avail)
+    need_device("token_logprobs_bwd", logits, lse, entropy, dlogp, dentropy)
+    small = []
+    for name, t, shape in (("lse", lse, tokens.shape + (2,)), ("entropy", entropy, tokens.shape), ("dlogp", dlogp, tokens.shape),
+                           ("dentropy", dentropy, tokens.shape)):
+        if t is not None and (t.shape != shape or t.dtype != th.float32):
+            raise ValueError("token_logprobs_bwd: %s is float32 of shape %s, not %s %s" % (name, tuple(shape), t.dtype, tuple(t.shape)))
+        small.append(t.contiguous() if t is not None else None)
+    out = th.empty(logits.shape, dtype=logits.dtype, device=dev)
+    with th.cuda.device(dev):
+        _abi.check(_abi.lib().ec_token_logprobs_bwd(*head, *[_p(t) for t in small], _p(out), _stream(dev)),
+                   "ec_token_logprobs_bwd")
+    del keep
+    return out
+
+
+class _TokenLogprobsFn(th.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, avail, top_k):
+        f = token_logprobs_fwd(logits, tokens, avail, top_k)
+        ctx.save_for_backward(logits, tokens, avail, f.lse, f.entropy)
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(*[t for t in (f.top_logp, f.top_index, f.lse) if t is not None])
+        return tuple(f)
+
+    @staticmethod
+    @th.autograd.function.once_differentiable
+    def backward(ctx, dlogp, dentropy, *_):
+        logits, tokens, avail, lse, entropy = ctx.saved_tensors
+        if dlogp is None and dentropy is None:
+            return None, None, None, None
+        return token_logprobs_bwd(logits, tokens, lse, entropy, dlogp, dentropy, avail), None, None, None
+
+
+def token_logprobs(logits, tokens, avail=None, top_k=0):
+    """token_logprobs_fwd with gradients of logp and entropy for logits (the alternatives and lse carry none).  Not while a
+    HIP graph is recorded (RuntimeError, unless logits need no gradient): record token_logprobs_fwd and token_logprobs_bwd
+    there."""
+    if th.is_grad_enabled() and logits.requires_grad:
+        refuse_capture("token_logprobs", "token_logprobs_fwd and token_logprobs_bwd")
+        return TokenLogprobs(*_TokenLogprobsFn.apply(logits, tokens, avail, top_k))
+    return token_logprobs_fwd(logits, tokens, avail, top_k)

@@ -1,11 +1,18 @@
-"""Host side of ec_adam_clip_step (include/marl_amd.h): `clip_grad_norm_` + `Adam.step()` of up to four small networks
-in one launch.  The optimiser objects stay the owners of their state (exp_avg, exp_avg_sq, step), so state_dicts and
-checkpoints are torch's; the kernel updates those tensors in place."""
+"""Host side of the optimiser kernels (include/marl_amd.h).
+
+ec_adam_clip_step: `clip_grad_norm_` + `Adam.step()` of up to four small networks in one launch.  The optimiser objects stay
+the owners of their state (exp_avg, exp_avg_sq, step), so state_dicts and checkpoints are torch's; the kernel updates those
+tensors in place.
+
+ec_grad_clip_coef, ec_adamw_step: AdamW over any number of tensors of any size, moments in 32 or 8 bits (`AdamW`, and
+`clip_coef` / `adamw_step` on lists of tensors)."""
 import ctypes as C
 
 import torch as th
 
 from marl_amd import _abi
+from marl_amd.utils.mlp_device import _p, _stream
+from marl_amd.utils.norm_device import DTYPES
 
 MAX_NETS, MAX_TENSORS = 4, 16
 
@@ -88,3 +95,248 @@ def clip_adam_step(optimizers, max_norm):
     for opt in optimizers:
         opt._opt_called = True  # (what an lr_scheduler looks at to tell that step() came first)
     return True
+
+
+# ---- AdamW over many tensors of any size (ec_grad_clip_coef, ec_adamw_step) ----
+QBLOCK = 256                      # elements that share a scale of the 8-bit states
+STATE8 = th.float8_e4m3fn
+
+
+def scale_count(p):
+    """scales of one 8-bit state of p"""
+    return -(-p.numel() // QBLOCK)
+
+
+def _pointers(who, name, tensors, dev, numel, dtypes=None, same=None):
+    """addresses of contiguous tensors on dev: element counts as `numel`, types as the set `dtypes` or as the list `same`"""
+    if len(tensors) != len(numel):
+        raise ValueError("%s: %d %s for %d tensors" % (who, len(tensors), name, len(numel)))
+    out = []
+    for i, t in enumerate(tensors):
+        if t.device != dev or t.numel() != numel[i] or not t.is_contiguous() or t.dtype not in (dtypes or (same[i].dtype,)):
+            raise ValueError("%s: %s[%d] is %s %s on %s%s; %d contiguous elements of %s on %s are needed"
+                             % (who, name, i, t.dtype, tuple(t.shape), t.device, "" if t.is_contiguous() else ", not contiguous",
+                                numel[i], "/".join(map(str, dtypes or (same[i].dtype,))), dev))
+        out.append(t.data_ptr())
+    return out
+
+
+def _device_of(who, tensors):
+    if not tensors:
+        raise ValueError("%s: no tensors" % who)
+    dev = tensors[0].device
+    if dev.type != "cuda":
+        raise RuntimeError("%s needs device tensors: marl_amd has no CPU fallback" % who)
+    return dev
+
+
+def clip_coef(grads, max_norm):
+    """(norm, coef) of the gradients in the list (float32, bfloat16, float16): their total 2-norm and clip_grad_norm_'s factor
+    min(1, max_norm / (norm + 1e-6)), as float32 scalars on the device.  The gradients are only read: hand coef to
+    adamw_step.  The sums are double and in a fixed order."""
+    grads = list(grads)
+    dev = _device_of("clip_coef", grads)
+    if not max_norm > 0:
+        raise ValueError("clip_coef: max_norm %r" % (max_norm,))
+    numel = [g.numel() for g in grads]
+    G = _pointers("clip_coef", "grads", grads, dev, numel, dtypes=tuple(DTYPES))
+    n = len(grads)
+    numel = (C.c_int64 * n)(*numel)
+    L = _abi.lib()
+    nbytes = L.ec_grad_clip_workspace(n, numel)
+    work = th.empty(nbytes // 8, dtype=th.float64, device=dev)
+    norm, coef = th.empty(2, dtype=th.float32, device=dev).unbind(0)
+    with th.cuda.device(dev):
+        _abi.check(L.ec_grad_clip_coef(n, (C.c_void_p * n)(*G), numel, (C.c_int32 * n)(*[DTYPES[g.dtype] for g in grads]),
+                                       C.c_double(max_norm), _p(norm), _p(coef), _p(work), nbytes, _stream(dev)),
+                   "ec_grad_clip_coef")
+    return norm, coef
+
+
+def adamw_step(params, grads, exp_avg, exp_avg_sq, exp_avg_scale=None, exp_avg_sq_scale=None, *, step, lr, betas=(0.9, 0.999),
+               eps=1e-8, weight_decay=1e-2, max_norm=None, coef=None):
+    """One AdamW step over lists of contiguous tensors on one device, in place:
+      m = m + (g - m)(1 - b1);  v = v b2 + (1 - b2) g^2
+      p = p (1 - lr weight_decay) - lr / (1 - b1^step) m / (sqrt(v) / sqrt(1 - b2^step) + eps)
+    params, grads: float32, bfloat16 or float16 (grads[i] as params[i]); the arithmetic is float32, rounded once to a
+    parameter's type.
+    States in 32 bits: exp_avg, exp_avg_sq float32.  In 8 bits: exp_avg, exp_avg_sq float8_e4m3fn with exp_avg_scale,
+    exp_avg_sq_scale [scale_count(p)] float32, where exp_avg * scale is m and exp_avg_sq * scale is sqrt(v), one scale for each
+    256 consecutive elements.
+    step: this step's count, from 1 on; or a float32 scalar on the device (what a HIP graph needs), which the call advances
+    first, and with which lr may be such a scalar too.
+    max_norm: the gradients enter scaled by clip_coef(grads, max_norm)'s coef, and its norm is returned; coef: scaled by that
+    device scalar (one clip over several calls).  The gradients are only read."""
+    who = "adamw_step"
+    dev = _device_of(who, params)
+    n = len(params)
+    numel = [p.numel() for p in params]
+    P = _pointers(who, "params", params, dev, numel, dtypes=tuple(DTYPES))
+    live = [a for a, k in zip(P, numel) if k]
+    if len(set(live)) != len(live):
+        raise ValueError("adamw_step: the same parameter twice")
+    G = _pointers(who, "grads", grads, dev, numel, same=params)
+    bits = 8 if exp_avg_scale is not None else 32
+    st = (STATE8,) if bits == 8 else (th.float32,)
+    M = _pointers(who, "exp_avg", exp_avg, dev, numel, dtypes=st)
+    V = _pointers(who, "exp_avg_sq", exp_avg_sq, dev, numel, dtypes=st)
+    MS = VS = None
+    if bits == 8:
+        if exp_avg_sq_scale is None:
+            raise ValueError("adamw_step: exp_avg_scale without exp_avg_sq_scale")
+        blocks = [-(-k // QBLOCK) for k in numel]
+        MS = (C.c_void_p * n)(*_pointers(who, "exp_avg_scale", exp_avg_scale, dev, blocks, dtypes=(th.float32,)))
+        VS = (C.c_void_p * n)(*_pointers(who, "exp_avg_sq_scale", exp_avg_sq_scale, dev, blocks, dtypes=(th.float32,)))
+    elif exp_avg_sq_scale is not None:
+        raise ValueError("adamw_step: exp_avg_sq_scale without exp_avg_scale")
+    for name, t in (("step", step), ("lr", lr), ("coef", coef)):
+        if isinstance(t, th.Tensor) and (t.device != dev or t.dtype != th.float32 or t.numel() != 1):
+            raise ValueError("adamw_step: %s on the device is one float32 value on %s" % (name, dev))
+    dyn = None
+    if isinstance(step, th.Tensor):
+        dyn = th.empty(3, dtype=th.float32, device=dev)
+    elif isinstance(lr, th.Tensor):
+        raise ValueError("adamw_step: a learning rate on the device needs a step count there")
+    elif not step >= 1:
+        raise ValueError("adamw_step: step %r (from 1 on)" % (step,))
+    elif th.cuda.is_current_stream_capturing():
+        raise RuntimeError("adamw_step: a recorded HIP graph would repeat step %r; pass a step count on the device" % (step,))
+    b1, b2 = (float(b) for b in betas)
+    if not (0 <= b1 < 1 and 0 <= b2 < 1 and eps >= 0 and weight_decay >= 0 and (isinstance(lr, th.Tensor) or lr >= 0)):
+        raise ValueError("adamw_step: lr %r, betas %r, eps %r, weight_decay %r" % (lr, betas, eps, weight_decay))
+    norm = None
+    if max_norm is not None:
+        if coef is not None:
+            raise ValueError("adamw_step: max_norm and coef")
+        norm, coef = clip_coef(grads, max_norm)
+    vps = lambda xs: (C.c_void_p * n)(*xs)
+    on_dev = dyn is not None
+    with th.cuda.device(dev):
+        _abi.check(_abi.lib().ec_adamw_step(
+            n, vps(P), vps(G), vps(M), vps(V), MS, VS, (C.c_int64 * n)(*numel), (C.c_int32 * n)(*[DTYPES[p.dtype] for p in params]),
+            bits, _p(coef), C.c_double(0.0 if on_dev else float(step)), _p(step if on_dev else None), _p(dyn),
+            C.c_double(0.0 if isinstance(lr, th.Tensor) else float(lr)), _p(lr if isinstance(lr, th.Tensor) else None),
+            C.c_double(b1), C.c_double(b2), C.c_double(eps), C.c_double(weight_decay), _stream(dev)), "ec_adamw_step")
+    th.autograd.graph.increment_version(params)  # (written through raw pointers: autograd has to know)
+    return norm
+
+
+class AdamW(th.optim.Optimizer):
+    """torch.optim.AdamW's update (decoupled weight decay, no amsgrad) over all tensors in a few launches, with moments in 32
+    bits or in 8 (state_bits, per group), and clip_grad_norm_ over all groups on the way (max_norm; the gradients stay as
+    they are; `last_norm` holds the norm).  Parameters: contiguous, on one device, float32, bfloat16 or float16.
+
+    State: state[p] = {"step", "exp_avg", "exp_avg_sq"} and, with 8 bits, {"exp_avg_scale", "exp_avg_sq_scale"} (see
+    adamw_step); state_dict / load_state_dict keep their types.  capturable: the step count lives on the device, one for the
+    parameters of a group, and lr may be a device scalar -- for steps recorded into a HIP graph."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, max_norm=None, state_bits=32,
+                 capturable=False):
+        if max_norm is not None and not max_norm > 0:
+            raise ValueError("AdamW: max_norm %r" % (max_norm,))
+        self.max_norm, self.last_norm = max_norm, None
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
+                                      capturable=capturable))
+
+    def __getstate__(self):  # (torch's names three attributes: what a copy or a pickle keeps)
+        return dict(super().__getstate__(), max_norm=self.max_norm, last_norm=None)
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        g = self.param_groups[-1]
+        try:
+            if g["state_bits"] not in (8, 32):
+                raise ValueError("AdamW: state_bits %r (8 or 32)" % (g["state_bits"],))
+            if isinstance(g["lr"], th.Tensor) and not g["capturable"]:
+                raise ValueError("AdamW: a learning rate on the device needs capturable=True")
+            b1, b2 = g["betas"]
+            if not (0 <= b1 < 1 and 0 <= b2 < 1 and g["eps"] >= 0 and g["weight_decay"] >= 0
+                    and (isinstance(g["lr"], th.Tensor) or g["lr"] >= 0)):
+                raise ValueError("AdamW: lr %r, betas %r, eps %r, weight_decay %r" % (g["lr"], g["betas"], g["eps"], g["weight_decay"]))
+            dev = self.param_groups[0]["params"][0].device
+            for p in g["params"]:
+                if p.dtype not in DTYPES or not p.is_contiguous() or p.device != dev:
+                    raise ValueError("AdamW: a parameter of type %s, strides %s on %s (contiguous float32, bfloat16 or float16 on one "
+                                     "device)" % (p.dtype, p.stride(), p.device))
+        except ValueError:
+            self.param_groups.pop()
+            raise
+
+    def _init(self, group, p):
+        if th.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW: the first step of a parameter makes its state; take it before a HIP graph is recorded")
+        st = self.state[p]
+        kw = dict(device=p.device)
+        if group["state_bits"] == 8:
+            for k in ("exp_avg", "exp_avg_sq"):
+                st[k] = th.zeros(p.shape, dtype=th.uint8, **kw).view(STATE8)
+                st[k + "_scale"] = th.zeros(scale_count(p), dtype=th.float32, **kw)
+        else:
+            st["exp_avg"] = th.zeros(p.shape, dtype=th.float32, **kw)
+            st["exp_avg_sq"] = th.zeros(p.shape, dtype=th.float32, **kw)
+        if not group["capturable"]:
+            st["step"] = 0
+        else:  # one count for the group
+            have = [self.state[q]["step"] for q in group["params"] if "step" in self.state.get(q, ())]
+            st["step"] = have[0] if have else th.zeros((), dtype=th.float32, **kw)
+        return st
+
+    @th.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with th.enable_grad():
+                loss = closure()
+        calls, every = [], []
+        for group in self.param_groups:
+            by_step = {}
+            for p in group["params"]:
+                g = p.grad
+                if g is None:
+                    continue
+                if g.is_sparse:
+                    raise RuntimeError("AdamW: sparse gradients are not supported")
+                if not g.is_contiguous():
+                    g = g.contiguous()
+                st = self.state[p] if p in self.state else self._init(group, p)
+                step = st["step"]
+                by_step.setdefault(None if group["capturable"] else step, []).append((p, g, st))
+                every.append(g)
+            calls += [(group, step, ts) for step, ts in by_step.items()]
+        if not every:
+            return loss
+        coef = None
+        if self.max_norm is not None:
+            self.last_norm, coef = clip_coef(every, self.max_norm)
+        for group, step, ts in calls:
+            cols = lambda k: [st[k] for _, _, st in ts]
+            scales = [cols("exp_avg_scale"), cols("exp_avg_sq_scale")] if group["state_bits"] == 8 else []
+            adamw_step([p for p, _, _ in ts], [g for _, g, _ in ts], cols("exp_avg"), cols("exp_avg_sq"), *scales,
+                       step=ts[0][2]["step"] if step is None else step + 1, lr=group["lr"], betas=group["betas"], eps=group["eps"],
+                       weight_decay=group["weight_decay"], coef=coef)
+            if step is not None:  # (after the call: a refused one has counted nothing)
+                for _, _, st in ts:
+                    st["step"] = step + 1
+        return loss
+
+    def load_state_dict(self, state_dict):
+        """torch's load casts states to their parameter's type: here they keep their own, and a capturable group gets its one
+        step count back"""
+        super().load_state_dict(state_dict)
+        for saved, group in zip(state_dict["param_groups"], self.param_groups):
+            count = None
+            for i, p in zip(saved["params"], group["params"]):
+                if i not in state_dict["state"]:
+                    continue
+                st = self.state[p]
+                for k, v in state_dict["state"][i].items():
+                    if k == "step":
+                        if group["capturable"]:
+                            if count is None:
+                                count = th.as_tensor(float(v), dtype=th.float32).to(p.device)
+                            v = count
+                        else:
+                            v = int(v)
+                    else:
+                        v = v.detach().to(p.device, copy=True)
+                    st[k] = v
