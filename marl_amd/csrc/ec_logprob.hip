@@ -59,12 +59,14 @@ __device__ __forceinline__ Stat join(const Stat& a, const Stat& b) {
     return o;
 }
 
-__device__ __forceinline__ Stat wave_join(Stat a) {
+// the sets of W lanes as one, in all of them
+template <int W>
+__device__ __forceinline__ Stat lanes_join(Stat a) {
     Stat o;
-    o.m = lanes_max<64>(a.m);
+    o.m = lanes_max<W>(a.m);
     const float t = fmaxf((a.m - o.m) * LOG2E, -200.0f), f = __builtin_amdgcn_exp2f(t);
-    o.s2 = lanes_sum<64>((a.s2 + a.s1 * t) * f);
-    o.s1 = lanes_sum<64>(a.s1 * f);
+    o.s2 = lanes_sum<W>((a.s2 + a.s1 * t) * f);
+    o.s1 = lanes_sum<W>(a.s1 * f);
     return o;
 }
 
@@ -150,52 +152,61 @@ __device__ __forceinline__ float logit_at(const T* l, const char* av, int64_t c)
     return (float)l[c];
 }
 
-// what a row's statistics say, by the lanes of one wave
-template <typename T, int MASK>
-__device__ __forceinline__ void finish_row(const LpArgs& p, int64_t r, const Stat& s, const TopList& top) {
-    const int lane = threadIdx.x & 63;
-    const bool none = s.s1 == 0.0f;  // nothing but excluded entries
-    const float ln = none ? 0.0f : __builtin_amdgcn_logf(s.s1) * LN2;
-    if (lane == 0) {
-        if (p.lse) {
-            p.lse[2 * r] = none ? -INF : s.m;
-            p.lse[2 * r + 1] = ln;
-        }
-        if (p.entropy) p.entropy[r] = none ? 0.0f : ln - s.s2 * LN2 / s.s1;
-        if (p.logp) {
-            const int64_t t = p.tokens[r];
-            float v = 0.0f;
-            if (t >= p.vocab) {
-                v = NAN;
-            } else if (t >= 0) {
-                const float l = logit_at<T, MASK>(row_of<T>(p, r), MASK ? mask_of<MASK>(p, r) : nullptr, t);
-                v = none ? -INF : (l - s.m) - ln;
-            }
-            p.logp[r] = v;
-        }
+// log p of a row's token, whose logit is l
+__device__ __forceinline__ float logp_of(const LpArgs& p, int64_t token, float l, const Stat& s, float ln) {
+    if (token < 0) return 0.0f;
+    if (token >= p.vocab) return NAN;
+    return s.s1 == 0.0f ? -INF : (l - s.m) - ln;
+}
+__device__ __forceinline__ float log_s1(const Stat& s) { return s.s1 == 0.0f ? 0.0f : __builtin_amdgcn_logf(s.s1) * LN2; }
+
+// a row's lse, entropy and log-prob, by one lane (s1 = 0: nothing but excluded entries)
+__device__ __forceinline__ void write_row(const LpArgs& p, int64_t r, const Stat& s, float ln, float logp) {
+    const bool none = s.s1 == 0.0f;
+    if (p.lse) {
+        p.lse[2 * r] = none ? -INF : s.m;
+        p.lse[2 * r + 1] = ln;
     }
-    if (p.top_k && lane < p.top_k) {
-        float v = -INF;
-        int64_t at = -1;
-        if (!(s.s1 < INF)) {
-            v = NAN;  // a NaN or +inf among the entries
-        } else if (top.mine) {
-            v = (value_of((uint32_t)(top.mine >> 32)) - s.m) - ln;
-            at = (int64_t)(uint32_t)~(uint32_t)top.mine;
-        }
-        p.top_logp[r * p.top_k + lane] = v;
-        p.top_index[r * p.top_k + lane] = at;
+    if (p.entropy) p.entropy[r] = none ? 0.0f : ln - s.s2 * LN2 / s.s1;
+    if (p.logp) p.logp[r] = logp;
+}
+__device__ __forceinline__ void write_top(const LpArgs& p, int64_t r, int i, const Stat& s, float ln, uint64_t key) {
+    float v = -INF;
+    int64_t at = -1;
+    if (!(s.s1 < INF)) {
+        v = NAN;  // a NaN or +inf among the entries
+    } else if (key) {
+        v = (value_of((uint32_t)(key >> 32)) - s.m) - ln;
+        at = (int64_t)(uint32_t)~(uint32_t)key;
     }
+    p.top_logp[r * p.top_k + i] = v;
+    p.top_index[r * p.top_k + i] = at;
 }
 
-// a block of 256 threads per row, or per split of a row
-template <typename T, int MASK, bool TOP>
+// what a row's statistics say, by its W lanes (lane t of them); the alternatives by a whole wave
+template <typename T, int MASK>
+__device__ __forceinline__ void finish_row(const LpArgs& p, int64_t r, int t, const Stat& s, const TopList* top) {
+    const float ln = log_s1(s);
+    if (t == 0) {
+        const int64_t tok = p.tokens[r];
+        const float l = tok >= 0 && tok < p.vocab ? logit_at<T, MASK>(row_of<T>(p, r), MASK ? mask_of<MASK>(p, r) : nullptr, tok) : 0.0f;
+        write_row(p, r, s, ln, logp_of(p, tok, l, s, ln));
+    }
+    if (top && t < p.top_k) write_top(p, r, t, s, ln, top->mine);
+}
+
+// TPR threads a row: 16 or 64 (each row once), or a block of 256 per row or split of a row
+template <typename T, int MASK, bool TOP, int TPR>
 __global__ void __launch_bounds__(256) k_logp_fwd(LpArgs p) {
-    constexpr int V = 16 / sizeof(T);
+    constexpr int V = 16 / sizeof(T), W = TPR < 64 ? TPR : 64;
     __shared__ Stat s_stat[4];
-    __shared__ uint64_t s_top[TOP ? 4 : 1][MAX_TOP];
-    const int64_t r = blockIdx.x / p.splits;
-    const int split = (int)(blockIdx.x % p.splits), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __shared__ uint64_t s_top[TOP && TPR == 256 ? 4 : 1][MAX_TOP];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, t = threadIdx.x % TPR;
+    // (every thread makes every round: a group of rows past the last reads the last and writes nothing)
+    const int64_t r0 = TPR == 256 ? blockIdx.x / p.splits : (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+    const bool on = r0 < p.rows;
+    const int64_t r = on ? r0 : p.rows - 1;
+    const int split = TPR == 256 ? (int)(blockIdx.x % p.splits) : 0;
     const T* l = row_of<T>(p, r);
     const char* av = MASK ? mask_of<MASK>(p, r) : nullptr;
     const int64_t c0 = (int64_t)split * p.per_split;
@@ -203,12 +214,12 @@ __global__ void __launch_bounds__(256) k_logp_fwd(LpArgs p) {
     Stat s{-FLT_MAX, 0.0f, 0.0f};
     TopList top;
     top.clear(p.top_k);
-    for (int64_t b = c0; b < c1; b += 256 * V * U) {  // (the same rounds for every thread: the lists need whole waves)
+    for (int64_t b = c0; b < c1; b += TPR * V * U) {  // (the same rounds for every thread: the lists need whole waves)
         float f[U][V];
         float top_f = -INF;
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const int64_t c = b + (u * 256 + (int)threadIdx.x) * V;
+            const int64_t c = b + (u * TPR + t) * V;
             load_logits<T, MASK>(l, av, c, c1 - c, f[u]);
         }
 #pragma unroll
@@ -217,8 +228,8 @@ __global__ void __launch_bounds__(256) k_logp_fwd(LpArgs p) {
             for (int j = 0; j < V; j++) top_f = fmaxf(top_f, f[u][j]);
         const float m = fmaxf(s.m, top_f);
         {
-            const float t = fmaxf((s.m - m) * LOG2E, -200.0f), g = __builtin_amdgcn_exp2f(t);
-            s.s2 = (s.s2 + s.s1 * t) * g;
+            const float d = fmaxf((s.m - m) * LOG2E, -200.0f), g = __builtin_amdgcn_exp2f(d);
+            s.s2 = (s.s2 + s.s1 * d) * g;
             s.s1 *= g;
             s.m = m;
         }
@@ -226,9 +237,9 @@ __global__ void __launch_bounds__(256) k_logp_fwd(LpArgs p) {
         for (int u = 0; u < U; u++)
 #pragma unroll
             for (int j = 0; j < V; j++) {
-                const float t = (f[u][j] - m) * LOG2E, e = __builtin_amdgcn_exp2f(t);
+                const float d = (f[u][j] - m) * LOG2E, e = __builtin_amdgcn_exp2f(d);
                 s.s1 += e;
-                s.s2 = __builtin_fmaf(e, fmaxf(t, -200.0f), s.s2);  // (t = -inf: 0 * -inf)
+                s.s2 = __builtin_fmaf(e, fmaxf(d, -200.0f), s.s2);  // (d = -inf: 0 * -inf)
             }
         if (TOP) {
             // an entry equal to the k-th has the larger index, unless it is of this very batch: only larger ones count
@@ -237,23 +248,27 @@ __global__ void __launch_bounds__(256) k_logp_fwd(LpArgs p) {
                 for (int u = 0; u < U; u++)
 #pragma unroll
                     for (int j = 0; j < V; j++) {
-                        const int64_t c = b + (u * 256 + (int)threadIdx.x) * V + j;
+                        const int64_t c = b + (u * TPR + t) * V + j;
                         top.take(f[u][j] > -INF ? key_of(f[u][j], (uint32_t)c) : 0);
                     }
             }
         }
     }
-    s = wave_join(s);
+    s = lanes_join<W>(s);
+    if (TPR < 256) {
+        if (on) finish_row<T, MASK>(p, r, t, s, TOP ? &top : nullptr);
+        return;
+    }
     if (lane == 0) s_stat[wave] = s;
-    if (TOP && lane < p.top_k) s_top[wave][lane] = top.mine;
+    if (TOP && lane < p.top_k) s_top[TOP && TPR == 256 ? wave : 0][lane] = top.mine;
     __syncthreads();
     if (wave) return;
 #pragma unroll
     for (int w = 1; w < 4; w++) {
         s = join(s, s_stat[w]);
-        if (TOP) top.take(lane < p.top_k ? s_top[w][lane] : 0);
+        if (TOP) top.take(lane < p.top_k ? s_top[TOP && TPR == 256 ? w : 0][lane] : 0);
     }
-    if (p.splits == 1) return finish_row<T, MASK>(p, r, s, top);
+    if (p.splits == 1) return finish_row<T, MASK>(p, r, t, s, TOP ? &top : nullptr);
     char* to = p.work + (r * p.splits + split) * part_bytes(p.top_k);
     if (lane == 0) ((float*)to)[0] = s.m, ((float*)to)[1] = s.s1, ((float*)to)[2] = s.s2;
     if (TOP && lane < p.top_k) ((uint64_t*)(to + 16))[lane] = top.mine;
@@ -270,44 +285,164 @@ __global__ void __launch_bounds__(64) k_logp_join(LpArgs p) {
         const float* f = (const float*)(from + i * part_bytes(p.top_k));
         s = join(s, Stat{f[0], f[1], f[2]});
     }
-    s = wave_join(s);
+    s = lanes_join<64>(s);
     TopList top;
     top.clear(p.top_k);
     if (p.top_k)
         for (int i = 0; i < p.splits; i++)
             top.take(lane < p.top_k ? ((const uint64_t*)(from + i * part_bytes(p.top_k) + 16))[lane] : 0);
-    finish_row<T, MASK>(p, r, s, top);
+    finish_row<T, MASK>(p, r, lane, s, p.top_k ? &top : nullptr);
 }
 
-// a block per row and 256 * V * U columns of it
-template <typename T, int MASK>
+// what the gradient of a row's entries needs
+struct RowGrad {
+    float m, l2, h2, base, g;
+    int64_t tok;
+    bool none;
+};
+__device__ __forceinline__ RowGrad row_grad(const LpArgs& p, int64_t r) {
+    RowGrad o;
+    o.tok = p.tokens[r];
+    o.m = p.lse[2 * r];
+    o.l2 = p.lse[2 * r + 1] * LOG2E;
+    o.none = o.m == -INF;
+    o.g = !p.dlogp || o.tok < 0 ? 0.0f : o.tok >= p.vocab ? NAN : p.dlogp[r];
+    const float h = p.dentropy ? p.dentropy[r] : 0.0f;
+    o.h2 = h * LN2;
+    o.base = o.g + h * p.entropy_in[r];
+    return o;
+}
+__device__ __forceinline__ float entry_grad(const RowGrad& w, float l, int64_t c) {
+    const float t = (l - w.m) * LOG2E - w.l2;  // log2 p
+    float d = -__builtin_amdgcn_exp2f(t) * __builtin_fmaf(w.h2, fmaxf(t, -200.0f), w.base);
+    if (c == w.tok) d += w.g;
+    return w.none || l == -INF ? 0.0f : d;
+}
+
+// TPR threads a row: 16 or 64 for a whole row, or a block of 256 per TPR * V * U columns of a row
+template <typename T, int MASK, int TPR>
 __global__ void __launch_bounds__(256) k_logp_bwd(LpArgs p) {
     constexpr int V = 16 / sizeof(T);
-    const int64_t r = blockIdx.x / p.splits;
-    const int64_t c0 = (int64_t)(blockIdx.x % p.splits) * p.per_split;
+    const int64_t r = TPR == 256 ? blockIdx.x / p.splits : (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+    if (r >= p.rows) return;
+    const int64_t c0 = TPR == 256 ? (int64_t)(blockIdx.x % p.splits) * p.per_split : 0;
+    const int64_t c1 = TPR == 256 && c0 + p.per_split < p.vocab ? c0 + p.per_split : p.vocab;
     const T* l = row_of<T>(p, r);
     const char* av = MASK ? mask_of<MASK>(p, r) : nullptr;
     T* out = (T*)p.dlogits + r * p.vocab;
-    const int64_t tok = p.tokens[r];
-    const float m = p.lse[2 * r], ln = p.lse[2 * r + 1], ent = p.entropy_in[r];
-    const float g = !p.dlogp || tok < 0 ? 0.0f : tok >= p.vocab ? NAN : p.dlogp[r];
-    const float h = p.dentropy ? p.dentropy[r] : 0.0f;
-    const bool none = m == -INF;
-    const float l2 = ln * LOG2E, h2 = h * LN2, base = g + h * ent;
+    const RowGrad w = row_grad(p, r);
+    const int t = threadIdx.x % TPR;
+    for (int64_t b = c0; b < c1; b += TPR * V * U) {
+        float f[U][V];
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-        const int64_t c = c0 + (u * 256 + (int)threadIdx.x) * V;
-        if (c >= p.vocab) return;
+        for (int u = 0; u < U; u++) {
+            const int64_t c = b + (u * TPR + t) * V;
+            load_logits<T, MASK>(l, av, c, c1 - c, f[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int64_t c = b + (u * TPR + t) * V;
+#pragma unroll
+            for (int j = 0; j < V; j++) f[u][j] = entry_grad(w, f[u][j], c + j);
+            store_upto(out + c, c1 - c, f[u]);
+        }
+    }
+}
+
+// ---- few entries a row (the env's action sets): a lane per row ----
+// 256 rows are staged through LDS as fp32, excluded entries as -inf, at an odd stride (lanes that walk down their rows hit
+// different banks); packed rows come in and gradients leave 16 bytes a lane whatever the row's width.
+constexpr int FEW = 63;  // (64 KB of LDS a block)
+
+__device__ __forceinline__ int row_in(int i, int vocab, uint32_t by_vocab) {  // i / vocab
+    return vocab == 1 ? i : (int)__umulhi((uint32_t)i, by_vocab);
+}
+
+template <typename T, int MASK>
+__device__ __forceinline__ void stage_rows(const LpArgs& p, int64_t r0, int n, int stride, uint32_t by_vocab, bool packed, float* s) {
+    constexpr int V = 16 / sizeof(T);
+    if (packed) {  // the tile is one run of n * vocab elements, in logits and mask
+        const T* l = (const T*)p.logits + r0 * p.vocab;
+        const char* av = MASK ? (const char*)p.avail + r0 * p.vocab * (MASK == 1 ? 1 : 4) : nullptr;
+        const int all = n * p.vocab;
+        for (int i = threadIdx.x * V; i < all; i += 256 * V) {
+            float f[V];
+            load_logits<T, MASK>(l, av, i, all - i, f);
+            int row = row_in(i, p.vocab, by_vocab), col = i - row * p.vocab;
+#pragma unroll
+            for (int j = 0; j < V; j++) {
+                if (i + j < all) s[row * stride + col] = f[j];
+                if (++col == p.vocab) col = 0, row++;
+            }
+        }
+    } else {
+        for (int i = threadIdx.x; i < n * p.vocab; i += 256) {
+            const int row = row_in(i, p.vocab, by_vocab), col = i - row * p.vocab;
+            s[row * stride + col] = logit_at<T, MASK>(row_of<T>(p, r0 + row), MASK ? mask_of<MASK>(p, r0 + row) : nullptr, col);
+        }
+    }
+}
+
+template <typename T, int MASK>
+__global__ void __launch_bounds__(256) k_logp_few_fwd(LpArgs p, uint32_t by_vocab, bool packed) {
+    extern __shared__ float s_rows[];
+    const int64_t r0 = (int64_t)blockIdx.x * 256, r = r0 + threadIdx.x;
+    const int n = (int)(p.rows - r0 < 256 ? p.rows - r0 : 256), stride = p.vocab | 1;
+    stage_rows<T, MASK>(p, r0, n, stride, by_vocab, packed, s_rows);
+    __syncthreads();
+    if ((int)threadIdx.x >= n) return;
+    const float* l = s_rows + threadIdx.x * stride;
+    Stat s{-FLT_MAX, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int j = 0; j < p.vocab; j++) s.m = fmaxf(s.m, l[j]);
+#pragma unroll 4
+    for (int j = 0; j < p.vocab; j++) {
+        const float d = (l[j] - s.m) * LOG2E, e = __builtin_amdgcn_exp2f(d);
+        s.s1 += e;
+        s.s2 = __builtin_fmaf(e, fmaxf(d, -200.0f), s.s2);
+    }
+    const float ln = log_s1(s);
+    const int64_t tok = p.tokens[r];
+    write_row(p, r, s, ln, logp_of(p, tok, tok >= 0 && tok < p.vocab ? l[tok] : 0.0f, s, ln));
+    uint64_t last = ~0ull;
+    for (int i = 0; i < p.top_k; i++) {  // the largest key below the last
+        uint64_t best = 0;
+        if (last)
+            for (int j = 0; j < p.vocab; j++) {
+                const uint64_t key = l[j] > -INF ? key_of(l[j], (uint32_t)j) : 0;
+                best = key < last && key > best ? key : best;
+            }
+        write_top(p, r, i, s, ln, best);
+        last = best;
+    }
+}
+
+template <typename T, int MASK>
+__global__ void __launch_bounds__(256) k_logp_few_bwd(LpArgs p, uint32_t by_vocab, bool packed) {
+    extern __shared__ float s_rows[];
+    constexpr int V = 16 / sizeof(T);
+    const int64_t r0 = (int64_t)blockIdx.x * 256, r = r0 + threadIdx.x;
+    const int n = (int)(p.rows - r0 < 256 ? p.rows - r0 : 256), stride = p.vocab | 1;
+    stage_rows<T, MASK>(p, r0, n, stride, by_vocab, packed, s_rows);
+    __syncthreads();
+    if ((int)threadIdx.x < n) {
+        const RowGrad w = row_grad(p, r);
+        float* l = s_rows + threadIdx.x * stride;
+#pragma unroll 4
+        for (int j = 0; j < p.vocab; j++) l[j] = entry_grad(w, l[j], j);
+    }
+    __syncthreads();
+    T* out = (T*)p.dlogits + r0 * p.vocab;
+    const int all = n * p.vocab;
+    for (int i = threadIdx.x * V; i < all; i += 256 * V) {
         float f[V];
-        load_logits<T, MASK>(l, av, c, p.vocab - c, f);
+        int row = row_in(i, p.vocab, by_vocab), col = i - row * p.vocab;
 #pragma unroll
         for (int j = 0; j < V; j++) {
-            const float t = (f[j] - m) * LOG2E - l2;  // log2 p
-            float d = -__builtin_amdgcn_exp2f(t) * __builtin_fmaf(h2, fmaxf(t, -200.0f), base);
-            if (c + j == tok) d += g;
-            f[j] = none || f[j] == -INF ? 0.0f : d;
+            f[j] = i + j < all ? s_rows[row * stride + col] : 0.0f;
+            if (++col == p.vocab) col = 0, row++;
         }
-        store_upto(out + c, p.vocab - c, f);
+        store_upto(out + i, all - i, f);
     }
 }
 
@@ -326,17 +461,74 @@ const char* bad(const char* who, const LpArgs& a, int dtype, int mask_dtype) {
     return msg;
 }
 
+// threads that share a row: at most 4 loads of 16 bytes each where 16 or 64 do (0: a lane per row); the alternatives take whole
+// waves
+int threads_for(int64_t vocab, int dtype, bool top) {
+    if (vocab <= FEW) return 0;
+    const int64_t vecs = cdiv(vocab, dtype == EC_F32 ? 4 : 8);
+    return vecs <= 64 && !top ? 16 : vecs <= 256 ? 64 : 256;
+}
+// rows that lie one behind the other, mask and logits
+bool is_packed(const LpArgs& a) {
+    const bool l = a.s_outer == a.inner * a.vocab && (a.inner == 1 || a.s_inner == a.vocab);
+    return l && (!a.avail || (a.a_outer == a.inner * a.vocab && (a.inner == 1 || a.a_inner == a.vocab)));
+}
+// i / vocab = umulhi(i, by_vocab) for i < 2^16 and 2 <= vocab < 2^16: the excess over 2^32 / vocab is below 1
+uint32_t by_vocab(int vocab) { return (uint32_t)((((uint64_t)1 << 32) + vocab - 1) / vocab); }
+
 // few rows: a row is split over as many blocks as fill the GPU, at least one batch of loads each
 int splits_for(int64_t rows, int64_t vocab, int dtype) {
+    if (threads_for(vocab, dtype, true) != 256) return 1;
     const int64_t batch = 256 * U * (dtype == EC_F32 ? 4 : 8);
     const int64_t most = cdiv(vocab, batch), want = cdiv(1024, rows);
     return (int)(want < most ? want : most);
 }
 
-#define EC_LP_TYPES(GO)                                   \
-    if (dtype == EC_F32) { GO(float) }                    \
-    if (dtype == EC_BF16) { GO(bf16) }                    \
-    if (dtype == EC_F16) { GO(f16) }
+template <typename T, int MASK>
+void go_fwd(const LpArgs& a, int dtype, hipStream_t st) {
+    const int tpr = threads_for(a.vocab, dtype, a.top_k > 0);
+    const auto blocks = [&](int rows) { return dim3((unsigned)cdiv(a.rows, rows)); };
+    const dim3 b(256);
+    if (tpr == 0) {
+        hipLaunchKernelGGL((k_logp_few_fwd<T, MASK>), blocks(256), b, 256 * (a.vocab | 1) * 4, st, a, by_vocab(a.vocab), is_packed(a));
+    } else if (tpr == 16) {
+        hipLaunchKernelGGL((k_logp_fwd<T, MASK, false, 16>), blocks(16), b, 0, st, a);
+    } else if (tpr == 64) {
+        if (a.top_k) hipLaunchKernelGGL((k_logp_fwd<T, MASK, true, 64>), blocks(4), b, 0, st, a);
+        else hipLaunchKernelGGL((k_logp_fwd<T, MASK, false, 64>), blocks(4), b, 0, st, a);
+    } else {
+        const dim3 grid((unsigned)(a.rows * a.splits));
+        if (a.top_k) hipLaunchKernelGGL((k_logp_fwd<T, MASK, true, 256>), grid, b, 0, st, a);
+        else hipLaunchKernelGGL((k_logp_fwd<T, MASK, false, 256>), grid, b, 0, st, a);
+        if (a.splits > 1) hipLaunchKernelGGL((k_logp_join<T, MASK>), dim3((unsigned)a.rows), dim3(64), 0, st, a);
+    }
+}
+
+template <typename T, int MASK>
+void go_bwd(const LpArgs& a, int dtype, hipStream_t st) {
+    const int tpr = threads_for(a.vocab, dtype, false);
+    const auto blocks = [&](int rows) { return dim3((unsigned)cdiv(a.rows, rows)); };
+    const dim3 b(256);
+    if (tpr == 0)
+        hipLaunchKernelGGL((k_logp_few_bwd<T, MASK>), blocks(256), b, 256 * (a.vocab | 1) * 4, st, a, by_vocab(a.vocab), is_packed(a));
+    else if (tpr == 16)
+        hipLaunchKernelGGL((k_logp_bwd<T, MASK, 16>), blocks(16), b, 0, st, a);
+    else if (tpr == 64)
+        hipLaunchKernelGGL((k_logp_bwd<T, MASK, 64>), blocks(4), b, 0, st, a);
+    else
+        hipLaunchKernelGGL((k_logp_bwd<T, MASK, 256>), dim3((unsigned)(a.rows * a.splits)), b, 0, st, a);
+}
+
+#define EC_LP_GO(GO, T)                                  \
+    {                                                    \
+        if (mask_dtype == 0) GO<T, 0>(a, dtype, st);     \
+        if (mask_dtype == 1) GO<T, 1>(a, dtype, st);     \
+        if (mask_dtype == 2) GO<T, 2>(a, dtype, st);     \
+    }
+#define EC_LP_TYPES(GO)                       \
+    if (dtype == EC_F32) EC_LP_GO(GO, float)  \
+    if (dtype == EC_BF16) EC_LP_GO(GO, bf16)  \
+    if (dtype == EC_F16) EC_LP_GO(GO, f16)
 
 }  // namespace
 
@@ -368,20 +560,7 @@ extern "C" int ec_token_logprobs_fwd(const void* logits, int64_t inner, int64_t 
     a.per_split = (int)(cdiv(cdiv(vocab, a.splits), batch) * batch < INT32_MAX ? cdiv(cdiv(vocab, a.splits), batch) * batch : INT32_MAX);
     if (rows * a.splits > INT32_MAX) return ec::fail(EC_EINVAL, "ec_token_logprobs_fwd: %lld rows", (long long)rows);
     const hipStream_t st = (hipStream_t)stream;
-    const dim3 grid((unsigned)(rows * a.splits));
-#define EC_GO2(T, M)                                                                               \
-    {                                                                                              \
-        if (top_k) hipLaunchKernelGGL((k_logp_fwd<T, M, true>), grid, dim3(256), 0, st, a);        \
-        else hipLaunchKernelGGL((k_logp_fwd<T, M, false>), grid, dim3(256), 0, st, a);             \
-        if (a.splits > 1) hipLaunchKernelGGL((k_logp_join<T, M>), dim3((unsigned)rows), dim3(64), 0, st, a); \
-    }
-#define EC_GO(T)                          \
-    if (mask_dtype == 0) EC_GO2(T, 0)     \
-    if (mask_dtype == 1) EC_GO2(T, 1)     \
-    if (mask_dtype == 2) EC_GO2(T, 2)
-    EC_LP_TYPES(EC_GO)
-#undef EC_GO
-#undef EC_GO2
+    EC_LP_TYPES(go_fwd)
     EC_HIP(hipGetLastError());
     return EC_OK;
 }
@@ -398,16 +577,10 @@ extern "C" int ec_token_logprobs_bwd(const void* logits, int64_t inner, int64_t 
     if (!lse || !entropy || !dlogits) return ec::fail(EC_EINVAL, "ec_token_logprobs_bwd: null argument");
     a.lse = const_cast<float*>(lse), a.entropy_in = entropy, a.dlogp = dlogp, a.dentropy = dentropy, a.dlogits = dlogits;
     a.per_split = 256 * U * (dtype == EC_F32 ? 4 : 8);
-    a.splits = (int)cdiv(vocab, a.per_split);
+    a.splits = threads_for(vocab, dtype, false) == 256 ? (int)cdiv(vocab, a.per_split) : 1;
     if (rows * a.splits > INT32_MAX) return ec::fail(EC_EINVAL, "ec_token_logprobs_bwd: %lld rows", (long long)rows);
     const hipStream_t st = (hipStream_t)stream;
-    const dim3 grid((unsigned)(rows * a.splits));
-#define EC_GO(T)                                                                                        \
-    if (mask_dtype == 0) hipLaunchKernelGGL((k_logp_bwd<T, 0>), grid, dim3(256), 0, st, a);             \
-    if (mask_dtype == 1) hipLaunchKernelGGL((k_logp_bwd<T, 1>), grid, dim3(256), 0, st, a);             \
-    if (mask_dtype == 2) hipLaunchKernelGGL((k_logp_bwd<T, 2>), grid, dim3(256), 0, st, a);
-    EC_LP_TYPES(EC_GO)
-#undef EC_GO
+    EC_LP_TYPES(go_bwd)
     EC_HIP(hipGetLastError());
     return EC_OK;
 }
