@@ -8,8 +8,7 @@ from collections import namedtuple
 import torch as th
 
 from marl_amd import _abi
-from marl_amd.utils.mlp_device import _p, _stream
-from marl_amd.utils.norm_device import need_device, need_dtype, refuse_capture
+from marl_amd.utils.norm_device import launch, need_device, need_dtype, ptr, refuse_capture
 
 MAX_TOP = 64  # EC_TOKEN_LOGPROBS_MAX_TOP
 
@@ -19,6 +18,9 @@ TokenLogprobs = namedtuple("TokenLogprobs", "logp entropy top_logp top_index lse
 def _layout(t, vocab):
     """(tensor, inner, outer stride, inner stride): the rows of t [..., vocab] as [outer, inner] of them, a view where the
     strides allow one (a slice of steps out of [batch, steps, vocab] does)"""
+    if t.dim() == 2:
+        t = t if vocab == 1 or t.stride(1) == 1 else t.contiguous()
+        return t, 1, t.stride(0), 0
     lead = t.shape[:-1]
     inner = lead[-1] if len(lead) >= 2 else 1
     outer = lead[:-1].numel() if len(lead) >= 2 else lead.numel()
@@ -44,7 +46,7 @@ def _inputs(who, logits, tokens, avail):
         if avail.is_floating_point() or avail.is_complex():
             raise TypeError("%s: avail of type %s (bool or integers)" % (who, avail.dtype))
         try:
-            avail = avail.expand(logits.shape)
+            avail = avail if avail.shape == logits.shape else avail.expand(logits.shape)
         except RuntimeError:
             raise ValueError("%s: avail of shape %s for logits of shape %s" % (who, tuple(avail.shape), tuple(logits.shape))) from None
         if avail.dtype not in (th.bool, th.uint8, th.int8, th.int32):
@@ -56,7 +58,7 @@ def _inputs(who, logits, tokens, avail):
     logits, inner, so, si = _layout(logits, vocab)
     tokens = tokens.to(th.int64).contiguous()
     # (the tensors are kept by the caller until the launch is made)
-    head = (_p(logits), inner, so, si, _p(tokens), _p(avail), kind, ao, ai, code, tokens.numel(), vocab)
+    head = (logits.data_ptr(), inner, so, si, tokens.data_ptr(), ptr(avail), kind, ao, ai, code, tokens.numel(), vocab)
     return dev, head, (logits, tokens, avail)
 
 
@@ -76,16 +78,14 @@ def token_logprobs_fwd(logits, tokens, avail=None, top_k=0):
         raise ValueError("token_logprobs_fwd: top_k %d (0 .. %d)" % (top_k, MAX_TOP))
     lead = tuple(tokens.shape)
     rows, vocab, code = head[-2], head[-1], head[-3]
-    f32 = lambda *s: th.empty(s, dtype=th.float32, device=dev)
-    logp, entropy, lse = f32(*lead), f32(*lead), f32(*lead, 2)
-    top_logp = f32(*lead, top_k) if top_k else None
+    logp, entropy = th.empty((2,) + lead, dtype=th.float32, device=dev).unbind(0)
+    lse = th.empty(lead + (2,), dtype=th.float32, device=dev)
+    top_logp = th.empty(lead + (top_k,), dtype=th.float32, device=dev) if top_k else None
     top_index = th.empty(lead + (top_k,), dtype=th.int64, device=dev) if top_k else None
-    L = _abi.lib()
-    nbytes = L.ec_token_logprobs_workspace(rows, vocab, code, top_k)
+    nbytes = _abi.lib().ec_token_logprobs_workspace(rows, vocab, code, top_k)
     work = th.empty(nbytes, dtype=th.uint8, device=dev) if nbytes else None
-    with th.cuda.device(dev):
-        _abi.check(L.ec_token_logprobs_fwd(*head, top_k, _p(logp), _p(entropy), _p(lse), _p(top_logp), _p(top_index), _p(work),
-                                           nbytes, _stream(dev)), "ec_token_logprobs_fwd")
+    launch("ec_token_logprobs_fwd", dev, *head, top_k, logp.data_ptr(), entropy.data_ptr(), lse.data_ptr(), ptr(top_logp),
+           ptr(top_index), ptr(work), nbytes)
     del keep
     return TokenLogprobs(logp, entropy, top_logp, top_index, lse)
 
@@ -103,10 +103,8 @@ def token_logprobs_bwd(logits, tokens, lse, entropy, dlogp=None, dentropy=None, 
         if t is not None and (t.shape != shape or t.dtype != th.float32):
             raise ValueError("token_logprobs_bwd: %s is float32 of shape %s, not %s %s" % (name, tuple(shape), t.dtype, tuple(t.shape)))
         small.append(t.contiguous() if t is not None else None)
-    out = th.empty(logits.shape, dtype=logits.dtype, device=dev)
-    with th.cuda.device(dev):
-        _abi.check(_abi.lib().ec_token_logprobs_bwd(*head, *[_p(t) for t in small], _p(out), _stream(dev)),
-                   "ec_token_logprobs_bwd")
+    out = th.empty_like(logits, memory_format=th.contiguous_format)
+    launch("ec_token_logprobs_bwd", dev, *head, *map(ptr, small), out.data_ptr())
     del keep
     return out
 

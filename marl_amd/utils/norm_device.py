@@ -2,27 +2,40 @@
 
 `layer_norm` is the autograd form; `layer_norm_fwd` and `layer_norm_bwd` are the two passes by hand, for update steps that
 keep no autograd graph and for recording into a HIP graph."""
-import ctypes as C
-
 import torch as th
 
 from marl_amd import _abi
-from marl_amd.utils.mlp_device import _p, _stream
 
 DTYPES = {th.float32: 0, th.bfloat16: 1, th.float16: 2}  # EC_F32, EC_BF16, EC_F16
 
 
 def need_device(who, *tensors):
     """one ROCm device for all of them (None: not given)"""
-    dev = tensors[0].device
+    at = tensors[0].get_device()
     for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise RuntimeError("%s needs device tensors: marl_amd has no CPU fallback" % who)
-        if t.device != dev:
-            raise ValueError("%s: tensors on %s and %s" % (who, dev, t.device))
-    return dev
+        if t is not None and t.get_device() != at or at < 0:
+            if not t.is_cuda or at < 0:
+                raise RuntimeError("%s needs device tensors: marl_amd has no CPU fallback" % who)
+            raise ValueError("%s: tensors on %s and %s" % (who, tensors[0].device, t.device))
+    return tensors[0].device
+
+
+def ptr(t):
+    return t.data_ptr() if t is not None else None
+
+
+def launch(name, dev, *args):
+    """the C entry point `name` on dev's current stream (the last argument of each).  Calls of a few microseconds are
+    what these operators' small sizes cost, so the device is only switched when it is another, and pointers go in as ints"""
+    fn, at = getattr(_abi.lib(), name), dev.index
+    stream = th._C._cuda_getCurrentRawStream(at)
+    if th._C._cuda_getDevice() == at:
+        rc = fn(*args, stream)
+    else:
+        with th.cuda.device(dev):
+            rc = fn(*args, stream)
+    if rc:
+        _abi.check(rc, name)
 
 
 def need_dtype(who, t):
@@ -42,7 +55,8 @@ def refuse_capture(who, instead):
 
 def _rows(t, cols):
     """[rows, cols] with contiguous columns; a view where the strides allow one"""
-    t = t.reshape(-1, cols)
+    if t.dim() != 2:
+        t = t.reshape(-1, cols)
     return t if cols == 1 or t.stride(1) == 1 else t.contiguous()
 
 
@@ -57,7 +71,7 @@ def _check(who, x, weight, bias, eps):
     for t in (weight, bias):
         if t is None:
             continue
-        if tuple(t.shape) != (x.shape[-1],):
+        if t.dim() != 1 or t.shape[0] != x.shape[-1]:
             raise ValueError("%s: weight / bias of shape %s for %d columns" % (who, tuple(t.shape), x.shape[-1]))
         wcode = need_dtype(who, t)
         if t.dtype not in (x.dtype, th.float32) or (weight is not None and bias is not None and weight.dtype != bias.dtype):
@@ -73,15 +87,14 @@ def layer_norm_fwd(x, weight=None, bias=None, eps=1e-5, want_stats=True):
     cols = x.shape[-1]
     x2 = _rows(x, cols)
     rows = x2.shape[0]
-    y = th.empty(x.shape, dtype=x.dtype, device=dev)
+    y = th.empty_like(x, memory_format=th.contiguous_format)
     mean = rstd = None
     if want_stats:
         mean, rstd = th.empty((2,) + tuple(x.shape[:-1]), dtype=th.float32, device=dev).unbind(0)
     weight = weight.contiguous() if weight is not None else None
     bias = bias.contiguous() if bias is not None else None
-    with th.cuda.device(dev):
-        _abi.check(_abi.lib().ec_layer_norm_fwd(_p(x2), x2.stride(0), _p(weight), _p(bias), code, wcode, rows, cols,
-                                                C.c_double(eps), _p(y), _p(mean), _p(rstd), _stream(dev)), "ec_layer_norm_fwd")
+    launch("ec_layer_norm_fwd", dev, x2.data_ptr(), x2.stride(0), ptr(weight), ptr(bias), code, wcode, rows, cols, eps, y.data_ptr(),
+           ptr(mean), ptr(rstd))
     return y, mean, rstd
 
 
@@ -104,20 +117,18 @@ def layer_norm_bwd(dy, x, mean, rstd, weight=None, want_dx=True, want_dweight=Tr
     ptype = weight.dtype if weight is not None else (param_dtype or x.dtype)
     x2, dy2 = _rows(x, cols), _rows(dy, cols)
     rows = x2.shape[0]
-    dx = th.empty(x.shape, dtype=x.dtype, device=dev) if want_dx else None
+    dx = th.empty_like(x, memory_format=th.contiguous_format) if want_dx else None
     if rows == 0:
         zeros = lambda want: th.zeros(cols, dtype=ptype, device=dev) if want else None
         return dx, zeros(want_dweight), zeros(want_dbias)
     dw = th.empty(cols, dtype=ptype, device=dev) if want_dweight else None
     db = th.empty(cols, dtype=ptype, device=dev) if want_dbias else None
-    L = _abi.lib()
-    n_part = L.ec_layer_norm_bwd_partials(rows, cols, code) if want_dweight or want_dbias else 0
+    n_part = _abi.lib().ec_layer_norm_bwd_partials(rows, cols, code) if want_dweight or want_dbias else 0
     partials = th.empty(n_part, 2, cols, dtype=th.float32, device=dev) if n_part else None
     weight = weight.contiguous() if weight is not None else None
-    with th.cuda.device(dev):
-        _abi.check(L.ec_layer_norm_bwd(_p(dy2), dy2.stride(0), _p(x2), x2.stride(0), _p(mean.contiguous()), _p(rstd.contiguous()),
-                                       _p(weight), code, wcode, rows, cols, _p(dx), _p(partials), n_part, _p(dw), _p(db),
-                                       _stream(dev)), "ec_layer_norm_bwd")
+    mean, rstd = mean.contiguous(), rstd.contiguous()
+    launch("ec_layer_norm_bwd", dev, dy2.data_ptr(), dy2.stride(0), x2.data_ptr(), x2.stride(0), mean.data_ptr(), rstd.data_ptr(),
+           ptr(weight), code, wcode, rows, cols, ptr(dx), ptr(partials), n_part, ptr(dw), ptr(db))
     return dx, dw, db
 
 

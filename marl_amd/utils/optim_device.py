@@ -6,13 +6,14 @@ tensors in place.
 
 ec_grad_clip_coef, ec_adamw_step: AdamW over any number of tensors of any size, moments in 32 or 8 bits (`AdamW`, and
 `clip_coef` / `adamw_step` on lists of tensors)."""
+import array
 import ctypes as C
+import operator
 
 import torch as th
 
 from marl_amd import _abi
-from marl_amd.utils.mlp_device import _p, _stream
-from marl_amd.utils.norm_device import DTYPES
+from marl_amd.utils.norm_device import DTYPES, launch, ptr
 
 MAX_NETS, MAX_TENSORS = 4, 16
 
@@ -100,6 +101,7 @@ def clip_adam_step(optimizers, max_norm):
 # ---- AdamW over many tensors of any size (ec_grad_clip_coef, ec_adamw_step) ----
 QBLOCK = 256                      # elements that share a scale of the 8-bit states
 STATE8 = th.float8_e4m3fn
+_FLOATS = set(DTYPES)
 
 
 def scale_count(p):
@@ -107,18 +109,31 @@ def scale_count(p):
     return -(-p.numel() // QBLOCK)
 
 
-def _pointers(who, name, tensors, dev, numel, dtypes=None, same=None):
-    """addresses of contiguous tensors on dev: element counts as `numel`, types as the set `dtypes` or as the list `same`"""
+_DTYPE, _NUMEL, _DEVICE, _PTR, _PACKED = (operator.attrgetter("dtype"), th.Tensor.numel, th.Tensor.get_device, th.Tensor.data_ptr,
+                                          th.Tensor.is_contiguous)
+
+
+def _pointers(who, name, tensors, at, numel, dtypes):
+    """addresses (array of 64-bit words) of contiguous tensors on device `at`, with `numel` elements each and types in `dtypes`
+    (a set for all of them, or a list, one each).  Whole lists at a time: at hundreds of tensors these checks are the call's
+    longest part on the host"""
+    kinds = list(map(_DTYPE, tensors))
+    if (list(map(_NUMEL, tensors)) == numel and set(map(_DEVICE, tensors)) == {at} and set(map(_PACKED, tensors)) == {True}
+            and (kinds == dtypes if isinstance(dtypes, list) else dtypes.issuperset(kinds))):
+        return array.array("Q", map(_PTR, tensors))
     if len(tensors) != len(numel):
         raise ValueError("%s: %d %s for %d tensors" % (who, len(tensors), name, len(numel)))
-    out = []
     for i, t in enumerate(tensors):
-        if t.device != dev or t.numel() != numel[i] or not t.is_contiguous() or t.dtype not in (dtypes or (same[i].dtype,)):
-            raise ValueError("%s: %s[%d] is %s %s on %s%s; %d contiguous elements of %s on %s are needed"
+        want = {dtypes[i]} if isinstance(dtypes, list) else dtypes
+        if t.get_device() != at or t.numel() != numel[i] or not t.is_contiguous() or t.dtype not in want:
+            raise ValueError("%s: %s[%d] is %s %s on %s%s; %d contiguous elements of %s on cuda:%d are needed"
                              % (who, name, i, t.dtype, tuple(t.shape), t.device, "" if t.is_contiguous() else ", not contiguous",
-                                numel[i], "/".join(map(str, dtypes or (same[i].dtype,))), dev))
-        out.append(t.data_ptr())
-    return out
+                                numel[i], "/".join(map(str, want)), at))
+
+
+def _address(a):
+    """of an array's words (None: NULL)"""
+    return a.buffer_info()[0] if a is not None else None
 
 
 def _device_of(who, tensors):
@@ -138,18 +153,18 @@ def clip_coef(grads, max_norm):
     dev = _device_of("clip_coef", grads)
     if not max_norm > 0:
         raise ValueError("clip_coef: max_norm %r" % (max_norm,))
-    numel = [g.numel() for g in grads]
-    G = _pointers("clip_coef", "grads", grads, dev, numel, dtypes=tuple(DTYPES))
-    n = len(grads)
-    numel = (C.c_int64 * n)(*numel)
-    L = _abi.lib()
-    nbytes = L.ec_grad_clip_workspace(n, numel)
-    work = th.empty(nbytes // 8, dtype=th.float64, device=dev)
-    norm, coef = th.empty(2, dtype=th.float32, device=dev).unbind(0)
-    with th.cuda.device(dev):
-        _abi.check(L.ec_grad_clip_coef(n, (C.c_void_p * n)(*G), numel, (C.c_int32 * n)(*[DTYPES[g.dtype] for g in grads]),
-                                       C.c_double(max_norm), _p(norm), _p(coef), _p(work), nbytes, _stream(dev)),
-                   "ec_grad_clip_coef")
+    numel = list(map(_NUMEL, grads))
+    G = _pointers("clip_coef", "grads", grads, dev.index, numel, _FLOATS)
+    return _clip_coef(dev, G, array.array("q", numel), array.array("i", map(DTYPES.get, map(_DTYPE, grads))), max_norm)
+
+
+def _clip_coef(dev, G, numel, codes, max_norm):
+    n, counts = len(numel), numel.buffer_info()[0]
+    nbytes = _abi.lib().ec_grad_clip_workspace(n, counts)
+    work = th.empty(nbytes // 8 + 1, dtype=th.float64, device=dev)
+    norm, coef = work[-1:].view(th.float32).unbind(0)
+    launch("ec_grad_clip_coef", dev, n, _address(G), counts, _address(codes), max_norm, norm.data_ptr(), coef.data_ptr(), work.data_ptr(),
+           nbytes)
     return norm, coef
 
 
@@ -169,24 +184,26 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, exp_avg_scale=None, exp_avg_s
     device scalar (one clip over several calls).  The gradients are only read."""
     who = "adamw_step"
     dev = _device_of(who, params)
-    n = len(params)
-    numel = [p.numel() for p in params]
-    P = _pointers(who, "params", params, dev, numel, dtypes=tuple(DTYPES))
-    live = [a for a, k in zip(P, numel) if k]
-    if len(set(live)) != len(live):
-        raise ValueError("adamw_step: the same parameter twice")
-    G = _pointers(who, "grads", grads, dev, numel, same=params)
+    n, at = len(params), dev.index
+    numel = list(map(_NUMEL, params))
+    kinds = list(map(_DTYPE, params))
+    P = _pointers(who, "params", params, at, numel, _FLOATS)
+    if len(set(P)) != n:
+        live = [a for a, k in zip(P, numel) if k]
+        if len(set(live)) != len(live):
+            raise ValueError("adamw_step: the same parameter twice")
+    G = _pointers(who, "grads", grads, at, numel, kinds)
     bits = 8 if exp_avg_scale is not None else 32
-    st = (STATE8,) if bits == 8 else (th.float32,)
-    M = _pointers(who, "exp_avg", exp_avg, dev, numel, dtypes=st)
-    V = _pointers(who, "exp_avg_sq", exp_avg_sq, dev, numel, dtypes=st)
+    st = {STATE8} if bits == 8 else {th.float32}
+    M = _pointers(who, "exp_avg", exp_avg, at, numel, st)
+    V = _pointers(who, "exp_avg_sq", exp_avg_sq, at, numel, st)
     MS = VS = None
     if bits == 8:
         if exp_avg_sq_scale is None:
             raise ValueError("adamw_step: exp_avg_scale without exp_avg_sq_scale")
         blocks = [-(-k // QBLOCK) for k in numel]
-        MS = (C.c_void_p * n)(*_pointers(who, "exp_avg_scale", exp_avg_scale, dev, blocks, dtypes=(th.float32,)))
-        VS = (C.c_void_p * n)(*_pointers(who, "exp_avg_sq_scale", exp_avg_sq_scale, dev, blocks, dtypes=(th.float32,)))
+        MS = _pointers(who, "exp_avg_scale", exp_avg_scale, at, blocks, {th.float32})
+        VS = _pointers(who, "exp_avg_sq_scale", exp_avg_sq_scale, at, blocks, {th.float32})
     elif exp_avg_sq_scale is not None:
         raise ValueError("adamw_step: exp_avg_sq_scale without exp_avg_scale")
     for name, t in (("step", step), ("lr", lr), ("coef", coef)):
@@ -208,15 +225,14 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, exp_avg_scale=None, exp_avg_s
     if max_norm is not None:
         if coef is not None:
             raise ValueError("adamw_step: max_norm and coef")
-        norm, coef = clip_coef(grads, max_norm)
-    vps = lambda xs: (C.c_void_p * n)(*xs)
-    on_dev = dyn is not None
-    with th.cuda.device(dev):
-        _abi.check(_abi.lib().ec_adamw_step(
-            n, vps(P), vps(G), vps(M), vps(V), MS, VS, (C.c_int64 * n)(*numel), (C.c_int32 * n)(*[DTYPES[p.dtype] for p in params]),
-            bits, _p(coef), C.c_double(0.0 if on_dev else float(step)), _p(step if on_dev else None), _p(dyn),
-            C.c_double(0.0 if isinstance(lr, th.Tensor) else float(lr)), _p(lr if isinstance(lr, th.Tensor) else None),
-            C.c_double(b1), C.c_double(b2), C.c_double(eps), C.c_double(weight_decay), _stream(dev)), "ec_adamw_step")
+        if not max_norm > 0:
+            raise ValueError("adamw_step: max_norm %r" % (max_norm,))
+    counts, codes = array.array("q", numel), array.array("i", map(DTYPES.get, kinds))
+    if max_norm is not None:
+        norm, coef = _clip_coef(dev, G, counts, codes, max_norm)
+    on_dev, lr_dev = dyn is not None, isinstance(lr, th.Tensor)
+    launch("ec_adamw_step", dev, n, *map(_address, (P, G, M, V, MS, VS, counts, codes)), bits, ptr(coef), 0.0 if on_dev else step,
+           ptr(step if on_dev else None), ptr(dyn), 0.0 if lr_dev else lr, ptr(lr if lr_dev else None), b1, b2, eps, weight_decay)
     th.autograd.graph.increment_version(params)  # (written through raw pointers: autograd has to know)
     return norm
 
