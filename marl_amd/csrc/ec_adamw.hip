@@ -22,8 +22,8 @@ namespace {
 using namespace ecs;
 
 constexpr int MAX_TENSORS = 48;          // (the argument block stays under the 4 KB a launch can carry)
-constexpr int CHUNK = 4096;              // elements a block
-constexpr int QBLOCK = 256;              // elements that share a scale: a wave, four each
+constexpr int CHUNK = 2048;              // elements a block
+constexpr int QBLOCK = 256;              // elements that share a scale
 constexpr float QMAX = 448.0f, QMIN = 0.001953125f;
 
 struct Tensor {
@@ -39,136 +39,191 @@ struct Group {
 };
 struct Hyper {
     float omb1, b2, omb2, eps;           // 1 - beta, rounded once from double
-    float step_size, bc2_sqrt, keep;     // lr / (1 - b1^t), sqrt(1 - b2^t), 1 - lr wd
+    float step_size, inv_bc2, keep;      // lr / (1 - b1^t), 1 / sqrt(1 - b2^t), 1 - lr wd
     const float* coef;                   // of the gradients, on the device, or NULL: 1
-    const float* dyn;                    // {step_size, bc2_sqrt, keep} on the device, or NULL
+    const float* dyn;                    // {step_size, inv_bc2, keep} on the device, or NULL
 };
 static_assert(sizeof(Group) + sizeof(Hyper) + 64 <= 4096, "argument block");
 
+// the tensor of a block: each lane compares one entry of `first` (a bisection would be a chain of loads)
 __device__ __forceinline__ int tensor_of(const Group& a, uint32_t block) {
-    int lo = 0, hi = a.count;            // first[lo] <= block < first[hi]
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (a.first[mid] <= block) lo = mid;
-        else hi = mid;
-    }
-    return lo;
+    const int lane = threadIdx.x & 63;
+    const bool at = lane < a.count && a.first[lane < MAX_TENSORS ? lane : 0] <= block;
+    return __popcll(__ballot(at)) - 1;
 }
 
-__device__ __forceinline__ void read_hyper(Hyper& h, float& coef) {
-    coef = h.coef ? *h.coef : 1.0f;
-    if (h.dyn) h.step_size = h.dyn[0], h.bc2_sqrt = h.dyn[1], h.keep = h.dyn[2];
+__device__ __forceinline__ float read_hyper(Hyper& h) {
+    if (h.dyn) h.step_size = h.dyn[0], h.inv_bc2 = h.dyn[1], h.keep = h.dyn[2];
+    return h.coef ? *h.coef : 1.0f;
 }
 
-// m, v -> m', v' and p -> p'; root: sqrt(v').  One rounding per operation, in the order of the formulas above
+// sqrt to one unit in the last place, for every v >= 0 (the instruction alone takes what is below 2^-126 as 0)
+__device__ __forceinline__ float root_of(float v) {
+    const bool small = v < 1e-30f;
+    const float r = __builtin_amdgcn_sqrtf(small ? v * 18446744073709551616.0f : v);
+    return small ? r * 2.3283064365386962890625e-10f : r;
+}
+
+// m, v -> m', v' and p -> p'; root: sqrt(v').  The quotient is a product with v_rcp's inverse (one unit in the last place):
+// its error is that of the step, far below a rounding of p
 __device__ __forceinline__ void adam(const Hyper& h, float coef, float g, float& p, float& m, float& v, float& root) {
     g *= coef;
-    m = m + (g - m) * h.omb1;
-    v = v * h.b2 + h.omb2 * g * g;
-    root = sqrtf(v);
-    p = p * h.keep - h.step_size * m / (root / h.bc2_sqrt + h.eps);
+    m = __builtin_fmaf(g - m, h.omb1, m);
+    v = __builtin_fmaf(h.omb2 * g, g, v * h.b2);
+    root = root_of(v);
+    const float inv = __builtin_amdgcn_rcpf(__builtin_fmaf(root, h.inv_bc2, h.eps));
+    p = __builtin_fmaf(-h.step_size * m, inv, p * h.keep);
 }
 
+// A block takes CHUNK consecutive elements of one tensor, eight a thread, all loads ahead of all stores (a loop with less in
+// flight, or with stores between its loads, runs at 5.2 TB/s against 5.9).  16-bit types: eight in a row; fp32: two runs of
+// four, half a chunk (or, with 8-bit states, half a scale's block) apart.
 template <typename T>
+struct Take {
+    static constexpr int EACH = sizeof(T) == 4 ? 4 : 8, RUNS = 8 / EACH;
+};
+
+template <typename T, bool NT>
 __global__ void __launch_bounds__(256) k_adamw32(Group a, Hyper h) {
+    constexpr int E = Take<T>::EACH, R = Take<T>::RUNS;
     const int k = tensor_of(a, blockIdx.x);
     const Tensor t = a.t[k];
-    float coef;
-    read_hyper(h, coef);
-    const int64_t e0 = (int64_t)(blockIdx.x - a.first[k]) * CHUNK;
-#pragma unroll 4
-    for (int i = 0; i < CHUNK / 1024; i++) {
-        const int64_t e = e0 + i * 1024 + threadIdx.x * 4, n = t.n - e;
-        float p[4], g[4], m[4], v[4], root;
-        load_upto((const T*)t.p + e, n, 0.0f, p);
-        load_upto((const T*)t.g + e, n, 0.0f, g);
-        load_upto((const float*)t.m + e, n, 0.0f, m);
-        load_upto((const float*)t.v + e, n, 0.0f, v);
+    const int64_t e0 = (int64_t)(blockIdx.x - a.first[k]) * CHUNK + threadIdx.x * E;
+    float p[R][E], g[R][E], m[R][E], v[R][E], root;
 #pragma unroll
-        for (int j = 0; j < 4; j++) adam(h, coef, g[j], p[j], m[j], v[j], root);
-        store_upto((T*)t.p + e, n, p);
-        store_upto((float*)t.m + e, n, m);
-        store_upto((float*)t.v + e, n, v);
+    for (int i = 0; i < R; i++) {
+        const int64_t e = e0 + i * (CHUNK / R), n = t.n - e;
+        load_upto<T, E, NT>((const T*)t.g + e, n, 0.0f, g[i]);
+        load_upto<float, E, NT>((const float*)t.m + e, n, 0.0f, m[i]);
+        load_upto<float, E, NT>((const float*)t.v + e, n, 0.0f, v[i]);
+        load_upto<T, E, NT>((const T*)t.p + e, n, 0.0f, p[i]);
+    }
+    const float coef = read_hyper(h);
+#pragma unroll
+    for (int i = 0; i < R; i++)
+#pragma unroll
+        for (int j = 0; j < E; j++) adam(h, coef, g[i][j], p[i][j], m[i][j], v[i][j], root);
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+        const int64_t e = e0 + i * (CHUNK / R), n = t.n - e;
+        store_upto<T, E, NT>((T*)t.p + e, n, p[i]);
+        store_upto<float, E, NT>((float*)t.m + e, n, m[i]);
+        store_upto<float, E, NT>((float*)t.v + e, n, v[i]);
     }
 }
 
-// four e4m3 values of a dword
-__device__ __forceinline__ void unpack8(uint32_t q, float (&f)[4]) {
-    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)q, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)q, true);
-    f[0] = lo[0], f[1] = lo[1], f[2] = hi[0], f[3] = hi[1];
-}
-__device__ __forceinline__ uint32_t pack8(const float (&f)[4]) {
-    int q = __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false);
-    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], q, true);
-}
-typedef uint32_t u32_any __attribute__((aligned(1)));
-__device__ __forceinline__ uint32_t load8(const uint8_t* q, int64_t n) {
-    if (n >= 4) return *reinterpret_cast<const u32_any*>(q);
-    uint32_t x = 0;
+// N e4m3 values of N bytes at any address (N = 4, 8), the first n of them; the others 0 / untouched
+template <int N>
+struct Bytes {
+    uint32_t w[N / 4];
+};
+template <int N, bool NT>
+__device__ __forceinline__ Bytes<N> load8(const uint8_t* q, int64_t n) {
+    Bytes<N> b;
+    if (n >= N) {
+        const auto v = load_raw<NT, uint8_t, N>(q);
+        __builtin_memcpy(&b, &v, N);
+        return b;
+    }
 #pragma unroll
-    for (int j = 0; j < 3; j++)
-        if (j < n) x |= (uint32_t)q[j] << (8 * j);
-    return x;
+    for (int k = 0; k < N / 4; k++) {
+        b.w[k] = 0;
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (4 * k + j < n) b.w[k] |= (uint32_t)q[4 * k + j] << (8 * j);
+    }
+    return b;
 }
-__device__ __forceinline__ void store8(uint8_t* q, int64_t n, uint32_t x) {
-    if (n >= 4) {
-        *reinterpret_cast<u32_any*>(q) = x;
+template <int N, bool NT>
+__device__ __forceinline__ void store8(uint8_t* q, int64_t n, const Bytes<N>& b) {
+    if (n >= N) {
+        raw_t<uint8_t, N> v;
+        __builtin_memcpy(&v, &b, N);
+        store_raw<NT, uint8_t, N>(q, v);
         return;
     }
 #pragma unroll
-    for (int j = 0; j < 3; j++)
-        if (j < n) q[j] = (uint8_t)(x >> (8 * j));
+    for (int j = 0; j < N; j++)
+        if (j < n) q[j] = (uint8_t)(b.w[j / 4] >> (8 * (j % 4)));
 }
-// the scale of a block whose largest magnitude has these bits (a NaN's are larger than any number's: it marks the whole
-// block), and its inverse; a block of zeros, or of what is too small for 1 / s, is held as zeros
-__device__ __forceinline__ float scale_of(uint32_t most, float& inv) {
-    float s = bitsf(most) / QMAX;
+template <int N>
+__device__ __forceinline__ void unpack8(const Bytes<N>& b, float scale, float (&f)[N]) {
+#pragma unroll
+    for (int k = 0; k < N / 4; k++) {
+        const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)b.w[k], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)b.w[k], true);
+        f[4 * k] = lo[0] * scale, f[4 * k + 1] = lo[1] * scale, f[4 * k + 2] = hi[0] * scale, f[4 * k + 3] = hi[1] * scale;
+    }
+}
+template <int N>
+__device__ __forceinline__ Bytes<N> pack8(const float (&f)[N]) {
+    Bytes<N> b;
+#pragma unroll
+    for (int k = 0; k < N / 4; k++) {
+        const int q = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * k], f[4 * k + 1], 0, false);
+        b.w[k] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[4 * k + 2], f[4 * k + 3], q, true);
+    }
+    return b;
+}
+// the scale of a block with this largest magnitude (NaN left out: it stays its element's), and its inverse; a block of zeros,
+// or of what is too small for 1 / s, is held as zeros
+__device__ __forceinline__ float scale_of(float most, float& inv) {
+    float s = most * (1.0f / QMAX);
     s = s < 1.17549435e-38f ? 0.0f : s;
-    inv = s != 0.0f ? 1.0f / s : 0.0f;
+    inv = s != 0.0f ? __builtin_amdgcn_rcpf(s) : 0.0f;
     return s;
 }
 
-template <typename T>
+// half a wave takes the 256 elements of a scale
+template <typename T, bool NT>
 __global__ void __launch_bounds__(256) k_adamw8(Group a, Hyper h) {
-    const int k = tensor_of(a, blockIdx.x), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    constexpr int E = Take<T>::EACH, R = Take<T>::RUNS;
+    const int k = tensor_of(a, blockIdx.x);
     const Tensor t = a.t[k];
-    float coef;
-    read_hyper(h, coef);
-    const int64_t b0 = (int64_t)(blockIdx.x - a.first[k]) * (CHUNK / QBLOCK);
-#pragma unroll 4
-    for (int i = 0; i < CHUNK / QBLOCK / 4; i++) {
-        const int64_t b = b0 + i * 4 + wave, e = b * QBLOCK + lane * 4, n = t.n - e;
-        if (b * QBLOCK >= t.n) break;  // (the same for all lanes of the wave)
-        float p[4], g[4], m[4], v[4], root[4];
-        load_upto((const T*)t.p + e, n, 0.0f, p);
-        load_upto((const T*)t.g + e, n, 0.0f, g);
-        unpack8(load8((const uint8_t*)t.m + e, n), m);
-        unpack8(load8((const uint8_t*)t.v + e, n), v);
-        const float ms = t.ms[b], vs = t.vs[b];
-        uint32_t most_m = 0, most_v = 0;
+    const int64_t b = (int64_t)(blockIdx.x - a.first[k]) * (CHUNK / QBLOCK) + threadIdx.x / 32, e0 = b * QBLOCK + (threadIdx.x & 31) * E;
+    const bool on = b * QBLOCK < t.n;
+    float p[R][E], g[R][E], m[R][E], v[R][E];
+    Bytes<E> qm[R], qv[R];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            m[j] *= ms;
-            v[j] *= vs;
-            v[j] *= v[j];
-            adam(h, coef, g[j], p[j], m[j], v[j], root[j]);
-            const uint32_t am = fbits(m[j]) & 0x7fffffffu, av = fbits(root[j]) & 0x7fffffffu;
-            most_m = am > most_m ? am : most_m;
-            most_v = av > most_v ? av : most_v;
-        }
-        float im, iv;
-        const float sm = scale_of(lanes_umax<64>(most_m), im), sv = scale_of(lanes_umax<64>(most_v), iv);
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            m[j] *= im;
-            const float q = root[j] * iv;
-            v[j] = root[j] > 0.0f && sv > 0.0f && q < QMIN ? QMIN : q;
-        }
-        store_upto((T*)t.p + e, n, p);
-        store8((uint8_t*)t.m + e, n, pack8(m));
-        store8((uint8_t*)t.v + e, n, pack8(v));
-        if (lane == 0) t.ms[b] = sm, t.vs[b] = sv;
+    for (int i = 0; i < R; i++) {
+        const int64_t e = e0 + i * (QBLOCK / R), n = t.n - e;
+        load_upto<T, E, NT>((const T*)t.g + e, n, 0.0f, g[i]);
+        qm[i] = load8<E, NT>((const uint8_t*)t.m + e, n);
+        qv[i] = load8<E, NT>((const uint8_t*)t.v + e, n);
+        load_upto<T, E, NT>((const T*)t.p + e, n, 0.0f, p[i]);
     }
+    const float ms = on ? t.ms[b] : 0.0f, vs = on ? t.vs[b] : 0.0f;
+    const float coef = read_hyper(h);
+    float most_m = 0.0f, most_v = 0.0f;
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+        unpack8(qm[i], ms, m[i]);
+        unpack8(qv[i], vs, v[i]);
+#pragma unroll
+        for (int j = 0; j < E; j++) {
+            float root;
+            v[i][j] *= v[i][j];
+            adam(h, coef, g[i][j], p[i][j], m[i][j], v[i][j], root);
+            v[i][j] = root;
+            most_m = fmaxf(most_m, fabsf(m[i][j]));
+            most_v = fmaxf(most_v, root);
+        }
+    }
+    float im, iv;
+    const float sm = scale_of(lanes_max<32>(most_m), im), sv = scale_of(lanes_max<32>(most_v), iv);
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+        const int64_t e = e0 + i * (QBLOCK / R), n = t.n - e;
+#pragma unroll
+        for (int j = 0; j < E; j++) {
+            m[i][j] *= im;
+            const float q = v[i][j] * iv, least = q < QMIN ? QMIN : q;  // (a NaN stays one)
+            v[i][j] = v[i][j] == 0.0f ? 0.0f : least;
+        }
+        store_upto<T, E, NT>((T*)t.p + e, n, p[i]);
+        store8<E, NT>((uint8_t*)t.m + e, n, pack8(m[i]));
+        store8<E, NT>((uint8_t*)t.v + e, n, pack8(v[i]));
+    }
+    if (on && (threadIdx.x & 31) == 0) t.ms[b] = sm, t.vs[b] = sv;
 }
 
 // partial[blockIdx.x] = sum g^2 over `chunk` elements of a tensor, in double
@@ -179,12 +234,16 @@ __global__ void __launch_bounds__(256) k_sumsq(Group a, int64_t chunk, double* p
     const T* g = (const T*)a.t[k].g;
     const int64_t e0 = (int64_t)(blockIdx.x - a.first[k]) * chunk;
     const int64_t e1 = e0 + chunk < a.t[k].n ? e0 + chunk : a.t[k].n;
+    constexpr int E = 16 / sizeof(T), U = 4;
     double x = 0.0;
-    for (int64_t e = e0 + threadIdx.x * 4; e < e1; e += 1024) {
-        float f[4];
-        load_upto(g + e, e1 - e, 0.0f, f);
+    for (int64_t b = e0 + threadIdx.x * E; b < e1; b += 256 * E * U) {
+        float f[U][E];
 #pragma unroll
-        for (int j = 0; j < 4; j++) x = fma((double)f[j], (double)f[j], x);
+        for (int u = 0; u < U; u++) load_upto(g + b + u * 256 * E, e1 - b - u * 256 * E, 0.0f, f[u]);
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int j = 0; j < E; j++) x = fma((double)f[u][j], (double)f[u][j], x);
     }
     for (int o = 32; o >= 1; o >>= 1) x += __shfl_xor(x, o);
     if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = x;
@@ -208,19 +267,19 @@ __global__ void __launch_bounds__(1024) k_clip_coef(const double* partial, int64
     *coef = c < 1.0f || c != c ? c : 1.0f;  // (a NaN norm reaches every gradient, as in clip_grad_norm_)
 }
 
-// what follows from a step count (and a learning rate) on the device: dyn = {step_size, bc2_sqrt, keep}
+// what follows from a step count (and a learning rate) on the device: dyn = {step_size, inv_bc2, keep}
 __global__ void __launch_bounds__(64) k_count_step(float* step, const float* lr_dev, double lr, double b1, double b2, double wd,
                                                    float* dyn) {
     if (threadIdx.x) return;
     const double t = (double)*step + 1.0, rate = lr_dev ? (double)*lr_dev : lr;
     *step = (float)t;
     dyn[0] = (float)(rate / (1.0 - pow(b1, t)));
-    dyn[1] = (float)sqrt(1.0 - pow(b2, t));
+    dyn[1] = (float)(1.0 / sqrt(1.0 - pow(b2, t)));
     dyn[2] = (float)(1.0 - rate * wd);
 }
 
 // elements a block of k_sumsq takes: about 4096 blocks in all
-int64_t norm_chunk(int64_t total) { return cdiv(cdiv(total, 4096), CHUNK) * CHUNK; }
+int64_t norm_chunk(int64_t total) { return cdiv(cdiv(total, 4096), 8192) * 8192; }
 
 int64_t norm_parts(int32_t count, const int64_t* numel) {
     int64_t total = 0, parts = 0;
@@ -229,6 +288,21 @@ int64_t norm_parts(int32_t count, const int64_t* numel) {
     const int64_t chunk = norm_chunk(total);
     for (int i = 0; i < count; i++) parts += cdiv(numel[i], chunk);
     return parts;
+}
+
+// from this many elements on nothing of one step is left in the caches for the next: the streaming hint then
+constexpr int64_t NT_ELEMENTS = 8 << 20;
+
+template <typename T>
+void go_step(const Group& a, const Hyper& h, uint32_t blocks, bool q, bool far, hipStream_t st) {
+    const dim3 g(blocks), b(256);
+    if (q) {
+        if (far) hipLaunchKernelGGL((k_adamw8<T, true>), g, b, 0, st, a, h);
+        else hipLaunchKernelGGL((k_adamw8<T, false>), g, b, 0, st, a, h);
+    } else {
+        if (far) hipLaunchKernelGGL((k_adamw32<T, true>), g, b, 0, st, a, h);
+        else hipLaunchKernelGGL((k_adamw32<T, false>), g, b, 0, st, a, h);
+    }
 }
 
 const char* bad_tensors(const char* who, int32_t count, const void* const* grads, const int64_t* numel, const int32_t* dtypes,
@@ -345,25 +419,19 @@ extern "C" int ec_adamw_step(int32_t count, void* const* params, const void* con
         hipLaunchKernelGGL(k_count_step, dim3(1), dim3(64), 0, st, step_dev, lr_dev, lr, beta1, beta2, weight_decay, dyn);
     } else {
         h.step_size = (float)(lr / (1.0 - pow(beta1, step_host)));
-        h.bc2_sqrt = (float)sqrt(1.0 - pow(beta2, step_host));
+        h.inv_bc2 = (float)(1.0 / sqrt(1.0 - pow(beta2, step_host)));
         h.keep = (float)(1.0 - lr * weight_decay);
     }
+    const bool far = total >= NT_ELEMENTS;
     each_group(count, numel, dtypes, CHUNK,
                [&](int i) {
                    return Tensor{params[i], exp_avg[i], exp_avg_sq[i], grads[i], q ? exp_avg_scale[i] : nullptr,
                                  q ? exp_avg_sq_scale[i] : nullptr, numel[i]};
                },
                [&](int type, const Group& a, uint32_t blocks) {
-                   const dim3 g(blocks), b(256);
-                   if (q) {
-                       if (type == EC_F32) hipLaunchKernelGGL(k_adamw8<float>, g, b, 0, st, a, h);
-                       if (type == EC_BF16) hipLaunchKernelGGL(k_adamw8<bf16>, g, b, 0, st, a, h);
-                       if (type == EC_F16) hipLaunchKernelGGL(k_adamw8<f16>, g, b, 0, st, a, h);
-                   } else {
-                       if (type == EC_F32) hipLaunchKernelGGL(k_adamw32<float>, g, b, 0, st, a, h);
-                       if (type == EC_BF16) hipLaunchKernelGGL(k_adamw32<bf16>, g, b, 0, st, a, h);
-                       if (type == EC_F16) hipLaunchKernelGGL(k_adamw32<f16>, g, b, 0, st, a, h);
-                   }
+                   if (type == EC_F32) go_step<float>(a, h, blocks, q, far, st);
+                   if (type == EC_BF16) go_step<bf16>(a, h, blocks, q, far, st);
+                   if (type == EC_F16) go_step<f16>(a, h, blocks, q, far, st);
                });
     EC_HIP(hipGetLastError());
     return EC_OK;

@@ -58,7 +58,7 @@ __device__ __forceinline__ void row_sum2(float& a, float& b, float2 (*s)[16], in
     }
 }
 
-template <typename T, int TPR, int NV>
+template <typename T, int TPR, int NV, bool NT>
 __global__ void __launch_bounds__(block_threads(TPR)) k_ln_fwd(NormArgs p) {
     constexpr int V = 16 / sizeof(T), RPB = block_threads(TPR) / TPR;
     __shared__ float2 s_red[2][16];
@@ -82,17 +82,24 @@ __global__ void __launch_bounds__(block_threads(TPR)) k_ln_fwd(NormArgs p) {
     int slot = 0;
     // (every thread of a block makes every round: the lane sums and barriers are for all; rows behind the last are read
     // as the last and not written)
-    for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < p.rows; r0 += (int64_t)gridDim.x * RPB, slot ^= 1) {
-        const bool on = r0 + g < p.rows;
-        const int64_t r = on ? r0 + g : p.rows - 1;
-        const T* x = (const T*)p.x + r * p.x_stride;
-        float f[NV][V];
-        float sum = 0.0f;
+    raw_t<T, V> next[NV];
+    const auto fetch = [&](int64_t r0) {
+        const T* x = (const T*)p.x + (r0 + g < p.rows ? r0 + g : p.rows - 1) * p.x_stride;
 #pragma unroll
         for (int i = 0; i < NV; i++) {
             const int c = (i * TPR + t) * V;
-            load_upto(x + c, (int64_t)p.cols - c, 0.0f, f[i]);
+            next[i] = load_raw_upto<NT, T, V>(x + c, p.cols - c);
         }
+    };
+    fetch((int64_t)blockIdx.x * RPB);
+    for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < p.rows; r0 += (int64_t)gridDim.x * RPB, slot ^= 1) {
+        const bool on = r0 + g < p.rows;
+        const int64_t r = r0 + g;
+        float f[NV][V];
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; i++) widen<T, V>(next[i], f[i]);
+        if (r0 + (int64_t)gridDim.x * RPB < p.rows) fetch(r0 + (int64_t)gridDim.x * RPB);  // (while this row is worked on)
 #pragma unroll
         for (int i = 0; i < NV; i++)
 #pragma unroll
@@ -140,7 +147,7 @@ __global__ void __launch_bounds__(block_threads(TPR)) k_ln_fwd(NormArgs p) {
                 const int c = (i * TPR + t) * V;
 #pragma unroll
                 for (int j = 0; j < V; j++) f[i][j] = __builtin_fmaf((f[i][j] - mean) * rstd, w[i][j], b[i][j]);
-                store_upto(y + c, (int64_t)p.cols - c, f[i]);
+                store_upto<T, V, NT>(y + c, p.cols - c, f[i]);
             }
             if (t == 0) {
                 if (p.mean) p.mean[r] = mean;
@@ -150,7 +157,7 @@ __global__ void __launch_bounds__(block_threads(TPR)) k_ln_fwd(NormArgs p) {
     }
 }
 
-template <typename T, int TPR, int NV>
+template <typename T, int TPR, int NV, bool NT>
 __global__ void __launch_bounds__(block_threads(TPR)) k_ln_bwd(NormArgs p) {
     constexpr int V = 16 / sizeof(T), RPB = block_threads(TPR) / TPR;
     __shared__ float2 s_red[2][16];
@@ -165,19 +172,33 @@ __global__ void __launch_bounds__(block_threads(TPR)) k_ln_bwd(NormArgs p) {
     }
     const float inv_c = 1.0f / (float)p.cols;
     int slot = 0;
-    for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < p.rows; r0 += (int64_t)gridDim.x * RPB, slot ^= 1) {
+    raw_t<T, V> next_x[NV], next_dy[NV];
+    float next_mean, next_rstd;
+    const auto fetch = [&](int64_t r0) {
         const bool on = r0 + g < p.rows;
         const int64_t r = on ? r0 + g : p.rows - 1;
         const T *x = (const T*)p.x + r * p.x_stride, *dy = (const T*)p.dy + r * p.dy_stride;
-        float h[NV][V], d[NV][V];
         // a row behind the last adds nothing to dw and db: its dy is taken as 0
 #pragma unroll
         for (int i = 0; i < NV; i++) {
             const int c = (i * TPR + t) * V;
-            load_upto(x + c, (int64_t)p.cols - c, 0.0f, h[i]);
-            load_upto(dy + c, on ? (int64_t)p.cols - c : 0, 0.0f, d[i]);
+            next_x[i] = load_raw_upto<NT, T, V>(x + c, p.cols - c);
+            next_dy[i] = load_raw_upto<NT, T, V>(dy + c, on ? p.cols - c : 0);
         }
-        const float mean = p.mean[r], rstd = p.rstd[r];
+        next_mean = p.mean[r], next_rstd = p.rstd[r];
+    };
+    fetch((int64_t)blockIdx.x * RPB);
+    for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < p.rows; r0 += (int64_t)gridDim.x * RPB, slot ^= 1) {
+        const bool on = r0 + g < p.rows;
+        const int64_t r = r0 + g;
+        float h[NV][V], d[NV][V];
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            widen<T, V>(next_x[i], h[i]);
+            widen<T, V>(next_dy[i], d[i]);
+        }
+        const float mean = next_mean, rstd = next_rstd;
+        if (r0 + (int64_t)gridDim.x * RPB < p.rows) fetch(r0 + (int64_t)gridDim.x * RPB);  // (while this row is worked on)
         float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; i++)
@@ -202,7 +223,7 @@ __global__ void __launch_bounds__(block_threads(TPR)) k_ln_bwd(NormArgs p) {
                 float o[V];
 #pragma unroll
                 for (int j = 0; j < V; j++) o[j] = rstd * (d[i][j] - s1 - h[i][j] * s2);
-                store_upto(dx + c, (int64_t)p.cols - c, o);
+                store_upto<T, V, NT>(dx + c, p.cols - c, o);
             }
         }
     }
@@ -243,7 +264,13 @@ __global__ void __launch_bounds__(1024) k_ln_wgrad(const float* partials, int n,
     const int c = blockIdx.x * 64 + (threadIdx.x & 63), l = threadIdx.x >> 6;
     float a = 0.0f;
     if (c < cols && out)
-        for (int k = l; k < n; k += 16) a += partials[((int64_t)k * 2 + blockIdx.y) * cols + c];
+        for (int k = l; k < n; k += 16 * 8) {
+            float f[8];  // (eight loads in flight: this kernel is nothing but their latency)
+#pragma unroll
+            for (int u = 0; u < 8; u++) f[u] = k + 16 * u < n ? partials[((int64_t)(k + 16 * u) * 2 + blockIdx.y) * cols + c] : 0.0f;
+#pragma unroll
+            for (int u = 0; u < 8; u++) a += f[u];
+        }
     s[l][threadIdx.x & 63] = a;
     __syncthreads();
     if (l == 0 && c < cols && out) {
@@ -352,16 +379,16 @@ __global__ void __launch_bounds__(64) k_ln_dw_wide(NormArgs p) {
     store_upto(part + p.cols + c, p.cols - c, db);
 }
 
-// ---- which variant: the fewest threads per row that hold it in at most 16 registers of values each ----
+// ---- which variant: the fewest threads per row that hold it in one vector each; two or four beyond 1024 threads ----
 struct Shape {
     int tpr, nv, rpb;  // tpr 0: the wide kernels
 };
 Shape shape_for(int64_t cols, int dtype) {
     const int64_t vecs = cdiv(cols, dtype == EC_F32 ? 4 : 8);
-    const int most = dtype == EC_F32 ? 4 : 2;  // vectors a thread
-    for (int tpr : {8, 16, 32, 64, 256, 512, 1024})
-        for (int nv = 1; nv <= most; nv *= 2)
-            if (vecs <= (int64_t)tpr * nv && (nv == 1 || tpr >= 64)) return {tpr, nv, block_threads(tpr) / tpr};
+    for (int tpr : {8, 16, 32, 64, 128, 256, 512, 1024})
+        if (vecs <= tpr) return tpr == 128 ? Shape{64, 2, 4} : Shape{tpr, 1, block_threads(tpr) / tpr};
+    if (vecs <= 2048) return {1024, 2, 1};
+    if (vecs <= 4096 && dtype == EC_F32) return {1024, 4, 1};
     return {0, 0, 1};
 }
 
@@ -371,25 +398,28 @@ int bwd_blocks(const Shape& s, int64_t rows) {
 }
 int wide_parts(int64_t rows) { return (int)(rows < 32 ? rows : 32); }
 
+// from this many elements on nothing of a tensor is left in the caches for who reads it next: the streaming hint then
+constexpr int64_t NT_ELEMENTS = 32 << 20;
+
 template <typename T, bool BWD, int TPR, int NV>
 void go(const NormArgs& a, unsigned blocks, hipStream_t st) {
-    if constexpr (BWD)
-        hipLaunchKernelGGL((k_ln_bwd<T, TPR, NV>), dim3(blocks), dim3(block_threads(TPR)), 0, st, a);
-    else
-        hipLaunchKernelGGL((k_ln_fwd<T, TPR, NV>), dim3(blocks), dim3(block_threads(TPR)), 0, st, a);
+    const dim3 g(blocks), b(block_threads(TPR));
+    const bool far = a.rows * a.cols >= NT_ELEMENTS;
+    if constexpr (BWD) {
+        if (far) hipLaunchKernelGGL((k_ln_bwd<T, TPR, NV, true>), g, b, 0, st, a);
+        else hipLaunchKernelGGL((k_ln_bwd<T, TPR, NV, false>), g, b, 0, st, a);
+    } else {
+        if (far) hipLaunchKernelGGL((k_ln_fwd<T, TPR, NV, true>), g, b, 0, st, a);
+        else hipLaunchKernelGGL((k_ln_fwd<T, TPR, NV, false>), g, b, 0, st, a);
+    }
 }
 
 template <typename T, bool BWD>
 void dispatch(const NormArgs& a, const Shape& s, unsigned blocks, hipStream_t st) {
-    constexpr int MOST = sizeof(T) == 4 ? 4 : 2;
-#define EC_LN(TPR, NV)                                       \
-    if constexpr (NV <= MOST)                                \
-        if (s.tpr == TPR && s.nv == NV) return go<T, BWD, TPR, NV>(a, blocks, st);
-    EC_LN(8, 1) EC_LN(16, 1) EC_LN(32, 1)
-    EC_LN(64, 1) EC_LN(64, 2) EC_LN(64, 4)
-    EC_LN(256, 1) EC_LN(256, 2) EC_LN(256, 4)
-    EC_LN(512, 1) EC_LN(512, 2) EC_LN(512, 4)
-    EC_LN(1024, 1) EC_LN(1024, 2) EC_LN(1024, 4)
+#define EC_LN(TPR, NV) \
+    if (s.tpr == TPR && s.nv == NV) return go<T, BWD, TPR, NV>(a, blocks, st);
+    EC_LN(8, 1) EC_LN(16, 1) EC_LN(32, 1) EC_LN(64, 1) EC_LN(64, 2) EC_LN(256, 1) EC_LN(512, 1) EC_LN(1024, 1) EC_LN(1024, 2)
+    if constexpr (sizeof(T) == 4) { EC_LN(1024, 4) }
 #undef EC_LN
 }
 

@@ -18,35 +18,63 @@ struct vec_of {
 };
 
 template <typename T, int N>
-__device__ __forceinline__ void load_n(const T* p, float (&f)[N]) {
-    const typename vec_of<T, N>::raw v = *reinterpret_cast<const typename vec_of<T, N>::type*>(p);
+using raw_t = typename vec_of<T, N>::raw;
+
+// NT: with the streaming hint, for what is read or written once (a read of 1 GB runs at 7.0 TB/s with it, 6.25 without; a copy
+// at 6.4 against 6.2)
+template <bool NT, typename T, int N>
+__device__ __forceinline__ raw_t<T, N> load_raw(const T* p) {
+    typedef typename vec_of<T, N>::type any;
+    if (NT) return __builtin_nontemporal_load(reinterpret_cast<const any*>(p));
+    return *reinterpret_cast<const any*>(p);
+}
+template <bool NT, typename T, int N>
+__device__ __forceinline__ void store_raw(T* p, raw_t<T, N> v) {
+    typedef typename vec_of<T, N>::type any;
+    if (NT) __builtin_nontemporal_store(v, reinterpret_cast<any*>(p));
+    else *reinterpret_cast<any*>(p) = v;
+}
+// the first n of N (n may be anything; n <= 0: nothing is touched), the others 0
+template <bool NT, typename T, int N>
+__device__ __forceinline__ raw_t<T, N> load_raw_upto(const T* p, int64_t n) {
+    if (n >= N) return load_raw<NT, T, N>(p);
+    raw_t<T, N> v;
+#pragma unroll
+    for (int j = 0; j < N; j++) v[j] = j < n ? p[j] : (T)0.0f;
+    return v;
+}
+template <typename T, int N>
+__device__ __forceinline__ void widen(raw_t<T, N> v, float (&f)[N]) {
 #pragma unroll
     for (int j = 0; j < N; j++) f[j] = (float)v[j];
 }
 
-template <typename T, int N>
+template <typename T, int N, bool NT = false>
+__device__ __forceinline__ void load_n(const T* p, float (&f)[N]) {
+    widen<T, N>(load_raw<NT, T, N>(p), f);
+}
+template <typename T, int N, bool NT = false>
 __device__ __forceinline__ void store_n(T* p, const float (&f)[N]) {
-    typename vec_of<T, N>::raw v;
+    raw_t<T, N> v;
 #pragma unroll
     for (int j = 0; j < N; j++) v[j] = (T)f[j];
-    *reinterpret_cast<typename vec_of<T, N>::type*>(p) = v;
+    store_raw<NT, T, N>(p, v);
 }
 
-// the same for the first n of N (n may be anything; n <= 0: nothing is touched)
-template <typename T, int N>
+// the same for the first n of N
+template <typename T, int N, bool NT = false>
 __device__ __forceinline__ void load_upto(const T* p, int64_t n, float fill, float (&f)[N]) {
     if (n >= N) {
-        load_n(p, f);
+        load_n<T, N, NT>(p, f);
     } else {
 #pragma unroll
         for (int j = 0; j < N; j++) f[j] = j < n ? (float)p[j] : fill;
     }
 }
-
-template <typename T, int N>
+template <typename T, int N, bool NT = false>
 __device__ __forceinline__ void store_upto(T* p, int64_t n, const float (&f)[N]) {
     if (n >= N) {
-        store_n(p, f);
+        store_n<T, N, NT>(p, f);
     } else {
 #pragma unroll
         for (int j = 0; j < N; j++)
