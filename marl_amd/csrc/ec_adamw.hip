@@ -83,16 +83,13 @@ struct Take {
     static constexpr int EACH = sizeof(T) == 4 ? 4 : 8, RUNS = 8 / EACH;
 };
 
-template <typename T, bool NT>
-__global__ void __launch_bounds__(256) k_adamw32(Group a, Hyper h) {
+template <typename T, bool NT, bool FULL>
+__device__ __forceinline__ void adamw32(const Tensor& t, int64_t e0, Hyper& h) {
     constexpr int E = Take<T>::EACH, R = Take<T>::RUNS;
-    const int k = tensor_of(a, blockIdx.x);
-    const Tensor t = a.t[k];
-    const int64_t e0 = (int64_t)(blockIdx.x - a.first[k]) * CHUNK + threadIdx.x * E;
     float p[R][E], g[R][E], m[R][E], v[R][E], root;
 #pragma unroll
     for (int i = 0; i < R; i++) {
-        const int64_t e = e0 + i * (CHUNK / R), n = t.n - e;
+        const int64_t e = e0 + i * (CHUNK / R), n = FULL ? E : t.n - e;
         load_upto<T, E, NT>((const T*)t.g + e, n, 0.0f, g[i]);
         load_upto<float, E, NT>((const float*)t.m + e, n, 0.0f, m[i]);
         load_upto<float, E, NT>((const float*)t.v + e, n, 0.0f, v[i]);
@@ -105,11 +102,20 @@ __global__ void __launch_bounds__(256) k_adamw32(Group a, Hyper h) {
         for (int j = 0; j < E; j++) adam(h, coef, g[i][j], p[i][j], m[i][j], v[i][j], root);
 #pragma unroll
     for (int i = 0; i < R; i++) {
-        const int64_t e = e0 + i * (CHUNK / R), n = t.n - e;
+        const int64_t e = e0 + i * (CHUNK / R), n = FULL ? E : t.n - e;
         store_upto<T, E, NT>((T*)t.p + e, n, p[i]);
         store_upto<float, E, NT>((float*)t.m + e, n, m[i]);
         store_upto<float, E, NT>((float*)t.v + e, n, v[i]);
     }
+}
+
+template <typename T, bool NT>
+__global__ void __launch_bounds__(256) k_adamw32(Group a, Hyper h) {
+    const int k = tensor_of(a, blockIdx.x);
+    const Tensor t = a.t[k];
+    const int64_t b0 = (int64_t)(blockIdx.x - a.first[k]) * CHUNK, e0 = b0 + threadIdx.x * Take<T>::EACH;
+    if (b0 + CHUNK <= t.n) adamw32<T, NT, true>(t, e0, h);
+    else adamw32<T, NT, false>(t, e0, h);
 }
 
 // N e4m3 values of N bytes at any address (N = 4, 8), the first n of them; the others 0 / untouched
@@ -173,19 +179,17 @@ __device__ __forceinline__ float scale_of(float most, float& inv) {
     return s;
 }
 
-// half a wave takes the 256 elements of a scale
-template <typename T, bool NT>
-__global__ void __launch_bounds__(256) k_adamw8(Group a, Hyper h) {
+// half a wave takes the 256 elements of a scale, the b-th of the tensor
+template <typename T, bool NT, bool FULL>
+__device__ __forceinline__ void adamw8(const Tensor& t, int64_t b, Hyper& h) {
     constexpr int E = Take<T>::EACH, R = Take<T>::RUNS;
-    const int k = tensor_of(a, blockIdx.x);
-    const Tensor t = a.t[k];
-    const int64_t b = (int64_t)(blockIdx.x - a.first[k]) * (CHUNK / QBLOCK) + threadIdx.x / 32, e0 = b * QBLOCK + (threadIdx.x & 31) * E;
-    const bool on = b * QBLOCK < t.n;
+    const int64_t e0 = b * QBLOCK + (threadIdx.x & 31) * E;
+    const bool on = FULL || b * QBLOCK < t.n;
     float p[R][E], g[R][E], m[R][E], v[R][E];
     Bytes<E> qm[R], qv[R];
 #pragma unroll
     for (int i = 0; i < R; i++) {
-        const int64_t e = e0 + i * (QBLOCK / R), n = t.n - e;
+        const int64_t e = e0 + i * (QBLOCK / R), n = FULL ? E : t.n - e;
         load_upto<T, E, NT>((const T*)t.g + e, n, 0.0f, g[i]);
         qm[i] = load8<E, NT>((const uint8_t*)t.m + e, n);
         qv[i] = load8<E, NT>((const uint8_t*)t.v + e, n);
@@ -212,7 +216,7 @@ __global__ void __launch_bounds__(256) k_adamw8(Group a, Hyper h) {
     const float sm = scale_of(lanes_max<32>(most_m), im), sv = scale_of(lanes_max<32>(most_v), iv);
 #pragma unroll
     for (int i = 0; i < R; i++) {
-        const int64_t e = e0 + i * (QBLOCK / R), n = t.n - e;
+        const int64_t e = e0 + i * (QBLOCK / R), n = FULL ? E : t.n - e;
 #pragma unroll
         for (int j = 0; j < E; j++) {
             m[i][j] *= im;
@@ -224,6 +228,15 @@ __global__ void __launch_bounds__(256) k_adamw8(Group a, Hyper h) {
         store8<E, NT>((uint8_t*)t.v + e, n, pack8(v[i]));
     }
     if (on && (threadIdx.x & 31) == 0) t.ms[b] = sm, t.vs[b] = sv;
+}
+
+template <typename T, bool NT>
+__global__ void __launch_bounds__(256) k_adamw8(Group a, Hyper h) {
+    const int k = tensor_of(a, blockIdx.x);
+    const Tensor t = a.t[k];
+    const int64_t c = blockIdx.x - a.first[k], b = c * (CHUNK / QBLOCK) + threadIdx.x / 32;
+    if ((c + 1) * CHUNK <= t.n) adamw8<T, NT, true>(t, b, h);
+    else adamw8<T, NT, false>(t, b, h);
 }
 
 // partial[blockIdx.x] = sum g^2 over `chunk` elements of a tensor, in double
@@ -238,8 +251,13 @@ __global__ void __launch_bounds__(256) k_sumsq(Group a, int64_t chunk, double* p
     double x = 0.0;
     for (int64_t b = e0 + threadIdx.x * E; b < e1; b += 256 * E * U) {
         float f[U][E];
+        if (b - threadIdx.x * E + 256 * E * U <= e1) {
 #pragma unroll
-        for (int u = 0; u < U; u++) load_upto(g + b + u * 256 * E, e1 - b - u * 256 * E, 0.0f, f[u]);
+            for (int u = 0; u < U; u++) load_n(g + b + u * 256 * E, f[u]);
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; u++) load_upto(g + b + u * 256 * E, e1 - b - u * 256 * E, 0.0f, f[u]);
+        }
 #pragma unroll
         for (int u = 0; u < U; u++)
 #pragma unroll

@@ -116,32 +116,34 @@ __device__ __forceinline__ const char* mask_of(const LpArgs& p, int64_t r) {
     return (const char*)p.avail + ((r / p.inner) * p.a_outer + (r % p.inner) * p.a_inner) * (MASK == 1 ? 1 : 4);
 }
 
-// the n first of the N logits at l + c, the others and the excluded as -inf
-template <typename T, int MASK, int N>
-__device__ __forceinline__ void load_logits(const T* l, const char* av, int64_t c, int64_t n, float (&f)[N]) {
-    load_upto(l + c, n, -INF, f);
-    if (MASK == 0) return;
-    if (n >= N) {
-        if (MASK == 1) {
-            typedef uint8_t bytes __attribute__((ext_vector_type(N)));
-            typedef bytes ubytes __attribute__((aligned(1)));
-            const bytes b = *reinterpret_cast<const ubytes*>(av + c);
+// U vectors of N logits from l + c on, `step` apart, those from column c1 on and the excluded as -inf.  FULL: all of them lie
+// below c1 (the loads then stand together, with no branch between them)
+template <typename T, int MASK, bool NT, bool FULL, int UU, int N>
+__device__ __forceinline__ void load_logits(const T* l, const char* av, int64_t c, int64_t step, int64_t c1, float (&f)[UU][N]) {
+    raw_t<T, N> raw[UU];
+    raw_t<uint8_t, N> b[MASK == 1 ? UU : 1];
+    raw_t<int32_t, 4> w[MASK == 2 ? UU : 1][N / 4];
 #pragma unroll
-            for (int j = 0; j < N; j++) f[j] = b[j] ? f[j] : -INF;
-        } else {
-            typedef int32_t ints __attribute__((ext_vector_type(4)));
-            typedef ints uints __attribute__((aligned(4)));
+    for (int u = 0; u < UU; u++) {
+        const int64_t at = c + u * step, n = FULL ? N : c1 - at;
+        raw[u] = load_raw_upto<NT, T, N>(l + at, n);
+        if (MASK == 1) b[MASK == 1 ? u : 0] = load_raw_upto<NT, uint8_t, N>((const uint8_t*)av + at, n);
+        if (MASK == 2)
 #pragma unroll
-            for (int q = 0; q < N / 4; q++) {
-                const ints b = *reinterpret_cast<const uints*>(av + (c + 4 * q) * 4);
+            for (int q = 0; q < N / 4; q++)
+                w[MASK == 2 ? u : 0][q] = load_raw_upto<NT, int32_t, 4>((const int32_t*)av + at + 4 * q, n - 4 * q);
+    }
 #pragma unroll
-                for (int j = 0; j < 4; j++) f[4 * q + j] = b[j] ? f[4 * q + j] : -INF;
-            }
+    for (int u = 0; u < UU; u++) {
+        widen<T, N>(raw[u], f[u]);
+        const int64_t n = FULL ? N : c1 - (c + u * step);
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            bool on = FULL || j < n;
+            if (MASK == 1) on = b[MASK == 1 ? u : 0][j] != 0;  // (behind the last: 0)
+            if (MASK == 2) on = w[MASK == 2 ? u : 0][j / 4][j % 4] != 0;
+            f[u][j] = on ? f[u][j] : -INF;
         }
-    } else {
-#pragma unroll
-        for (int j = 0; j < N; j++)
-            if (j < n && !(MASK == 1 ? av[c + j] != 0 : ((const int32_t*)av)[c + j] != 0)) f[j] = -INF;
     }
 }
 
@@ -196,7 +198,7 @@ __device__ __forceinline__ void finish_row(const LpArgs& p, int64_t r, int t, co
 }
 
 // TPR threads a row: 16 or 64 (each row once), or a block of 256 per row or split of a row
-template <typename T, int MASK, bool TOP, int TPR>
+template <typename T, int MASK, bool TOP, int TPR, bool NT>
 __global__ void __launch_bounds__(256) k_logp_fwd(LpArgs p) {
     constexpr int V = 16 / sizeof(T), W = TPR < 64 ? TPR : 64;
     __shared__ Stat s_stat[4];
@@ -217,11 +219,8 @@ __global__ void __launch_bounds__(256) k_logp_fwd(LpArgs p) {
     for (int64_t b = c0; b < c1; b += TPR * V * U) {  // (the same rounds for every thread: the lists need whole waves)
         float f[U][V];
         float top_f = -INF;
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int64_t c = b + (u * TPR + t) * V;
-            load_logits<T, MASK>(l, av, c, c1 - c, f[u]);
-        }
+        if (b + TPR * V * U <= c1) load_logits<T, MASK, NT, true>(l, av, b + t * V, TPR * V, c1, f);
+        else load_logits<T, MASK, NT, false>(l, av, b + t * V, TPR * V, c1, f);
 #pragma unroll
         for (int u = 0; u < U; u++)
 #pragma unroll
@@ -320,7 +319,7 @@ __device__ __forceinline__ float entry_grad(const RowGrad& w, float l, int64_t c
 }
 
 // TPR threads a row: 16 or 64 for a whole row, or a block of 256 per TPR * V * U columns of a row
-template <typename T, int MASK, int TPR>
+template <typename T, int MASK, int TPR, bool NT>
 __global__ void __launch_bounds__(256) k_logp_bwd(LpArgs p) {
     constexpr int V = 16 / sizeof(T);
     const int64_t r = TPR == 256 ? blockIdx.x / p.splits : (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
@@ -334,17 +333,15 @@ __global__ void __launch_bounds__(256) k_logp_bwd(LpArgs p) {
     const int t = threadIdx.x % TPR;
     for (int64_t b = c0; b < c1; b += TPR * V * U) {
         float f[U][V];
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int64_t c = b + (u * TPR + t) * V;
-            load_logits<T, MASK>(l, av, c, c1 - c, f[u]);
-        }
+        const bool full = b + TPR * V * U <= c1;
+        if (full) load_logits<T, MASK, NT, true>(l, av, b + t * V, TPR * V, c1, f);
+        else load_logits<T, MASK, NT, false>(l, av, b + t * V, TPR * V, c1, f);
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int64_t c = b + (u * TPR + t) * V;
 #pragma unroll
             for (int j = 0; j < V; j++) f[u][j] = entry_grad(w, f[u][j], c + j);
-            store_upto(out + c, c1 - c, f[u]);
+            store_upto<T, V, NT>(out + c, full ? V : c1 - c, f[u]);
         }
     }
 }
@@ -366,8 +363,9 @@ __device__ __forceinline__ void stage_rows(const LpArgs& p, int64_t r0, int n, i
         const char* av = MASK ? (const char*)p.avail + r0 * p.vocab * (MASK == 1 ? 1 : 4) : nullptr;
         const int all = n * p.vocab;
         for (int i = threadIdx.x * V; i < all; i += 256 * V) {
-            float f[V];
-            load_logits<T, MASK>(l, av, i, all - i, f);
+            float f1[1][V], (&f)[V] = f1[0];
+            if (i + V <= all) load_logits<T, MASK, false, true>(l, av, i, 0, all, f1);
+            else load_logits<T, MASK, false, false>(l, av, i, 0, all, f1);
             int row = row_in(i, p.vocab, by_vocab), col = i - row * p.vocab;
 #pragma unroll
             for (int j = 0; j < V; j++) {
@@ -492,14 +490,14 @@ void go_fwd(const LpArgs& a, int dtype, hipStream_t st) {
     if (tpr == 0) {
         hipLaunchKernelGGL((k_logp_few_fwd<T, MASK>), blocks(256), b, 256 * (a.vocab | 1) * 4, st, a, by_vocab(a.vocab), is_packed(a));
     } else if (tpr == 16) {
-        hipLaunchKernelGGL((k_logp_fwd<T, MASK, false, 16>), blocks(16), b, 0, st, a);
+        hipLaunchKernelGGL((k_logp_fwd<T, MASK, false, 16, false>), blocks(16), b, 0, st, a);
     } else if (tpr == 64) {
-        if (a.top_k) hipLaunchKernelGGL((k_logp_fwd<T, MASK, true, 64>), blocks(4), b, 0, st, a);
-        else hipLaunchKernelGGL((k_logp_fwd<T, MASK, false, 64>), blocks(4), b, 0, st, a);
+        if (a.top_k) hipLaunchKernelGGL((k_logp_fwd<T, MASK, true, 64, false>), blocks(4), b, 0, st, a);
+        else hipLaunchKernelGGL((k_logp_fwd<T, MASK, false, 64, false>), blocks(4), b, 0, st, a);
     } else {
         const dim3 grid((unsigned)(a.rows * a.splits));
-        if (a.top_k) hipLaunchKernelGGL((k_logp_fwd<T, MASK, true, 256>), grid, b, 0, st, a);
-        else hipLaunchKernelGGL((k_logp_fwd<T, MASK, false, 256>), grid, b, 0, st, a);
+        if (a.top_k) hipLaunchKernelGGL((k_logp_fwd<T, MASK, true, 256, true>), grid, b, 0, st, a);
+        else hipLaunchKernelGGL((k_logp_fwd<T, MASK, false, 256, true>), grid, b, 0, st, a);
         if (a.splits > 1) hipLaunchKernelGGL((k_logp_join<T, MASK>), dim3((unsigned)a.rows), dim3(64), 0, st, a);
     }
 }
@@ -512,11 +510,11 @@ void go_bwd(const LpArgs& a, int dtype, hipStream_t st) {
     if (tpr == 0)
         hipLaunchKernelGGL((k_logp_few_bwd<T, MASK>), blocks(256), b, 256 * (a.vocab | 1) * 4, st, a, by_vocab(a.vocab), is_packed(a));
     else if (tpr == 16)
-        hipLaunchKernelGGL((k_logp_bwd<T, MASK, 16>), blocks(16), b, 0, st, a);
+        hipLaunchKernelGGL((k_logp_bwd<T, MASK, 16, false>), blocks(16), b, 0, st, a);
     else if (tpr == 64)
-        hipLaunchKernelGGL((k_logp_bwd<T, MASK, 64>), blocks(4), b, 0, st, a);
+        hipLaunchKernelGGL((k_logp_bwd<T, MASK, 64, false>), blocks(4), b, 0, st, a);
     else
-        hipLaunchKernelGGL((k_logp_bwd<T, MASK, 256>), dim3((unsigned)(a.rows * a.splits)), b, 0, st, a);
+        hipLaunchKernelGGL((k_logp_bwd<T, MASK, 256, true>), dim3((unsigned)(a.rows * a.splits)), b, 0, st, a);
 }
 
 #define EC_LP_GO(GO, T)                                  \

@@ -49,19 +49,45 @@ __device__ __forceinline__ void row_sum2(float& a, float& b, float2 (*s)[16], in
     if (TPR > 64) {
         if ((threadIdx.x & 63) == 0) s[slot][threadIdx.x >> 6] = make_float2(a, b);
         __syncthreads();
-        a = b = 0.0f;
+        const float2 v = s[slot][threadIdx.x & (TPR / 64 - 1)];  // (a wave's value in each lane of a group)
+        a = lanes_sum<TPR / 64>(v.x);
+        b = lanes_sum<TPR / 64>(v.y);
+    }
+}
+
+// Vectors of a row, and what of them belongs to it.  A row's last vector is read whole where that stays inside the tensor
+// (it then holds the start of the next row, or padding) and masked: reading it element by element would cost every row a
+// wait of its own.
+template <typename T, int V>
+struct Mask {
+    uint32_t w[4];
+    __device__ __forceinline__ void set(int n) {  // the first n
 #pragma unroll
-        for (int w = 0; w < TPR / 64; w++) {
-            a += s[slot][w].x;
-            b += s[slot][w].y;
+        for (int k = 0; k < 4; k++) {
+            const int left = (n - k * (V / 4)) * (int)sizeof(T) * 8;  // bits of this word
+            w[k] = left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1;
         }
     }
+    __device__ __forceinline__ raw_t<T, V> of(raw_t<T, V> v) const {
+        uint32_t u[4];
+        __builtin_memcpy(u, &v, 16);
+#pragma unroll
+        for (int k = 0; k < 4; k++) u[k] &= w[k];
+        __builtin_memcpy(&v, u, 16);
+        return v;
+    }
+};
+// the vector of column c < cols of a row at `off`; end: the tensor's last element plus one
+template <bool NT, typename T, int V>
+__device__ __forceinline__ raw_t<T, V> row_vector(const T* base, int64_t off, int c, int cols, int64_t end) {
+    if (off + c + V <= end) return load_raw<NT, T, V>(base + off + c);
+    return load_raw_upto<NT, T, V>(base + off + c, cols - c);
 }
 
 template <typename T, int TPR, int NV, bool NT>
 __global__ void __launch_bounds__(block_threads(TPR)) k_ln_fwd(NormArgs p) {
     constexpr int V = 16 / sizeof(T), RPB = block_threads(TPR) / TPR;
-    __shared__ float2 s_red[2][16];
+    __shared__ float4 s_red[2][TPR > 64 ? TPR / 64 : 1];
     const int t = threadIdx.x % TPR, g = threadIdx.x / TPR;
     float w[NV][V], b[NV][V];
 #pragma unroll
@@ -70,25 +96,32 @@ __global__ void __launch_bounds__(block_threads(TPR)) k_ln_fwd(NormArgs p) {
         load_weight<T, V>(p.b, p.wdtype, (i * TPR + t) * V, p.cols, 0.0f, b[i]);
     }
     const float inv_c = 1.0f / (float)p.cols;
-    // columns that this thread's wave holds (TPR > 64)
-    int n_wave = 0;
+    // columns that this thread's wave holds (TPR > 64), as the sum of squares is first taken about the wave's own mean
+    float n_wave = 0.0f, inv_wave = 0.0f;
     if (TPR > 64) {
 #pragma unroll
         for (int i = 0; i < NV; i++) {
             const int left = p.cols - (i * TPR + (t & ~63)) * V;
-            n_wave += left <= 0 ? 0 : left < 64 * V ? left : 64 * V;
+            n_wave += (float)(left <= 0 ? 0 : left < 64 * V ? left : 64 * V);
         }
+        inv_wave = n_wave > 0.0f ? 1.0f / n_wave : 0.0f;
     }
     int slot = 0;
     // (every thread of a block makes every round: the lane sums and barriers are for all; rows behind the last are read
     // as the last and not written)
+    const bool ragged = p.cols % V != 0;
+    Mask<T, V> mask[NV];
+#pragma unroll
+    for (int i = 0; i < NV; i++) mask[i].set(p.cols - (i * TPR + t) * V);
+    const int64_t end = (p.rows - 1) * p.x_stride + p.cols;
     raw_t<T, V> next[NV];
     const auto fetch = [&](int64_t r0) {
-        const T* x = (const T*)p.x + (r0 + g < p.rows ? r0 + g : p.rows - 1) * p.x_stride;
+        const int64_t off = (r0 + g < p.rows ? r0 + g : p.rows - 1) * p.x_stride;
 #pragma unroll
         for (int i = 0; i < NV; i++) {
             const int c = (i * TPR + t) * V;
-            next[i] = load_raw_upto<NT, T, V>(x + c, p.cols - c);
+            next[i] = raw_t<T, V>{};
+            if (c < p.cols) next[i] = row_vector<NT, T, V>((const T*)p.x, off, c, p.cols, end);
         }
     };
     fetch((int64_t)blockIdx.x * RPB);
@@ -98,7 +131,7 @@ __global__ void __launch_bounds__(block_threads(TPR)) k_ln_fwd(NormArgs p) {
         float f[NV][V];
         float sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NV; i++) widen<T, V>(next[i], f[i]);
+        for (int i = 0; i < NV; i++) widen<T, V>(ragged ? mask[i].of(next[i]) : next[i], f[i]);
         if (r0 + (int64_t)gridDim.x * RPB < p.rows) fetch(r0 + (int64_t)gridDim.x * RPB);  // (while this row is worked on)
 #pragma unroll
         for (int i = 0; i < NV; i++)
@@ -106,7 +139,7 @@ __global__ void __launch_bounds__(block_threads(TPR)) k_ln_fwd(NormArgs p) {
             for (int j = 0; j < V; j++) sum += f[i][j];
         sum = lanes_sum<(TPR < 64 ? TPR : 64)>(sum);
         // squares about the mean of the row (TPR <= 64) or of the wave's part of it, then moved to the row's mean
-        const float about = TPR <= 64 ? sum * inv_c : n_wave ? sum / (float)n_wave : 0.0f;
+        const float about = sum * (TPR <= 64 ? inv_c : inv_wave);
         float sq = 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; i++) {
@@ -120,24 +153,11 @@ __global__ void __launch_bounds__(block_threads(TPR)) k_ln_fwd(NormArgs p) {
         sq = lanes_sum<(TPR < 64 ? TPR : 64)>(sq);
         float mean = about;
         if (TPR > 64) {
-            if ((threadIdx.x & 63) == 0) s_red[slot][threadIdx.x >> 6] = make_float2(sum, sq);
+            if ((threadIdx.x & 63) == 0) s_red[slot][threadIdx.x >> 6] = make_float4(sum, about, sq, n_wave);
             __syncthreads();
-            float tot = 0.0f;
-#pragma unroll
-            for (int k = 0; k < TPR / 64; k++) tot += s_red[slot][k].x;
-            mean = tot * inv_c;
-            sq = 0.0f;
-#pragma unroll
-            for (int k = 0; k < TPR / 64; k++) {
-                int n = 0;
-#pragma unroll
-                for (int i = 0; i < NV; i++) {
-                    const int left = p.cols - (i * TPR + k * 64) * V;
-                    n += left <= 0 ? 0 : left < 64 * V ? left : 64 * V;
-                }
-                const float off = n ? s_red[slot][k].x / (float)n - mean : 0.0f;
-                sq += s_red[slot][k].y + (float)n * off * off;
-            }
+            const float4 v = s_red[slot][threadIdx.x & (TPR / 64 - 1)];
+            mean = lanes_sum<TPR / 64>(v.x) * inv_c;
+            sq = lanes_sum<TPR / 64>(v.z + v.w * (v.y - mean) * (v.y - mean));
         }
         const float rstd = 1.0f / sqrtf(sq * inv_c + p.eps);
         if (on) {
@@ -172,18 +192,25 @@ __global__ void __launch_bounds__(block_threads(TPR)) k_ln_bwd(NormArgs p) {
     }
     const float inv_c = 1.0f / (float)p.cols;
     int slot = 0;
+    const bool ragged = p.cols % V != 0;
+    Mask<T, V> mask[NV];
+#pragma unroll
+    for (int i = 0; i < NV; i++) mask[i].set(p.cols - (i * TPR + t) * V);
+    const int64_t end_x = (p.rows - 1) * p.x_stride + p.cols, end_dy = (p.rows - 1) * p.dy_stride + p.cols;
     raw_t<T, V> next_x[NV], next_dy[NV];
     float next_mean, next_rstd;
     const auto fetch = [&](int64_t r0) {
         const bool on = r0 + g < p.rows;
         const int64_t r = on ? r0 + g : p.rows - 1;
-        const T *x = (const T*)p.x + r * p.x_stride, *dy = (const T*)p.dy + r * p.dy_stride;
         // a row behind the last adds nothing to dw and db: its dy is taken as 0
 #pragma unroll
         for (int i = 0; i < NV; i++) {
             const int c = (i * TPR + t) * V;
-            next_x[i] = load_raw_upto<NT, T, V>(x + c, p.cols - c);
-            next_dy[i] = load_raw_upto<NT, T, V>(dy + c, on ? p.cols - c : 0);
+            next_x[i] = next_dy[i] = raw_t<T, V>{};
+            if (c < p.cols) {
+                next_x[i] = row_vector<NT, T, V>((const T*)p.x, r * p.x_stride, c, p.cols, end_x);
+                if (on) next_dy[i] = row_vector<NT, T, V>((const T*)p.dy, r * p.dy_stride, c, p.cols, end_dy);
+            }
         }
         next_mean = p.mean[r], next_rstd = p.rstd[r];
     };
@@ -194,8 +221,8 @@ __global__ void __launch_bounds__(block_threads(TPR)) k_ln_bwd(NormArgs p) {
         float h[NV][V], d[NV][V];
 #pragma unroll
         for (int i = 0; i < NV; i++) {
-            widen<T, V>(next_x[i], h[i]);
-            widen<T, V>(next_dy[i], d[i]);
+            widen<T, V>(ragged ? mask[i].of(next_x[i]) : next_x[i], h[i]);
+            widen<T, V>(ragged ? mask[i].of(next_dy[i]) : next_dy[i], d[i]);
         }
         const float mean = next_mean, rstd = next_rstd;
         if (r0 + (int64_t)gridDim.x * RPB < p.rows) fetch(r0 + (int64_t)gridDim.x * RPB);  // (while this row is worked on)

@@ -37,10 +37,15 @@ __device__ __forceinline__ void store_raw(T* p, raw_t<T, N> v) {
 // the first n of N (n may be anything; n <= 0: nothing is touched), the others 0
 template <bool NT, typename T, int N>
 __device__ __forceinline__ raw_t<T, N> load_raw_upto(const T* p, int64_t n) {
-    if (n >= N) return load_raw<NT, T, N>(p);
-    raw_t<T, N> v;
+    raw_t<T, N> v = {};
+    if (n >= N) {
+        v = load_raw<NT, T, N>(p);
+    } else if (n > 0) {  // (all loads at once, the ones behind the last at its place: a branch each would be a wait each)
 #pragma unroll
-    for (int j = 0; j < N; j++) v[j] = j < n ? p[j] : (T)0.0f;
+        for (int j = 0; j < N; j++) v[j] = p[j < n ? j : (int)n - 1];
+#pragma unroll
+        for (int j = 0; j < N; j++) v[j] = j < n ? v[j] : (T)0.0f;
+    }
     return v;
 }
 template <typename T, int N>
@@ -64,11 +69,10 @@ __device__ __forceinline__ void store_n(T* p, const float (&f)[N]) {
 // the same for the first n of N
 template <typename T, int N, bool NT = false>
 __device__ __forceinline__ void load_upto(const T* p, int64_t n, float fill, float (&f)[N]) {
-    if (n >= N) {
-        load_n<T, N, NT>(p, f);
-    } else {
+    widen<T, N>(load_raw_upto<NT, T, N>(p, n), f);
+    if (n < N) {
 #pragma unroll
-        for (int j = 0; j < N; j++) f[j] = j < n ? (float)p[j] : fill;
+        for (int j = 0; j < N; j++) f[j] = j < n ? f[j] : fill;
     }
 }
 template <typename T, int N, bool NT = false>
