@@ -22,7 +22,7 @@ namespace {
 using namespace ecs;
 
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f, INF = INFINITY;
-constexpr int MAX_TOP = 64;
+constexpr int MAX_TOP = 64, MAX_SPLITS = 60;  // (a split per lane, and 2 * 60 * 64 keys of LDS, where they are joined)
 constexpr int U = 4;  // vectors a thread loads before it looks at them
 
 struct LpArgs {
@@ -76,6 +76,7 @@ __device__ __forceinline__ uint32_t order_of(float x) {
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float value_of(uint32_t o) { return bitsf(o & 0x80000000u ? o & 0x7fffffffu : ~o); }
+constexpr uint32_t ORDER_LOWEST = 0x00800000u;  // order_of(-FLT_MAX)
 __device__ __forceinline__ uint64_t key_of(float x, uint32_t index) { return ((uint64_t)order_of(x) << 32) | (uint32_t)~index; }
 
 __device__ __forceinline__ uint64_t lane_u64(uint64_t x, int lane) {
@@ -83,26 +84,96 @@ __device__ __forceinline__ uint64_t lane_u64(uint64_t x, int lane) {
            (uint32_t)__builtin_amdgcn_readlane((int)x, lane);
 }
 
-// the k best keys of a wave, the i-th in lane i; 0: none
+// LDS written and read by one wave: in order, once the compiler keeps it so
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+constexpr int POOL = 128;  // keys that a wave ranks at once
+
+// The k best keys of a wave, the i-th in lane i; 0: none.  What a batch of loads holds above the k-th joins them in a pool in
+// LDS, where every key's place is the number of larger ones (keys are distinct: the index is part of them).  Of the first
+// batch only what is no less than the k-th largest of the 64 lanes' maxima can be among the k best: for any but odd data
+// little more than k keys.  That bound is found bit by bit, to 18 bits (what is below it is a bound too): a comparison each,
+// and a count in the scalar unit.  (Keys inserted one after the other cost 250 cycles each: 10000 rows of 5001 in bf16 with
+// 20 alternatives took 185 us.)
 struct TopList {
-    uint64_t mine, least;  // least: the k-th (the same in all lanes)
-    int k;
-    __device__ __forceinline__ void clear(int k_) { mine = least = 0, k = k_; }
-    __device__ __forceinline__ float least_value() const { return least ? value_of((uint32_t)(least >> 32)) : -INF; }
-    // takes the keys of all lanes; every lane of the wave has to take part
-    __device__ __forceinline__ void take(uint64_t key) {
-        uint64_t left = __ballot(key > least);
+    uint64_t mine;
+    float least;  // the k-th's value (the same in all lanes), -inf where there are fewer
+    int k, have;
+    __device__ __forceinline__ void clear(int k_) { mine = 0, least = -INF, k = k_, have = 0; }
+    __device__ __forceinline__ void set_least() {
+        const uint64_t last = lane_u64(mine, k - 1);
+        least = last ? value_of((uint32_t)(last >> 32)) : -INF;
+    }
+    // the keys of all lanes, one after the other
+    __device__ __forceinline__ void insert(uint64_t key) {
         const int lane = threadIdx.x & 63;
+        uint64_t last = lane_u64(mine, k - 1), left = __ballot(key > last);
         while (left) {
             const int from = __ffsll((unsigned long long)left) - 1;
             const uint64_t c = lane_u64(key, from);
             const int at = __popcll(__ballot(mine > c));  // (sorted: the lanes with larger keys are the first)
             const uint64_t before = __shfl_up((unsigned long long)mine, 1);
             mine = lane < at ? mine : lane == at ? c : before;
-            least = lane_u64(mine, k - 1);
+            last = lane_u64(mine, k - 1);
             left &= left - 1;
-            left &= __ballot(key > least);
+            left &= __ballot(key > last);
         }
+    }
+    // a batch: f[u][j] is column c + u * step + j; top_f: the lane's largest.  Every lane of the wave has to take part
+    template <int UU, int N>
+    __device__ __forceinline__ void absorb(const float (&f)[UU][N], float top_f, int64_t c, int64_t step, uint64_t* pool) {
+        const int lane = threadIdx.x & 63;
+        uint32_t bound;
+        if (have == 0) {
+            const uint32_t o = order_of(top_f);
+            bound = 0;
+#pragma unroll
+            for (int b = 31; b >= 14; b--)
+                if (__popcll(__ballot(o >= (bound | (1u << b)))) >= k) bound |= 1u << b;
+        } else {
+            bound = order_of(least) + 1;  // an entry equal to the k-th has a larger index than it, being of a later batch
+        }
+        const float from = fmaxf(value_of(bound < ORDER_LOWEST ? ORDER_LOWEST : bound), -FLT_MAX);
+        if (lane < have) pool[lane] = mine;
+        int n = have;
+#pragma unroll
+        for (int u = 0; u < UU; u++)
+#pragma unroll
+            for (int j = 0; j < N; j++) {
+                const float x = f[u][j];
+                const bool in = x >= from;  // (-inf is below -FLT_MAX)
+                const uint64_t who = __ballot(in);
+                if (who) {
+                    const int at = n + __popcll(who & ((1ull << lane) - 1));
+                    if (in && at < POOL) pool[at] = key_of(x, (uint32_t)(c + u * step + j));
+                    n += __popcll(who);
+                }
+            }
+        if (n > POOL) {  // (many equal ones)
+#pragma unroll
+            for (int u = 0; u < UU; u++)
+#pragma unroll
+                for (int j = 0; j < N; j++) insert(f[u][j] > -INF ? key_of(f[u][j], (uint32_t)(c + u * step + j)) : 0);
+            have = __popcll(__ballot(lane < k && mine != 0));
+        } else {
+            wave_sync();
+            const uint64_t a = lane < n ? pool[lane] : 0, b = lane + 64 < n ? pool[lane + 64] : 0;
+            int ra = 0, rb = 0;
+            for (int i = 0; i < n; i++) ra += pool[i] > a;
+            if (n > 64)
+                for (int i = 0; i < n; i++) rb += pool[i] > b;
+            wave_sync();
+            if (a && ra < k) pool[ra] = a;
+            if (b && rb < k) pool[rb] = b;
+            wave_sync();
+            have = n < k ? n : k;
+            mine = lane < have ? pool[lane] : 0;
+            wave_sync();
+        }
+        set_least();
     }
 };
 
@@ -185,16 +256,14 @@ __device__ __forceinline__ void write_top(const LpArgs& p, int64_t r, int i, con
     p.top_index[r * p.top_k + i] = at;
 }
 
-// what a row's statistics say, by its W lanes (lane t of them); the alternatives by a whole wave
+// what a row's statistics say, by one lane
 template <typename T, int MASK>
-__device__ __forceinline__ void finish_row(const LpArgs& p, int64_t r, int t, const Stat& s, const TopList* top) {
-    const float ln = log_s1(s);
-    if (t == 0) {
+__device__ __forceinline__ void finish_row(const LpArgs& p, int64_t r, bool lead, const Stat& s, float ln) {
+    if (lead) {
         const int64_t tok = p.tokens[r];
         const float l = tok >= 0 && tok < p.vocab ? logit_at<T, MASK>(row_of<T>(p, r), MASK ? mask_of<MASK>(p, r) : nullptr, tok) : 0.0f;
         write_row(p, r, s, ln, logp_of(p, tok, l, s, ln));
     }
-    if (top && t < p.top_k) write_top(p, r, t, s, ln, top->mine);
 }
 
 // TPR threads a row: 16 or 64 (each row once), or a block of 256 per row or split of a row
@@ -202,7 +271,7 @@ template <typename T, int MASK, bool TOP, int TPR, bool NT>
 __global__ void __launch_bounds__(256) k_logp_fwd(LpArgs p) {
     constexpr int V = 16 / sizeof(T), W = TPR < 64 ? TPR : 64;
     __shared__ Stat s_stat[4];
-    __shared__ uint64_t s_top[TOP && TPR == 256 ? 4 : 1][MAX_TOP];
+    __shared__ uint64_t s_pool[TOP ? 4 : 1][TOP ? POOL : 1];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, t = threadIdx.x % TPR;
     // (every thread makes every round: a group of rows past the last reads the last and writes nothing)
     const int64_t r0 = TPR == 256 ? blockIdx.x / p.splits : (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
@@ -240,57 +309,106 @@ __global__ void __launch_bounds__(256) k_logp_fwd(LpArgs p) {
                 s.s1 += e;
                 s.s2 = __builtin_fmaf(e, fmaxf(d, -200.0f), s.s2);  // (d = -inf: 0 * -inf)
             }
-        if (TOP) {
-            // an entry equal to the k-th has the larger index, unless it is of this very batch: only larger ones count
-            if (__ballot(top_f > top.least_value())) {
-#pragma unroll
-                for (int u = 0; u < U; u++)
-#pragma unroll
-                    for (int j = 0; j < V; j++) {
-                        const int64_t c = b + (u * TPR + t) * V + j;
-                        top.take(f[u][j] > -INF ? key_of(f[u][j], (uint32_t)c) : 0);
-                    }
-            }
-        }
+        if (TOP)
+            if (__ballot(top_f > top.least)) top.absorb(f, top_f, b + t * V, TPR * V, s_pool[TOP ? wave : 0]);
     }
     s = lanes_join<W>(s);
     if (TPR < 256) {
-        if (on) finish_row<T, MASK>(p, r, t, s, TOP ? &top : nullptr);
+        const float ln = log_s1(s);
+        if (on) finish_row<T, MASK>(p, r, t == 0, s, ln);
+        if (TOP && on && t < p.top_k) write_top(p, r, t, s, ln, top.mine);
         return;
     }
     if (lane == 0) s_stat[wave] = s;
-    if (TOP && lane < p.top_k) s_top[TOP && TPR == 256 ? wave : 0][lane] = top.mine;
+    if (TOP && lane < p.top_k) s_pool[TOP ? wave : 0][lane] = top.mine;
     __syncthreads();
-    if (wave) return;
+    s = s_stat[0];
 #pragma unroll
-    for (int w = 1; w < 4; w++) {
-        s = join(s, s_stat[w]);
-        if (TOP) top.take(lane < p.top_k ? s_top[TOP && TPR == 256 ? w : 0][lane] : 0);
+    for (int w = 1; w < 4; w++) s = join(s, s_stat[w]);
+    const float ln = log_s1(s);
+    char* to = p.splits > 1 ? p.work + (r * p.splits + split) * part_bytes(p.top_k) : nullptr;
+    if (p.splits == 1) finish_row<T, MASK>(p, r, threadIdx.x == 0, s, ln);
+    else if (threadIdx.x == 0) ((float*)to)[0] = s.m, ((float*)to)[1] = s.s1, ((float*)to)[2] = s.s2;
+    if (TOP) {
+        // a key's place among the four waves' lists: its place in its own and the number of larger ones in the others (the
+        // places behind the last key, each wave its share of them, take "none")
+        int have = 0, at = lane;
+        for (int w = 0; w < 4; w++) {
+            const uint64_t* o = s_pool[TOP ? w : 0];
+            have += __popcll(__ballot(lane < p.top_k && o[lane] != 0));
+            if (w != wave)
+                for (int i = 0; i < p.top_k; i++) at += o[i] > top.mine;
+        }
+        if (lane >= p.top_k || !top.mine) at = p.top_k;
+        if (wave == 0 && lane >= have && lane < p.top_k) {
+            if (to) ((uint64_t*)(to + 16))[lane] = 0;
+            else write_top(p, r, lane, s, ln, 0);
+        }
+        if (at < p.top_k) {
+            if (to) ((uint64_t*)(to + 16))[at] = top.mine;
+            else write_top(p, r, at, s, ln, top.mine);
+        }
     }
-    if (p.splits == 1) return finish_row<T, MASK>(p, r, t, s, TOP ? &top : nullptr);
-    char* to = p.work + (r * p.splits + split) * part_bytes(p.top_k);
-    if (lane == 0) ((float*)to)[0] = s.m, ((float*)to)[1] = s.s1, ((float*)to)[2] = s.s2;
-    if (TOP && lane < p.top_k) ((uint64_t*)(to + 16))[lane] = top.mine;
 }
 
-// the splits of a row as one: a wave per row
+// the splits of a row as one: a block per row
 template <typename T, int MASK>
-__global__ void __launch_bounds__(64) k_logp_join(LpArgs p) {
+__global__ void __launch_bounds__(256) k_logp_join(LpArgs p) {
+    extern __shared__ uint64_t s_keys[];  // [splits][top_k], then those that may be among the best
+    __shared__ int s_n;
     const int64_t r = blockIdx.x;
-    const int lane = threadIdx.x;
-    const char* from = p.work + r * p.splits * part_bytes(p.top_k);
+    const int lane = threadIdx.x & 63, k = p.top_k, all = p.splits * k;
+    const char* from = p.work + r * p.splits * part_bytes(k);
+    // (every wave joins the statistics for itself)
     Stat s{-FLT_MAX, 0.0f, 0.0f};
     for (int i = lane; i < p.splits; i += 64) {
-        const float* f = (const float*)(from + i * part_bytes(p.top_k));
+        const float* f = (const float*)(from + i * part_bytes(k));
         s = join(s, Stat{f[0], f[1], f[2]});
     }
     s = lanes_join<64>(s);
-    TopList top;
-    top.clear(p.top_k);
-    if (p.top_k)
-        for (int i = 0; i < p.splits; i++)
-            top.take(lane < p.top_k ? ((const uint64_t*)(from + i * part_bytes(p.top_k) + 16))[lane] : 0);
-    finish_row<T, MASK>(p, r, lane, s, p.top_k ? &top : nullptr);
+    const float ln = log_s1(s);
+    finish_row<T, MASK>(p, r, threadIdx.x == 0, s, ln);
+    if (k == 0) return;
+    for (int i = threadIdx.x; i < all; i += 256) s_keys[i] = ((const uint64_t*)(from + (i / k) * part_bytes(k) + 16))[i % k];
+    if (threadIdx.x == 0) s_n = 0;
+    __syncthreads();
+    // no key below the k-th of one split can be among the best, nor one below the k-th largest of the splits' first
+    if (threadIdx.x < 64) {
+        uint64_t least = 0, first = 0;
+        if (lane < p.splits) first = s_keys[lane * k];
+        for (int i = lane; i < p.splits; i += 64) {
+            const uint64_t o = s_keys[i * k + k - 1];
+            least = o > least ? o : least;
+        }
+        int larger = 0;
+        for (int i = 0; i < 64; i++) {
+            const uint64_t o = lane_u64(first, i);
+            larger += o > first || (o == first && i < lane);
+            const uint64_t q = lane_u64(least, i);
+            least = q > least ? q : least;
+        }
+        const uint64_t heads = lane_u64(first, __ffsll((unsigned long long)__ballot(larger == k - 1)) - 1);
+        const uint64_t bound = heads > least ? heads : least;
+        for (int b = 0; b < all; b += 64) {
+            const uint64_t o = b + lane < all ? s_keys[b + lane] : 0;
+            const bool in = o && o >= bound;
+            const uint64_t who = __ballot(in);
+            const int at = s_n + __popcll(who & ((1ull << lane) - 1));
+            wave_sync();
+            if (in) s_keys[all + at] = o;
+            if (lane == 0) s_n += __popcll(who);
+            wave_sync();
+        }
+    }
+    __syncthreads();
+    const int n = s_n;
+    const uint64_t* some = s_keys + all;
+    for (int i = threadIdx.x; i < n; i += 256) {
+        int at = 0;
+        for (int q = 0; q < n; q++) at += some[q] > some[i];
+        if (at < k) write_top(p, r, at, s, ln, some[i]);
+    }
+    for (int i = n + threadIdx.x; i < k; i += 256) write_top(p, r, i, s, ln, 0);
 }
 
 // what the gradient of a row's entries needs
@@ -402,16 +520,18 @@ __global__ void __launch_bounds__(256) k_logp_few_fwd(LpArgs p, uint32_t by_voca
     const float ln = log_s1(s);
     const int64_t tok = p.tokens[r];
     write_row(p, r, s, ln, logp_of(p, tok, tok >= 0 && tok < p.vocab ? l[tok] : 0.0f, s, ln));
-    uint64_t last = ~0ull;
-    for (int i = 0; i < p.top_k; i++) {  // the largest key below the last
-        uint64_t best = 0;
-        if (last)
-            for (int j = 0; j < p.vocab; j++) {
-                const uint64_t key = l[j] > -INF ? key_of(l[j], (uint32_t)j) : 0;
-                best = key < last && key > best ? key : best;
-            }
-        write_top(p, r, i, s, ln, best);
-        last = best;
+    float* left = s_rows + threadIdx.x * stride;
+    for (int i = 0; i < p.top_k; i++) {  // the largest of what is left, the first of equal ones
+        float best = -INF;
+        int at = -1;
+#pragma unroll 4
+        for (int j = 0; j < p.vocab; j++) {
+            const bool more = left[j] > best;
+            best = more ? left[j] : best;
+            at = more ? j : at;
+        }
+        if (at >= 0) left[at] = -INF;
+        write_top(p, r, i, s, ln, at >= 0 ? key_of(best, (uint32_t)at) : 0);
     }
 }
 
@@ -475,12 +595,14 @@ bool is_packed(const LpArgs& a) {
 uint32_t by_vocab(int vocab) { return (uint32_t)((((uint64_t)1 << 32) + vocab - 1) / vocab); }
 
 // few rows: a row is split over as many blocks as fill the GPU, at least one batch of loads each
-int splits_for(int64_t rows, int64_t vocab, int dtype) {
-    if (threads_for(vocab, dtype, true) != 256) return 1;
-    const int64_t batch = 256 * U * (dtype == EC_F32 ? 4 : 8);
-    const int64_t most = cdiv(vocab, batch), want = cdiv(1024, rows);
-    return (int)(want < most ? want : most);
+int per_split(int64_t rows, int64_t vocab, int dtype) {
+    if (threads_for(vocab, dtype, true) != 256) return INT32_MAX;
+    const int64_t batch = 256 * U * (dtype == EC_F32 ? 4 : 8), batches = cdiv(vocab, batch), want = cdiv(1024, rows);
+    const int64_t splits = want < batches ? (want < MAX_SPLITS ? want : MAX_SPLITS) : (batches < MAX_SPLITS ? batches : MAX_SPLITS);
+    const int64_t each = cdiv(batches, splits) * batch;
+    return (int)(each < INT32_MAX ? each : INT32_MAX);
 }
+int splits_for(int64_t rows, int64_t vocab, int dtype) { return (int)cdiv(vocab, per_split(rows, vocab, dtype)); }
 
 template <typename T, int MASK>
 void go_fwd(const LpArgs& a, int dtype, hipStream_t st) {
@@ -498,7 +620,7 @@ void go_fwd(const LpArgs& a, int dtype, hipStream_t st) {
         const dim3 grid((unsigned)(a.rows * a.splits));
         if (a.top_k) hipLaunchKernelGGL((k_logp_fwd<T, MASK, true, 256, true>), grid, b, 0, st, a);
         else hipLaunchKernelGGL((k_logp_fwd<T, MASK, false, 256, true>), grid, b, 0, st, a);
-        if (a.splits > 1) hipLaunchKernelGGL((k_logp_join<T, MASK>), dim3((unsigned)a.rows), dim3(64), 0, st, a);
+        if (a.splits > 1) hipLaunchKernelGGL((k_logp_join<T, MASK>), dim3((unsigned)a.rows), b, 2 * 8 * a.splits * a.top_k, st, a);
     }
 }
 
@@ -554,8 +676,7 @@ extern "C" int ec_token_logprobs_fwd(const void* logits, int64_t inner, int64_t 
     a.top_k = top_k, a.logp = logp, a.entropy = entropy, a.lse = lse, a.top_logp = top_logp, a.top_index = top_index;
     a.work = (char*)work;
     a.splits = splits_for(rows, vocab, dtype);
-    const int64_t batch = 256 * U * (dtype == EC_F32 ? 4 : 8);
-    a.per_split = (int)(cdiv(cdiv(vocab, a.splits), batch) * batch < INT32_MAX ? cdiv(cdiv(vocab, a.splits), batch) * batch : INT32_MAX);
+    a.per_split = per_split(rows, vocab, dtype);
     if (rows * a.splits > INT32_MAX) return ec::fail(EC_EINVAL, "ec_token_logprobs_fwd: %lld rows", (long long)rows);
     const hipStream_t st = (hipStream_t)stream;
     EC_LP_TYPES(go_fwd)
