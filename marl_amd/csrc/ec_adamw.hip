@@ -125,32 +125,16 @@ struct Bytes {
 };
 template <int N, bool NT>
 __device__ __forceinline__ Bytes<N> load8(const uint8_t* q, int64_t n) {
+    const auto v = load_raw_upto<NT, uint8_t, N>(q, n);
     Bytes<N> b;
-    if (n >= N) {
-        const auto v = load_raw<NT, uint8_t, N>(q);
-        __builtin_memcpy(&b, &v, N);
-        return b;
-    }
-#pragma unroll
-    for (int k = 0; k < N / 4; k++) {
-        b.w[k] = 0;
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (4 * k + j < n) b.w[k] |= (uint32_t)q[4 * k + j] << (8 * j);
-    }
+    __builtin_memcpy(&b, &v, N);
     return b;
 }
 template <int N, bool NT>
 __device__ __forceinline__ void store8(uint8_t* q, int64_t n, const Bytes<N>& b) {
-    if (n >= N) {
-        raw_t<uint8_t, N> v;
-        __builtin_memcpy(&v, &b, N);
-        store_raw<NT, uint8_t, N>(q, v);
-        return;
-    }
-#pragma unroll
-    for (int j = 0; j < N; j++)
-        if (j < n) q[j] = (uint8_t)(b.w[j / 4] >> (8 * (j % 4)));
+    raw_t<uint8_t, N> v;
+    __builtin_memcpy(&v, &b, N);
+    store_raw_upto<NT, uint8_t, N>(q, n, v);
 }
 template <int N>
 __device__ __forceinline__ void unpack8(const Bytes<N>& b, float scale, float (&f)[N]) {

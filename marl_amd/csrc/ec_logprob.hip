@@ -23,7 +23,7 @@ using namespace ecs;
 
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f, INF = INFINITY;
 constexpr int MAX_TOP = 64, MAX_SPLITS = 60;  // (a split per lane, and 2 * 60 * 64 keys of LDS, where they are joined)
-constexpr int U = 4;  // vectors a thread loads before it looks at them
+constexpr int MOST_U = 4;  // vectors a thread loads before it looks at them, at most
 
 struct LpArgs {
     const void *logits, *avail;
@@ -266,8 +266,40 @@ __device__ __forceinline__ void finish_row(const LpArgs& p, int64_t r, bool lead
     }
 }
 
+// U vectors a thread from column b on into the row's statistics and alternatives (the same rounds for every thread: the lists
+// need whole waves).  FULL: all of them below c1
+template <typename T, int MASK, bool TOP, int TPR, int U, bool NT, bool FULL>
+__device__ __forceinline__ void logp_batch(const T* l, const char* av, int64_t b, int t, int64_t c1, Stat& s, TopList& top,
+                                           uint64_t* pool) {
+    constexpr int V = 16 / sizeof(T);
+    float f[U][V];
+    float top_f = -INF;
+    load_logits<T, MASK, NT, FULL>(l, av, b + t * V, TPR * V, c1, f);
+#pragma unroll
+    for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int j = 0; j < V; j++) top_f = fmaxf(top_f, f[u][j]);
+    const float m = fmaxf(s.m, top_f);
+    const float d0 = fmaxf((s.m - m) * LOG2E, -200.0f), g = __builtin_amdgcn_exp2f(d0);
+    s.s2 = (s.s2 + s.s1 * d0) * g;
+    s.s1 *= g;
+    s.m = m;
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        if (!FULL && TPR == 256 && b + u * TPR * V >= c1) break;  // (the same for all: nothing but -inf from here on)
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            const float d = (f[u][j] - m) * LOG2E, e = __builtin_amdgcn_exp2f(d);
+            s.s1 += e;
+            s.s2 = __builtin_fmaf(e, fmaxf(d, -200.0f), s.s2);  // (d = -inf: 0 * -inf)
+        }
+    }
+    if (TOP)
+        if (__ballot(top_f > top.least)) top.absorb(f, top_f, b + t * V, TPR * V, pool);
+}
+
 // TPR threads a row: 16 or 64 (each row once), or a block of 256 per row or split of a row
-template <typename T, int MASK, bool TOP, int TPR, bool NT>
+template <typename T, int MASK, bool TOP, int TPR, int U, bool NT>
 __global__ void __launch_bounds__(256) k_logp_fwd(LpArgs p) {
     constexpr int V = 16 / sizeof(T), W = TPR < 64 ? TPR : 64;
     __shared__ Stat s_stat[4];
@@ -285,33 +317,9 @@ __global__ void __launch_bounds__(256) k_logp_fwd(LpArgs p) {
     Stat s{-FLT_MAX, 0.0f, 0.0f};
     TopList top;
     top.clear(p.top_k);
-    for (int64_t b = c0; b < c1; b += TPR * V * U) {  // (the same rounds for every thread: the lists need whole waves)
-        float f[U][V];
-        float top_f = -INF;
-        if (b + TPR * V * U <= c1) load_logits<T, MASK, NT, true>(l, av, b + t * V, TPR * V, c1, f);
-        else load_logits<T, MASK, NT, false>(l, av, b + t * V, TPR * V, c1, f);
-#pragma unroll
-        for (int u = 0; u < U; u++)
-#pragma unroll
-            for (int j = 0; j < V; j++) top_f = fmaxf(top_f, f[u][j]);
-        const float m = fmaxf(s.m, top_f);
-        {
-            const float d = fmaxf((s.m - m) * LOG2E, -200.0f), g = __builtin_amdgcn_exp2f(d);
-            s.s2 = (s.s2 + s.s1 * d) * g;
-            s.s1 *= g;
-            s.m = m;
-        }
-#pragma unroll
-        for (int u = 0; u < U; u++)
-#pragma unroll
-            for (int j = 0; j < V; j++) {
-                const float d = (f[u][j] - m) * LOG2E, e = __builtin_amdgcn_exp2f(d);
-                s.s1 += e;
-                s.s2 = __builtin_fmaf(e, fmaxf(d, -200.0f), s.s2);  // (d = -inf: 0 * -inf)
-            }
-        if (TOP)
-            if (__ballot(top_f > top.least)) top.absorb(f, top_f, b + t * V, TPR * V, s_pool[TOP ? wave : 0]);
-    }
+    int64_t b = c0;
+    for (; b + TPR * V * U <= c1; b += TPR * V * U) logp_batch<T, MASK, TOP, TPR, U, NT, true>(l, av, b, t, c1, s, top, s_pool[TOP ? wave : 0]);
+    if (b < c1) logp_batch<T, MASK, TOP, TPR, U, NT, false>(l, av, b, t, c1, s, top, s_pool[TOP ? wave : 0]);
     s = lanes_join<W>(s);
     if (TPR < 256) {
         const float ln = log_s1(s);
@@ -359,54 +367,49 @@ __global__ void __launch_bounds__(256) k_logp_join(LpArgs p) {
     const int64_t r = blockIdx.x;
     const int lane = threadIdx.x & 63, k = p.top_k, all = p.splits * k;
     const char* from = p.work + r * p.splits * part_bytes(k);
-    // (every wave joins the statistics for itself)
+    // (every wave joins the statistics for itself; what is loaded is loaded first: this kernel is a chain of waits)
     Stat s{-FLT_MAX, 0.0f, 0.0f};
-    for (int i = lane; i < p.splits; i += 64) {
-        const float* f = (const float*)(from + i * part_bytes(k));
-        s = join(s, Stat{f[0], f[1], f[2]});
+    if (lane < p.splits) {
+        const float* f = (const float*)(from + lane * part_bytes(k));
+        s = Stat{f[0], f[1], f[2]};
     }
+    uint32_t first = 0, last = 0;  // order of each split's largest and k-th
+    if (threadIdx.x < 64 && k && lane < p.splits) {
+        const uint64_t* q = (const uint64_t*)(from + lane * part_bytes(k) + 16);
+        first = (uint32_t)(q[0] >> 32), last = (uint32_t)(q[k - 1] >> 32);
+    }
+    for (int i = threadIdx.x; i < all; i += 256) s_keys[i] = ((const uint64_t*)(from + (i / k) * part_bytes(k) + 16))[i % k];
     s = lanes_join<64>(s);
     const float ln = log_s1(s);
-    finish_row<T, MASK>(p, r, threadIdx.x == 0, s, ln);
+    finish_row<T, MASK>(p, r, threadIdx.x == 255, s, ln);
     if (k == 0) return;
-    for (int i = threadIdx.x; i < all; i += 256) s_keys[i] = ((const uint64_t*)(from + (i / k) * part_bytes(k) + 16))[i % k];
-    if (threadIdx.x == 0) s_n = 0;
     __syncthreads();
-    // no key below the k-th of one split can be among the best, nor one below the k-th largest of the splits' first
+    // nothing below the k-th of one split can be among the best, nor below the k-th largest of the splits' largest (TopList)
     if (threadIdx.x < 64) {
-        uint64_t least = 0, first = 0;
-        if (lane < p.splits) first = s_keys[lane * k];
-        for (int i = lane; i < p.splits; i += 64) {
-            const uint64_t o = s_keys[i * k + k - 1];
-            least = o > least ? o : least;
-        }
-        int larger = 0;
-        for (int i = 0; i < 64; i++) {
-            const uint64_t o = lane_u64(first, i);
-            larger += o > first || (o == first && i < lane);
-            const uint64_t q = lane_u64(least, i);
-            least = q > least ? q : least;
-        }
-        const uint64_t heads = lane_u64(first, __ffsll((unsigned long long)__ballot(larger == k - 1)) - 1);
-        const uint64_t bound = heads > least ? heads : least;
+        uint32_t heads = 0;
+#pragma unroll
+        for (int b = 31; b >= 14; b--)
+            if (__popcll(__ballot(first >= (heads | (1u << b)))) >= k) heads |= 1u << b;
+        last = lanes_umax<64>(last);
+        const uint64_t bound = (uint64_t)(heads > last ? heads : last) << 32;
+        int n = 0;
         for (int b = 0; b < all; b += 64) {
             const uint64_t o = b + lane < all ? s_keys[b + lane] : 0;
             const bool in = o && o >= bound;
             const uint64_t who = __ballot(in);
-            const int at = s_n + __popcll(who & ((1ull << lane) - 1));
-            wave_sync();
-            if (in) s_keys[all + at] = o;
-            if (lane == 0) s_n += __popcll(who);
-            wave_sync();
+            if (in) s_keys[all + n + __popcll(who & ((1ull << lane) - 1))] = o;
+            n += __popcll(who);
         }
+        if (lane == 0) s_n = n;
     }
     __syncthreads();
     const int n = s_n;
     const uint64_t* some = s_keys + all;
     for (int i = threadIdx.x; i < n; i += 256) {
+        const uint64_t mine = some[i];
         int at = 0;
-        for (int q = 0; q < n; q++) at += some[q] > some[i];
-        if (at < k) write_top(p, r, at, s, ln, some[i]);
+        for (int q = 0; q < n; q++) at += some[q] > mine;
+        if (at < k) write_top(p, r, at, s, ln, mine);
     }
     for (int i = n + threadIdx.x; i < k; i += 256) write_top(p, r, i, s, ln, 0);
 }
@@ -436,8 +439,23 @@ __device__ __forceinline__ float entry_grad(const RowGrad& w, float l, int64_t c
     return w.none || l == -INF ? 0.0f : d;
 }
 
+template <typename T, int MASK, int TPR, int U, bool NT, bool FULL>
+__device__ __forceinline__ void grad_batch(const RowGrad& w, const T* l, const char* av, T* out, int64_t b, int t, int64_t c1) {
+    constexpr int V = 16 / sizeof(T);
+    float f[U][V];
+    load_logits<T, MASK, NT, FULL>(l, av, b + t * V, TPR * V, c1, f);
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int64_t c = b + (u * TPR + t) * V;
+        if (!FULL && TPR == 256 && b + u * TPR * V >= c1) break;  // (the same for all)
+#pragma unroll
+        for (int j = 0; j < V; j++) f[u][j] = entry_grad(w, f[u][j], c + j);
+        store_upto<T, V, NT>(out + c, FULL ? V : c1 - c, f[u]);
+    }
+}
+
 // TPR threads a row: 16 or 64 for a whole row, or a block of 256 per TPR * V * U columns of a row
-template <typename T, int MASK, int TPR, bool NT>
+template <typename T, int MASK, int TPR, int U, bool NT>
 __global__ void __launch_bounds__(256) k_logp_bwd(LpArgs p) {
     constexpr int V = 16 / sizeof(T);
     const int64_t r = TPR == 256 ? blockIdx.x / p.splits : (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
@@ -449,25 +467,15 @@ __global__ void __launch_bounds__(256) k_logp_bwd(LpArgs p) {
     T* out = (T*)p.dlogits + r * p.vocab;
     const RowGrad w = row_grad(p, r);
     const int t = threadIdx.x % TPR;
-    for (int64_t b = c0; b < c1; b += TPR * V * U) {
-        float f[U][V];
-        const bool full = b + TPR * V * U <= c1;
-        if (full) load_logits<T, MASK, NT, true>(l, av, b + t * V, TPR * V, c1, f);
-        else load_logits<T, MASK, NT, false>(l, av, b + t * V, TPR * V, c1, f);
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int64_t c = b + (u * TPR + t) * V;
-#pragma unroll
-            for (int j = 0; j < V; j++) f[u][j] = entry_grad(w, f[u][j], c + j);
-            store_upto<T, V, NT>(out + c, full ? V : c1 - c, f[u]);
-        }
-    }
+    int64_t b = c0;
+    for (; b + TPR * V * U <= c1; b += TPR * V * U) grad_batch<T, MASK, TPR, U, NT, true>(w, l, av, out, b, t, c1);
+    if (b < c1) grad_batch<T, MASK, TPR, U, NT, false>(w, l, av, out, b, t, c1);
 }
 
 // ---- few entries a row (the env's action sets): a lane per row ----
 // 256 rows are staged through LDS as fp32, excluded entries as -inf, at an odd stride (lanes that walk down their rows hit
 // different banks); packed rows come in and gradients leave 16 bytes a lane whatever the row's width.
-constexpr int FEW = 63;  // (64 KB of LDS a block)
+constexpr int FEW = 62;  // (64 KB of LDS a block)
 
 __device__ __forceinline__ int row_in(int i, int vocab, uint32_t by_vocab) {  // i / vocab
     return vocab == 1 ? i : (int)__umulhi((uint32_t)i, by_vocab);
@@ -484,6 +492,11 @@ __device__ __forceinline__ void stage_rows(const LpArgs& p, int64_t r0, int n, i
             float f1[1][V], (&f)[V] = f1[0];
             if (i + V <= all) load_logits<T, MASK, false, true>(l, av, i, 0, all, f1);
             else load_logits<T, MASK, false, false>(l, av, i, 0, all, f1);
+            if (stride == p.vocab) {  // (an odd width is its own stride: the tile lies in LDS as in memory, which has room for the last)
+#pragma unroll
+                for (int q = 0; q < V; q += 4) *(float4*)(s + i + q) = make_float4(f[q], f[q + 1], f[q + 2], f[q + 3]);
+                continue;
+            }
             int row = row_in(i, p.vocab, by_vocab), col = i - row * p.vocab;
 #pragma unroll
             for (int j = 0; j < V; j++) {
@@ -554,11 +567,19 @@ __global__ void __launch_bounds__(256) k_logp_few_bwd(LpArgs p, uint32_t by_voca
     const int all = n * p.vocab;
     for (int i = threadIdx.x * V; i < all; i += 256 * V) {
         float f[V];
-        int row = row_in(i, p.vocab, by_vocab), col = i - row * p.vocab;
+        if (stride == p.vocab) {
 #pragma unroll
-        for (int j = 0; j < V; j++) {
-            f[j] = i + j < all ? s_rows[row * stride + col] : 0.0f;
-            if (++col == p.vocab) col = 0, row++;
+            for (int q = 0; q < V; q += 4) {
+                const float4 v = *(const float4*)(s_rows + i + q);
+                f[q] = v.x, f[q + 1] = v.y, f[q + 2] = v.z, f[q + 3] = v.w;
+            }
+        } else {
+            int row = row_in(i, p.vocab, by_vocab), col = i - row * p.vocab;
+#pragma unroll
+            for (int j = 0; j < V; j++) {
+                f[j] = i + j < all ? s_rows[row * stride + col] : 0.0f;
+                if (++col == p.vocab) col = 0, row++;
+            }
         }
         store_upto(out + i, all - i, f);
     }
@@ -586,6 +607,11 @@ int threads_for(int64_t vocab, int dtype, bool top) {
     const int64_t vecs = cdiv(vocab, dtype == EC_F32 ? 4 : 8);
     return vecs <= 64 && !top ? 16 : vecs <= 256 ? 64 : 256;
 }
+// vectors a thread then takes at once: as few as hold the row (what is loaded past it is computed with all the same)
+int vectors_for(int64_t vocab, int dtype, int tpr) {
+    const int64_t each = cdiv(cdiv(vocab, dtype == EC_F32 ? 4 : 8), tpr);
+    return each <= 1 ? 1 : each <= 2 ? 2 : MOST_U;
+}
 // rows that lie one behind the other, mask and logits
 bool is_packed(const LpArgs& a) {
     const bool l = a.s_outer == a.inner * a.vocab && (a.inner == 1 || a.s_inner == a.vocab);
@@ -597,46 +623,60 @@ uint32_t by_vocab(int vocab) { return (uint32_t)((((uint64_t)1 << 32) + vocab - 
 // few rows: a row is split over as many blocks as fill the GPU, at least one batch of loads each
 int per_split(int64_t rows, int64_t vocab, int dtype) {
     if (threads_for(vocab, dtype, true) != 256) return INT32_MAX;
-    const int64_t batch = 256 * U * (dtype == EC_F32 ? 4 : 8), batches = cdiv(vocab, batch), want = cdiv(1024, rows);
+    const int64_t batch = 256 * MOST_U * (dtype == EC_F32 ? 4 : 8), batches = cdiv(vocab, batch), want = cdiv(1024, rows);
     const int64_t splits = want < batches ? (want < MAX_SPLITS ? want : MAX_SPLITS) : (batches < MAX_SPLITS ? batches : MAX_SPLITS);
     const int64_t each = cdiv(batches, splits) * batch;
     return (int)(each < INT32_MAX ? each : INT32_MAX);
 }
 int splits_for(int64_t rows, int64_t vocab, int dtype) { return (int)cdiv(vocab, per_split(rows, vocab, dtype)); }
 
+int few_lds(int vocab) { return (256 * (vocab | 1) + 8) * 4; }  // (the last vector of a tile may be a partial one)
+
 template <typename T, int MASK>
 void go_fwd(const LpArgs& a, int dtype, hipStream_t st) {
-    const int tpr = threads_for(a.vocab, dtype, a.top_k > 0);
+    const int tpr = threads_for(a.vocab, dtype, a.top_k > 0), u = tpr ? vectors_for(a.vocab, dtype, tpr) : 0;
     const auto blocks = [&](int rows) { return dim3((unsigned)cdiv(a.rows, rows)); };
     const dim3 b(256);
     if (tpr == 0) {
-        hipLaunchKernelGGL((k_logp_few_fwd<T, MASK>), blocks(256), b, 256 * (a.vocab | 1) * 4, st, a, by_vocab(a.vocab), is_packed(a));
+        hipLaunchKernelGGL((k_logp_few_fwd<T, MASK>), blocks(256), b, few_lds(a.vocab), st, a, by_vocab(a.vocab), is_packed(a));
     } else if (tpr == 16) {
-        hipLaunchKernelGGL((k_logp_fwd<T, MASK, false, 16, false>), blocks(16), b, 0, st, a);
+        if (u == 1) hipLaunchKernelGGL((k_logp_fwd<T, MASK, false, 16, 1, false>), blocks(16), b, 0, st, a);
+        else if (u == 2) hipLaunchKernelGGL((k_logp_fwd<T, MASK, false, 16, 2, false>), blocks(16), b, 0, st, a);
+        else hipLaunchKernelGGL((k_logp_fwd<T, MASK, false, 16, 4, false>), blocks(16), b, 0, st, a);
+    } else if (tpr == 64 && a.top_k) {
+        if (u == 1) hipLaunchKernelGGL((k_logp_fwd<T, MASK, true, 64, 1, false>), blocks(4), b, 0, st, a);
+        else if (u == 2) hipLaunchKernelGGL((k_logp_fwd<T, MASK, true, 64, 2, false>), blocks(4), b, 0, st, a);
+        else hipLaunchKernelGGL((k_logp_fwd<T, MASK, true, 64, 4, false>), blocks(4), b, 0, st, a);
     } else if (tpr == 64) {
-        if (a.top_k) hipLaunchKernelGGL((k_logp_fwd<T, MASK, true, 64, false>), blocks(4), b, 0, st, a);
-        else hipLaunchKernelGGL((k_logp_fwd<T, MASK, false, 64, false>), blocks(4), b, 0, st, a);
+        if (u == 2) hipLaunchKernelGGL((k_logp_fwd<T, MASK, false, 64, 2, false>), blocks(4), b, 0, st, a);
+        else hipLaunchKernelGGL((k_logp_fwd<T, MASK, false, 64, 4, false>), blocks(4), b, 0, st, a);
     } else {
         const dim3 grid((unsigned)(a.rows * a.splits));
-        if (a.top_k) hipLaunchKernelGGL((k_logp_fwd<T, MASK, true, 256, true>), grid, b, 0, st, a);
-        else hipLaunchKernelGGL((k_logp_fwd<T, MASK, false, 256, true>), grid, b, 0, st, a);
+        if (a.top_k) hipLaunchKernelGGL((k_logp_fwd<T, MASK, true, 256, MOST_U, true>), grid, b, 0, st, a);
+        else hipLaunchKernelGGL((k_logp_fwd<T, MASK, false, 256, MOST_U, true>), grid, b, 0, st, a);
         if (a.splits > 1) hipLaunchKernelGGL((k_logp_join<T, MASK>), dim3((unsigned)a.rows), b, 2 * 8 * a.splits * a.top_k, st, a);
     }
 }
 
 template <typename T, int MASK>
 void go_bwd(const LpArgs& a, int dtype, hipStream_t st) {
-    const int tpr = threads_for(a.vocab, dtype, false);
+    const int tpr = threads_for(a.vocab, dtype, false), u = tpr ? vectors_for(a.vocab, dtype, tpr) : 0;
     const auto blocks = [&](int rows) { return dim3((unsigned)cdiv(a.rows, rows)); };
     const dim3 b(256);
     if (tpr == 0)
-        hipLaunchKernelGGL((k_logp_few_bwd<T, MASK>), blocks(256), b, 256 * (a.vocab | 1) * 4, st, a, by_vocab(a.vocab), is_packed(a));
+        hipLaunchKernelGGL((k_logp_few_bwd<T, MASK>), blocks(256), b, few_lds(a.vocab), st, a, by_vocab(a.vocab), is_packed(a));
+    else if (tpr == 16 && u == 1)
+        hipLaunchKernelGGL((k_logp_bwd<T, MASK, 16, 1, false>), blocks(16), b, 0, st, a);
+    else if (tpr == 16 && u == 2)
+        hipLaunchKernelGGL((k_logp_bwd<T, MASK, 16, 2, false>), blocks(16), b, 0, st, a);
     else if (tpr == 16)
-        hipLaunchKernelGGL((k_logp_bwd<T, MASK, 16, false>), blocks(16), b, 0, st, a);
+        hipLaunchKernelGGL((k_logp_bwd<T, MASK, 16, 4, false>), blocks(16), b, 0, st, a);
+    else if (tpr == 64 && u == 2)
+        hipLaunchKernelGGL((k_logp_bwd<T, MASK, 64, 2, false>), blocks(4), b, 0, st, a);
     else if (tpr == 64)
-        hipLaunchKernelGGL((k_logp_bwd<T, MASK, 64, false>), blocks(4), b, 0, st, a);
+        hipLaunchKernelGGL((k_logp_bwd<T, MASK, 64, 4, false>), blocks(4), b, 0, st, a);
     else
-        hipLaunchKernelGGL((k_logp_bwd<T, MASK, 256, true>), dim3((unsigned)(a.rows * a.splits)), b, 0, st, a);
+        hipLaunchKernelGGL((k_logp_bwd<T, MASK, 256, MOST_U, true>), dim3((unsigned)(a.rows * a.splits)), b, 0, st, a);
 }
 
 #define EC_LP_GO(GO, T)                                  \
@@ -695,7 +735,7 @@ extern "C" int ec_token_logprobs_bwd(const void* logits, int64_t inner, int64_t 
     if (rows == 0) return EC_OK;
     if (!lse || !entropy || !dlogits) return ec::fail(EC_EINVAL, "ec_token_logprobs_bwd: null argument");
     a.lse = const_cast<float*>(lse), a.entropy_in = entropy, a.dlogp = dlogp, a.dentropy = dentropy, a.dlogits = dlogits;
-    a.per_split = 256 * U * (dtype == EC_F32 ? 4 : 8);
+    a.per_split = 256 * MOST_U * (dtype == EC_F32 ? 4 : 8);
     a.splits = threads_for(vocab, dtype, false) == 256 ? (int)cdiv(vocab, a.per_split) : 1;
     if (rows * a.splits > INT32_MAX) return ec::fail(EC_EINVAL, "ec_token_logprobs_bwd: %lld rows", (long long)rows);
     const hipStream_t st = (hipStream_t)stream;

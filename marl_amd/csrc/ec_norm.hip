@@ -77,6 +77,15 @@ struct Mask {
         return v;
     }
 };
+// v, of which the compiler from here on knows nothing: what was made from it before is made again, not kept
+template <typename T, int V>
+__device__ __forceinline__ raw_t<T, V> afresh(raw_t<T, V> v) {
+    uint32_t u[4];
+    __builtin_memcpy(u, &v, 16);
+    asm volatile("" : "+v"(u[0]), "+v"(u[1]), "+v"(u[2]), "+v"(u[3]));
+    __builtin_memcpy(&v, u, 16);
+    return v;
+}
 // the vector of column c < cols of a row at `off`; end: the tensor's last element plus one
 template <bool NT, typename T, int V>
 __device__ __forceinline__ raw_t<T, V> row_vector(const T* base, int64_t off, int c, int cols, int64_t end) {
@@ -181,7 +190,7 @@ template <typename T, int TPR, int NV, bool NT>
 __global__ void __launch_bounds__(block_threads(TPR)) k_ln_bwd(NormArgs p) {
     constexpr int V = 16 / sizeof(T), RPB = block_threads(TPR) / TPR;
     __shared__ float2 s_red[2][16];
-    __shared__ float s_part[RPB > 1 ? 2 : 1][RPB > 1 ? V : 1][RPB > 1 ? 256 : 1];
+    __shared__ float s_part[2][RPB > 1 ? V : 1][RPB > 1 ? 256 : 1];
     const int t = threadIdx.x % TPR, g = threadIdx.x / TPR;
     float w[NV][V], dw[NV][V], db[NV][V];
 #pragma unroll
@@ -214,31 +223,36 @@ __global__ void __launch_bounds__(block_threads(TPR)) k_ln_bwd(NormArgs p) {
         }
         next_mean = p.mean[r], next_rstd = p.rstd[r];
     };
-    fetch((int64_t)blockIdx.x * RPB);
+    // (a block of 1024 threads has 128 registers a thread: no room for the next row with two vectors or more)
+    constexpr bool AHEAD = TPR < 1024 || NV == 1;
+    if (AHEAD) fetch((int64_t)blockIdx.x * RPB);
     for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < p.rows; r0 += (int64_t)gridDim.x * RPB, slot ^= 1) {
         const bool on = r0 + g < p.rows;
         const int64_t r = r0 + g;
-        float h[NV][V], d[NV][V];
+        // (without room for the next row the row stays as it was read, and xhat is made from it twice: half the registers)
+        raw_t<T, V> x[NV], dy[NV];
+        if (!AHEAD) fetch(r0);
 #pragma unroll
         for (int i = 0; i < NV; i++) {
-            widen<T, V>(ragged ? mask[i].of(next_x[i]) : next_x[i], h[i]);
-            widen<T, V>(ragged ? mask[i].of(next_dy[i]) : next_dy[i], d[i]);
+            x[i] = ragged ? mask[i].of(next_x[i]) : next_x[i];
+            dy[i] = ragged ? mask[i].of(next_dy[i]) : next_dy[i];
         }
         const float mean = next_mean, rstd = next_rstd;
-        if (r0 + (int64_t)gridDim.x * RPB < p.rows) fetch(r0 + (int64_t)gridDim.x * RPB);  // (while this row is worked on)
+        if (AHEAD && r0 + (int64_t)gridDim.x * RPB < p.rows) fetch(r0 + (int64_t)gridDim.x * RPB);  // (while this row is worked on)
         float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NV; i++)
+        for (int i = 0; i < NV; i++) {
 #pragma unroll
             for (int j = 0; j < V; j++) {
-                h[i][j] = (h[i][j] - mean) * rstd;
+                const float h = ((float)x[i][j] - mean) * rstd, d = (float)dy[i][j], a = d * w[i][j];
                 // (columns behind the last: d is 0 there, and w 0 or 1)
-                dw[i][j] = __builtin_fmaf(d[i][j], h[i][j], dw[i][j]);
-                db[i][j] += d[i][j];
-                d[i][j] *= w[i][j];
-                s1 += d[i][j];
-                s2 = __builtin_fmaf(d[i][j], h[i][j], s2);
+                dw[i][j] = __builtin_fmaf(d, h, dw[i][j]);
+                db[i][j] += d;
+                s1 += a;
+                s2 = __builtin_fmaf(a, h, s2);
             }
+            if (!AHEAD) __builtin_amdgcn_sched_barrier(0);  // (vectors one after the other: interleaved they need more registers)
+        }
         row_sum2<TPR>(s1, s2, s_red, slot);
         s1 *= inv_c;
         s2 *= inv_c;
@@ -247,10 +261,15 @@ __global__ void __launch_bounds__(block_threads(TPR)) k_ln_bwd(NormArgs p) {
 #pragma unroll
             for (int i = 0; i < NV; i++) {
                 const int c = (i * TPR + t) * V;
+                const raw_t<T, V> x2 = AHEAD ? x[i] : afresh<T, V>(x[i]), dy2 = AHEAD ? dy[i] : afresh<T, V>(dy[i]);
                 float o[V];
 #pragma unroll
-                for (int j = 0; j < V; j++) o[j] = rstd * (d[i][j] - s1 - h[i][j] * s2);
+                for (int j = 0; j < V; j++) {
+                    const float h = ((float)x2[j] - mean) * rstd;
+                    o[j] = rstd * (__builtin_fmaf((float)dy2[j], w[i][j], -s1) - h * s2);
+                }
                 store_upto<T, V, NT>(dx + c, p.cols - c, o);
+                if (!AHEAD) __builtin_amdgcn_sched_barrier(0);
             }
         }
     }
@@ -259,24 +278,30 @@ __global__ void __launch_bounds__(block_threads(TPR)) k_ln_bwd(NormArgs p) {
 #pragma unroll
     for (int i = 0; i < NV; i++) {
         const int c = (i * TPR + t) * V;
-        if (RPB > 1) {  // the block's row groups, in a fixed order
+        if (RPB > 1) {  // the row groups of a wave, then the waves, in a fixed order
+            const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
             __syncthreads();
 #pragma unroll
             for (int j = 0; j < V; j++) {
+#pragma unroll
+                for (int o = TPR; o < 64; o *= 2) {
+                    dw[i][j] += __shfl_xor(dw[i][j], o);
+                    db[i][j] += __shfl_xor(db[i][j], o);
+                }
                 s_part[0][j][threadIdx.x] = dw[i][j];
-                s_part[1 % (RPB > 1 ? 2 : 1)][j][threadIdx.x] = db[i][j];
+                s_part[1][j][threadIdx.x] = db[i][j];
             }
             __syncthreads();
-            if (g == 0)
+            if (wave == 0 && lane < TPR)
 #pragma unroll
-                for (int k = 1; k < RPB; k++)
+                for (int k = 1; k < 4; k++)
 #pragma unroll
                     for (int j = 0; j < V; j++) {
-                        dw[i][j] += s_part[0][j][k * TPR + t];
-                        db[i][j] += s_part[1 % (RPB > 1 ? 2 : 1)][j][k * TPR + t];
+                        dw[i][j] += s_part[0][j][k * 64 + t];
+                        db[i][j] += s_part[1][j][k * 64 + t];
                     }
         }
-        if (g == 0) {
+        if ((int)threadIdx.x < TPR) {
             store_upto(part + c, (int64_t)p.cols - c, dw[i]);
             store_upto(part + p.cols + c, (int64_t)p.cols - c, db[i]);
         }
@@ -412,7 +437,7 @@ struct Shape {
 };
 Shape shape_for(int64_t cols, int dtype) {
     const int64_t vecs = cdiv(cols, dtype == EC_F32 ? 4 : 8);
-    for (int tpr : {8, 16, 32, 64, 128, 256, 512, 1024})
+    for (int tpr : {2, 4, 8, 16, 32, 64, 128, 256, 512, 1024})
         if (vecs <= tpr) return tpr == 128 ? Shape{64, 2, 4} : Shape{tpr, 1, block_threads(tpr) / tpr};
     if (vecs <= 2048) return {1024, 2, 1};
     if (vecs <= 4096 && dtype == EC_F32) return {1024, 4, 1};
@@ -445,7 +470,7 @@ template <typename T, bool BWD>
 void dispatch(const NormArgs& a, const Shape& s, unsigned blocks, hipStream_t st) {
 #define EC_LN(TPR, NV) \
     if (s.tpr == TPR && s.nv == NV) return go<T, BWD, TPR, NV>(a, blocks, st);
-    EC_LN(8, 1) EC_LN(16, 1) EC_LN(32, 1) EC_LN(64, 1) EC_LN(64, 2) EC_LN(256, 1) EC_LN(512, 1) EC_LN(1024, 1) EC_LN(1024, 2)
+    EC_LN(2, 1) EC_LN(4, 1) EC_LN(8, 1) EC_LN(16, 1) EC_LN(32, 1) EC_LN(64, 1) EC_LN(64, 2) EC_LN(256, 1) EC_LN(512, 1) EC_LN(1024, 1) EC_LN(1024, 2)
     if constexpr (sizeof(T) == 4) { EC_LN(1024, 4) }
 #undef EC_LN
 }

@@ -34,19 +34,56 @@ __device__ __forceinline__ void store_raw(T* p, raw_t<T, N> v) {
     if (NT) __builtin_nontemporal_store(v, reinterpret_cast<any*>(p));
     else *reinterpret_cast<any*>(p) = v;
 }
+// The first `bytes` < 16 of a vector, the others 0: in pieces of 8, 4, 2 and 1 bytes, which are all under way together (an
+// element at a time, each in a branch of its own, would be a wait each, and an address each)
+typedef uint64_t u64_any __attribute__((aligned(1)));
+typedef uint32_t u32_any __attribute__((aligned(1)));
+typedef uint16_t u16_any __attribute__((aligned(1)));
+__device__ __forceinline__ void load_bytes(const char* p, int bytes, uint64_t (&w)[2]) {
+    uint64_t r8 = 0;
+    uint32_t r4 = 0, r2 = 0, r1 = 0;
+    if (bytes & 8) r8 = *(const u64_any*)p;
+    if (bytes & 4) r4 = *(const u32_any*)(p + (bytes & 8));
+    if (bytes & 2) r2 = *(const u16_any*)(p + (bytes & 12));
+    if (bytes & 1) r1 = *(const uint8_t*)(p + (bytes & 14));
+    const uint64_t low = (uint64_t)(r2 | ((bytes & 2) ? r1 << 16 : r1));  // the last 2 + 1 bytes
+    const uint64_t rest = (bytes & 4) ? low << 32 | r4 : low;             // the last 4 + 2 + 1
+    w[0] = (bytes & 8) ? r8 : rest;
+    w[1] = (bytes & 8) ? rest : 0;
+}
+__device__ __forceinline__ void store_bytes(char* p, int bytes, const uint64_t (&w)[2]) {
+    if (bytes & 8) *(u64_any*)p = w[0];
+    const uint64_t rest = (bytes & 8) ? w[1] : w[0];
+    if (bytes & 4) *(u32_any*)(p + (bytes & 8)) = (uint32_t)rest;
+    const uint32_t low = (bytes & 4) ? (uint32_t)(rest >> 32) : (uint32_t)rest;
+    if (bytes & 2) *(u16_any*)(p + (bytes & 12)) = (uint16_t)low;
+    if (bytes & 1) *(uint8_t*)(p + (bytes & 14)) = (uint8_t)((bytes & 2) ? low >> 16 : low);
+}
+
 // the first n of N (n may be anything; n <= 0: nothing is touched), the others 0
 template <bool NT, typename T, int N>
 __device__ __forceinline__ raw_t<T, N> load_raw_upto(const T* p, int64_t n) {
+    static_assert(N * sizeof(T) <= 16, "one vector");
     raw_t<T, N> v = {};
     if (n >= N) {
         v = load_raw<NT, T, N>(p);
-    } else if (n > 0) {  // (all loads at once, the ones behind the last at its place: a branch each would be a wait each)
-#pragma unroll
-        for (int j = 0; j < N; j++) v[j] = p[j < n ? j : (int)n - 1];
-#pragma unroll
-        for (int j = 0; j < N; j++) v[j] = j < n ? v[j] : (T)0.0f;
+    } else if (n > 0) {
+        uint64_t w[2];
+        load_bytes((const char*)p, (int)n * (int)sizeof(T), w);
+        __builtin_memcpy(&v, w, N * sizeof(T));
     }
     return v;
+}
+template <bool NT, typename T, int N>
+__device__ __forceinline__ void store_raw_upto(T* p, int64_t n, raw_t<T, N> v) {
+    static_assert(N * sizeof(T) <= 16, "one vector");
+    if (n >= N) {
+        store_raw<NT, T, N>(p, v);
+    } else if (n > 0) {
+        uint64_t w[2] = {};
+        __builtin_memcpy(w, &v, N * sizeof(T));
+        store_bytes((char*)p, (int)n * (int)sizeof(T), w);
+    }
 }
 template <typename T, int N>
 __device__ __forceinline__ void widen(raw_t<T, N> v, float (&f)[N]) {
@@ -58,31 +95,38 @@ template <typename T, int N, bool NT = false>
 __device__ __forceinline__ void load_n(const T* p, float (&f)[N]) {
     widen<T, N>(load_raw<NT, T, N>(p), f);
 }
-template <typename T, int N, bool NT = false>
-__device__ __forceinline__ void store_n(T* p, const float (&f)[N]) {
+template <typename T, int N>
+__device__ __forceinline__ raw_t<T, N> narrow(const float (&f)[N]) {
     raw_t<T, N> v;
 #pragma unroll
     for (int j = 0; j < N; j++) v[j] = (T)f[j];
-    store_raw<NT, T, N>(p, v);
+    return v;
+}
+template <typename T, int N, bool NT = false>
+__device__ __forceinline__ void store_n(T* p, const float (&f)[N]) {
+    store_raw<NT, T, N>(p, narrow<T, N>(f));
 }
 
-// the same for the first n of N
+// the same for the first n of N, which may be several vectors of 16 bytes
 template <typename T, int N, bool NT = false>
 __device__ __forceinline__ void load_upto(const T* p, int64_t n, float fill, float (&f)[N]) {
-    widen<T, N>(load_raw_upto<NT, T, N>(p, n), f);
-    if (n < N) {
+    constexpr int M = N * sizeof(T) <= 16 ? N : 16 / sizeof(T);
 #pragma unroll
-        for (int j = 0; j < N; j++) f[j] = j < n ? f[j] : fill;
+    for (int q = 0; q < N; q += M) {
+        const raw_t<T, M> v = load_raw_upto<NT, T, M>(p + q, n - q);
+#pragma unroll
+        for (int j = 0; j < M; j++) f[q + j] = q + j < n ? (float)v[j] : fill;
     }
 }
 template <typename T, int N, bool NT = false>
 __device__ __forceinline__ void store_upto(T* p, int64_t n, const float (&f)[N]) {
-    if (n >= N) {
-        store_n<T, N, NT>(p, f);
-    } else {
+    constexpr int M = N * sizeof(T) <= 16 ? N : 16 / sizeof(T);
 #pragma unroll
-        for (int j = 0; j < N; j++)
-            if (j < n) p[j] = (T)f[j];
+    for (int q = 0; q < N; q += M) {
+        raw_t<T, M> v;
+#pragma unroll
+        for (int j = 0; j < M; j++) v[j] = (T)f[q + j];
+        store_raw_upto<NT, T, M>(p + q, n - q, v);
     }
 }
 
