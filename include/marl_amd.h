@@ -555,8 +555,8 @@ int ec_bn_relu_dropout_bwd_dx(const float* dout, const float* x, const float* sc
 #define EC_BF16 1
 #define EC_F16 2
 
-/* Layer norm over the last dimension.  x [rows][cols] of `dtype` with row stride x_stride (elements, >= 0; the columns are
- * contiguous, any alignment); weight, bias [cols] of wdtype (EC_F32 or dtype), each optional (1 and 0).
+/* Layer norm over the last dimension.  x [rows][cols] of `dtype` with row stride x_stride (elements; at least cols, the
+ * columns are contiguous, any alignment); weight, bias [cols] of wdtype (EC_F32 or dtype), each optional (1 and 0).
  *   y = (x - mean) / sqrt(var + eps) * weight + bias, var = mean (x - mean)^2;  y [rows][cols] contiguous;
  *   mean, rstd [rows] f32, each optional.  1 <= cols <= 2^24. */
 int ec_layer_norm_fwd(const void* x, int64_t x_stride, const void* weight, const void* bias, int32_t dtype, int32_t wdtype,

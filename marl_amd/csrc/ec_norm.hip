@@ -40,6 +40,19 @@ __device__ __forceinline__ void load_weight(const void* w, int wdtype, int c, in
 
 constexpr int block_threads(int tpr) { return tpr < 256 ? 256 : tpr; }
 
+// the wave of this thread's row whose value this lane picks up: each of a row's TPR / 64 waves by some lane of a group
+template <int TPR>
+__device__ __forceinline__ int wave_slot() {
+    return ((threadIdx.x >> 6) & ~(TPR / 64 - 1)) | (threadIdx.x & (TPR / 64 - 1));
+}
+
+// 1 / sqrt(v) to one unit in the last place, for every v >= 0 (the instruction alone takes what is below 2^-126 as 0)
+__device__ __forceinline__ float inverse_root(float v) {
+    const bool small = v < 1e-30f;
+    const float q = __builtin_amdgcn_rsqf(small ? v * 18446744073709551616.0f : v);
+    return small ? q * 4294967296.0f : q;
+}
+
 // sum of (a, b) over the threads of a row.  TPR <= 64: in the wave; else through LDS, one barrier: `slot` alternates from
 // call to call, so that the reads of one call are over before the call after the next writes
 template <int TPR>
@@ -49,54 +62,79 @@ __device__ __forceinline__ void row_sum2(float& a, float& b, float2 (*s)[16], in
     if (TPR > 64) {
         if ((threadIdx.x & 63) == 0) s[slot][threadIdx.x >> 6] = make_float2(a, b);
         __syncthreads();
-        const float2 v = s[slot][threadIdx.x & (TPR / 64 - 1)];  // (a wave's value in each lane of a group)
+        const float2 v = s[slot][wave_slot<TPR>()];
         a = lanes_sum<TPR / 64>(v.x);
         b = lanes_sum<TPR / 64>(v.y);
     }
 }
 
-// Vectors of a row, and what of them belongs to it.  A row's last vector is read whole where that stays inside the tensor
-// (it then holds the start of the next row, or padding) and masked: reading it element by element would cost every row a
-// wait of its own.
-template <typename T, int V>
-struct Mask {
-    uint32_t w[4];
-    __device__ __forceinline__ void set(int n) {  // the first n
+// How a thread reads its vectors of a row: always, from an address inside the tensor, with no branch, and what does not
+// belong to the row is masked afterwards.  A row's last vector is read whole (it then holds the start of the next row, or
+// padding); at the end of the tensor it is read as much further in front as it sticks out, and shifted; a thread with no
+// columns reads the row's first.  (Read element by element, or under a condition, each would be a wait of its own.)
+template <typename T, int V, int TPR, int NV, bool NT>
+struct RowReader {
+    const T* base;
+    int64_t stride, rows, end;  // end: the tensor's last element plus one, at least V
+    int cols;
+    bool exact;                 // all of it belongs to the row, for every thread
+    __device__ __forceinline__ RowReader(const void* b, int64_t stride_, int64_t rows_, int cols_)
+        : base((const T*)b), stride(stride_), rows(rows_), end((rows_ - 1) * stride_ + cols_), cols(cols_), exact(cols_ == TPR * NV * V) {}
+    __device__ __forceinline__ int64_t row(int64_t r) const { return (r < rows ? r : rows - 1) * stride; }
+    __device__ __forceinline__ void load(int64_t r, int t, raw_t<T, V> (&v)[NV]) const {
+        const int64_t off = row(r);
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const int left = (n - k * (V / 4)) * (int)sizeof(T) * 8;  // bits of this word
-            w[k] = left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1;
+        for (int i = 0; i < NV; i++) {
+            const int c = (i * TPR + t) * V;
+            const int64_t at = off + (c < cols ? c : 0);
+            v[i] = load_raw<NT, T, V>(base + (at + V <= end ? at : end - V));
         }
     }
-    __device__ __forceinline__ raw_t<T, V> of(raw_t<T, V> v) const {
-        uint32_t u[4];
-        __builtin_memcpy(u, &v, 16);
+    // the words of a vector's first n elements
+    __device__ __forceinline__ static Words first(int n) {
+        const int keep = n * (int)sizeof(T) * 8;
+        return Words{keep >= 64 ? ~0ull : keep <= 0 ? 0ull : (1ull << keep) - 1, keep >= 128 ? ~0ull : keep <= 64 ? 0ull : (1ull << (keep - 64)) - 1};
+    }
+    __device__ __forceinline__ void masks(int t, Words (&m)[NV]) const {
 #pragma unroll
-        for (int k = 0; k < 4; k++) u[k] &= w[k];
-        __builtin_memcpy(&v, u, 16);
-        return v;
+        for (int i = 0; i < NV; i++) m[i] = first(cols - (i * TPR + t) * V);
+    }
+    __device__ __forceinline__ void mask(int64_t r, int t, const Words (&m)[NV], raw_t<T, V> (&v)[NV]) const {
+        if (exact) return;
+        const int64_t past = row(r) + V - end;
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int c = (i * TPR + t) * V;
+            Words w;
+            __builtin_memcpy(&w, &v[i], 16);
+            if (c < cols && past + c > 0) {  // (the tensor's last vector: read past + c elements early)
+                const int bits = (int)(past + c) * (int)sizeof(T) * 8;
+                w = bits >= 64 ? Words{w.hi >> (bits - 64), 0} : Words{w.lo >> bits | w.hi << (64 - bits), w.hi >> bits};
+            }
+            w.lo &= m[i].lo;
+            w.hi &= m[i].hi;
+            __builtin_memcpy(&v[i], &w, 16);
+        }
     }
 };
-// v, of which the compiler from here on knows nothing: what was made from it before is made again, not kept
-template <typename T, int V>
-__device__ __forceinline__ raw_t<T, V> afresh(raw_t<T, V> v) {
-    uint32_t u[4];
-    __builtin_memcpy(u, &v, 16);
-    asm volatile("" : "+v"(u[0]), "+v"(u[1]), "+v"(u[2]), "+v"(u[3]));
-    __builtin_memcpy(&v, u, 16);
-    return v;
-}
-// the vector of column c < cols of a row at `off`; end: the tensor's last element plus one
-template <bool NT, typename T, int V>
-__device__ __forceinline__ raw_t<T, V> row_vector(const T* base, int64_t off, int c, int cols, int64_t end) {
-    if (off + c + V <= end) return load_raw<NT, T, V>(base + off + c);
-    return load_raw_upto<NT, T, V>(base + off + c, cols - c);
+
+// v, of which the compiler from here on knows nothing.  What was made from it before is made again, not kept; and a load of
+// it is waited for here (by itself the compiler waits for the next row only behind this row's stores, and so for these too)
+template <typename T, int V, int NV>
+__device__ __forceinline__ void afresh(raw_t<T, V> (&v)[NV]) {
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        uint32_t u[4];
+        __builtin_memcpy(u, &v[i], 16);
+        asm volatile("" : "+v"(u[0]), "+v"(u[1]), "+v"(u[2]), "+v"(u[3]));
+        __builtin_memcpy(&v[i], u, 16);
+    }
 }
 
 template <typename T, int TPR, int NV, bool NT>
 __global__ void __launch_bounds__(block_threads(TPR)) k_ln_fwd(NormArgs p) {
     constexpr int V = 16 / sizeof(T), RPB = block_threads(TPR) / TPR;
-    __shared__ float4 s_red[2][TPR > 64 ? TPR / 64 : 1];
+    __shared__ float4 s_red[2][block_threads(TPR) / 64];
     const int t = threadIdx.x % TPR, g = threadIdx.x / TPR;
     float w[NV][V], b[NV][V];
 #pragma unroll
@@ -118,30 +156,20 @@ __global__ void __launch_bounds__(block_threads(TPR)) k_ln_fwd(NormArgs p) {
     int slot = 0;
     // (every thread of a block makes every round: the lane sums and barriers are for all; rows behind the last are read
     // as the last and not written)
-    const bool ragged = p.cols % V != 0;
-    Mask<T, V> mask[NV];
-#pragma unroll
-    for (int i = 0; i < NV; i++) mask[i].set(p.cols - (i * TPR + t) * V);
-    const int64_t end = (p.rows - 1) * p.x_stride + p.cols;
-    raw_t<T, V> next[NV];
-    const auto fetch = [&](int64_t r0) {
-        const int64_t off = (r0 + g < p.rows ? r0 + g : p.rows - 1) * p.x_stride;
-#pragma unroll
-        for (int i = 0; i < NV; i++) {
-            const int c = (i * TPR + t) * V;
-            next[i] = raw_t<T, V>{};
-            if (c < p.cols) next[i] = row_vector<NT, T, V>((const T*)p.x, off, c, p.cols, end);
-        }
-    };
-    fetch((int64_t)blockIdx.x * RPB);
+    const RowReader<T, V, TPR, NV, NT> in(p.x, p.x_stride, p.rows, p.cols);
+    raw_t<T, V> x[NV], next[NV];
+    Words own[NV];
+    in.masks(t, own);
+    in.load((int64_t)blockIdx.x * RPB + g, t, x);
     for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < p.rows; r0 += (int64_t)gridDim.x * RPB, slot ^= 1) {
-        const bool on = r0 + g < p.rows;
         const int64_t r = r0 + g;
+        const bool on = r < p.rows, more = r0 + (int64_t)gridDim.x * RPB < p.rows;
+        in.mask(r, t, own, x);
+        if (more) in.load(r + (int64_t)gridDim.x * RPB, t, next);  // (while this row is worked on)
         float f[NV][V];
         float sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NV; i++) widen<T, V>(ragged ? mask[i].of(next[i]) : next[i], f[i]);
-        if (r0 + (int64_t)gridDim.x * RPB < p.rows) fetch(r0 + (int64_t)gridDim.x * RPB);  // (while this row is worked on)
+        for (int i = 0; i < NV; i++) widen<T, V>(x[i], f[i]);
 #pragma unroll
         for (int i = 0; i < NV; i++)
 #pragma unroll
@@ -164,19 +192,28 @@ __global__ void __launch_bounds__(block_threads(TPR)) k_ln_fwd(NormArgs p) {
         if (TPR > 64) {
             if ((threadIdx.x & 63) == 0) s_red[slot][threadIdx.x >> 6] = make_float4(sum, about, sq, n_wave);
             __syncthreads();
-            const float4 v = s_red[slot][threadIdx.x & (TPR / 64 - 1)];
+            const float4 v = s_red[slot][wave_slot<(TPR > 64 ? TPR : 64)>()];
             mean = lanes_sum<TPR / 64>(v.x) * inv_c;
             sq = lanes_sum<TPR / 64>(v.z + v.w * (v.y - mean) * (v.y - mean));
         }
-        const float rstd = 1.0f / sqrtf(sq * inv_c + p.eps);
+        const float rstd = inverse_root(sq * inv_c + p.eps);
+        raw_t<T, V> y[NV];
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+#pragma unroll
+            for (int j = 0; j < V; j++) f[i][j] = __builtin_fmaf((f[i][j] - mean) * rstd, w[i][j], b[i][j]);
+            y[i] = narrow<T, V>(f[i]);
+        }
+        if (more) {
+            afresh<T, V, NV>(next);
+#pragma unroll
+            for (int i = 0; i < NV; i++) x[i] = next[i];
+        }
         if (on) {
-            T* y = (T*)p.out + r * p.cols;
 #pragma unroll
             for (int i = 0; i < NV; i++) {
                 const int c = (i * TPR + t) * V;
-#pragma unroll
-                for (int j = 0; j < V; j++) f[i][j] = __builtin_fmaf((f[i][j] - mean) * rstd, w[i][j], b[i][j]);
-                store_upto<T, V, NT>(y + c, p.cols - c, f[i]);
+                store_raw_upto<NT, T, V>((T*)p.out + r * p.cols + c, p.cols - c, y[i]);
             }
             if (t == 0) {
                 if (p.mean) p.mean[r] = mean;
@@ -201,45 +238,31 @@ __global__ void __launch_bounds__(block_threads(TPR)) k_ln_bwd(NormArgs p) {
     }
     const float inv_c = 1.0f / (float)p.cols;
     int slot = 0;
-    const bool ragged = p.cols % V != 0;
-    Mask<T, V> mask[NV];
-#pragma unroll
-    for (int i = 0; i < NV; i++) mask[i].set(p.cols - (i * TPR + t) * V);
-    const int64_t end_x = (p.rows - 1) * p.x_stride + p.cols, end_dy = (p.rows - 1) * p.dy_stride + p.cols;
-    raw_t<T, V> next_x[NV], next_dy[NV];
-    float next_mean, next_rstd;
-    const auto fetch = [&](int64_t r0) {
-        const bool on = r0 + g < p.rows;
-        const int64_t r = on ? r0 + g : p.rows - 1;
-        // a row behind the last adds nothing to dw and db: its dy is taken as 0
-#pragma unroll
-        for (int i = 0; i < NV; i++) {
-            const int c = (i * TPR + t) * V;
-            next_x[i] = next_dy[i] = raw_t<T, V>{};
-            if (c < p.cols) {
-                next_x[i] = row_vector<NT, T, V>((const T*)p.x, r * p.x_stride, c, p.cols, end_x);
-                if (on) next_dy[i] = row_vector<NT, T, V>((const T*)p.dy, r * p.dy_stride, c, p.cols, end_dy);
-            }
-        }
-        next_mean = p.mean[r], next_rstd = p.rstd[r];
-    };
-    // (a block of 1024 threads has 128 registers a thread: no room for the next row with two vectors or more)
+    const RowReader<T, V, TPR, NV, NT> in_x(p.x, p.x_stride, p.rows, p.cols), in_dy(p.dy, p.dy_stride, p.rows, p.cols);
+    // (a block of 1024 threads has 128 registers a thread: no room for the next row with two vectors or more; the row then
+    // stays as it was read, and xhat and dy w are made from it twice)
     constexpr bool AHEAD = TPR < 1024 || NV == 1;
-    if (AHEAD) fetch((int64_t)blockIdx.x * RPB);
+    raw_t<T, V> x[NV], dy[NV], next_x[NV], next_dy[NV];
+    float mean = 0.0f, rstd = 0.0f, next_mean = 0.0f, next_rstd = 0.0f;
+    Words own[NV];
+    in_x.masks(t, own);
+    const auto load = [&](int64_t r, raw_t<T, V>(&a)[NV], raw_t<T, V>(&b)[NV], float& m, float& s) {
+        in_x.load(r, t, a);
+        in_dy.load(r, t, b);
+        m = p.mean[r < p.rows ? r : p.rows - 1], s = p.rstd[r < p.rows ? r : p.rows - 1];
+    };
+    load((int64_t)blockIdx.x * RPB + g, x, dy, mean, rstd);
     for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < p.rows; r0 += (int64_t)gridDim.x * RPB, slot ^= 1) {
-        const bool on = r0 + g < p.rows;
-        const int64_t r = r0 + g;
-        // (without room for the next row the row stays as it was read, and xhat is made from it twice: half the registers)
-        raw_t<T, V> x[NV], dy[NV];
-        if (!AHEAD) fetch(r0);
+        const int64_t r = r0 + g, r_next = r + (int64_t)gridDim.x * RPB;
+        const bool on = r < p.rows, more = r0 + (int64_t)gridDim.x * RPB < p.rows;
+        in_x.mask(r, t, own, x);
+        in_dy.mask(r, t, own, dy);
+        if (AHEAD && more) load(r_next, next_x, next_dy, next_mean, next_rstd);  // (while this row is worked on)
+        if (RPB > 1 && !on) {  // a row behind the last adds nothing to dw and db
 #pragma unroll
-        for (int i = 0; i < NV; i++) {
-            x[i] = ragged ? mask[i].of(next_x[i]) : next_x[i];
-            dy[i] = ragged ? mask[i].of(next_dy[i]) : next_dy[i];
+            for (int i = 0; i < NV; i++) dy[i] = raw_t<T, V>{};
         }
-        const float mean = next_mean, rstd = next_rstd;
-        if (AHEAD && r0 + (int64_t)gridDim.x * RPB < p.rows) fetch(r0 + (int64_t)gridDim.x * RPB);  // (while this row is worked on)
-        float s1 = 0.0f, s2 = 0.0f;
+        float s1 = 0.0f, s2 = 0.0f, hs[AHEAD ? NV : 1][V], as[AHEAD ? NV : 1][V];
 #pragma unroll
         for (int i = 0; i < NV; i++) {
 #pragma unroll
@@ -250,28 +273,45 @@ __global__ void __launch_bounds__(block_threads(TPR)) k_ln_bwd(NormArgs p) {
                 db[i][j] += d;
                 s1 += a;
                 s2 = __builtin_fmaf(a, h, s2);
+                if (AHEAD) hs[AHEAD ? i : 0][j] = h, as[AHEAD ? i : 0][j] = a;
             }
             if (!AHEAD) __builtin_amdgcn_sched_barrier(0);  // (vectors one after the other: interleaved they need more registers)
         }
         row_sum2<TPR>(s1, s2, s_red, slot);
         s1 *= inv_c;
         s2 *= inv_c;
+        if (!AHEAD) {
+            afresh<T, V, NV>(x);
+            afresh<T, V, NV>(dy);
+        }
+        raw_t<T, V> dx[NV];
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            float o[V];
+#pragma unroll
+            for (int j = 0; j < V; j++) {
+                const float h = AHEAD ? hs[AHEAD ? i : 0][j] : ((float)x[i][j] - mean) * rstd;
+                const float a = AHEAD ? as[AHEAD ? i : 0][j] : (float)dy[i][j] * w[i][j];
+                o[j] = rstd * (a - s1 - h * s2);
+            }
+            dx[i] = narrow<T, V>(o);
+            if (!AHEAD) __builtin_amdgcn_sched_barrier(0);
+        }
+        if (AHEAD && more) {
+            afresh<T, V, NV>(next_x);
+            afresh<T, V, NV>(next_dy);
+#pragma unroll
+            for (int i = 0; i < NV; i++) x[i] = next_x[i], dy[i] = next_dy[i];
+            mean = next_mean, rstd = next_rstd;
+        }
         if (on && p.out) {
-            T* dx = (T*)p.out + r * p.cols;
 #pragma unroll
             for (int i = 0; i < NV; i++) {
                 const int c = (i * TPR + t) * V;
-                const raw_t<T, V> x2 = AHEAD ? x[i] : afresh<T, V>(x[i]), dy2 = AHEAD ? dy[i] : afresh<T, V>(dy[i]);
-                float o[V];
-#pragma unroll
-                for (int j = 0; j < V; j++) {
-                    const float h = ((float)x2[j] - mean) * rstd;
-                    o[j] = rstd * (__builtin_fmaf((float)dy2[j], w[i][j], -s1) - h * s2);
-                }
-                store_upto<T, V, NT>(dx + c, p.cols - c, o);
-                if (!AHEAD) __builtin_amdgcn_sched_barrier(0);
+                store_raw_upto<NT, T, V>((T*)p.out + r * p.cols + c, p.cols - c, dx[i]);
             }
         }
+        if (!AHEAD && more) load(r_next, x, dy, mean, rstd);
     }
     if (!p.partials) return;
     float* part = p.partials + (int64_t)blockIdx.x * 2 * p.cols;
@@ -279,7 +319,7 @@ __global__ void __launch_bounds__(block_threads(TPR)) k_ln_bwd(NormArgs p) {
     for (int i = 0; i < NV; i++) {
         const int c = (i * TPR + t) * V;
         if (RPB > 1) {  // the row groups of a wave, then the waves, in a fixed order
-            const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+            constexpr int APART = TPR < 64 ? 64 : TPR;
             __syncthreads();
 #pragma unroll
             for (int j = 0; j < V; j++) {
@@ -292,13 +332,13 @@ __global__ void __launch_bounds__(block_threads(TPR)) k_ln_bwd(NormArgs p) {
                 s_part[1][j][threadIdx.x] = db[i][j];
             }
             __syncthreads();
-            if (wave == 0 && lane < TPR)
+            if ((int)threadIdx.x < TPR)
 #pragma unroll
-                for (int k = 1; k < 4; k++)
+                for (int k = APART; k < 256; k += APART)
 #pragma unroll
                     for (int j = 0; j < V; j++) {
-                        dw[i][j] += s_part[0][j][k * 64 + t];
-                        db[i][j] += s_part[1][j][k * 64 + t];
+                        dw[i][j] += s_part[0][j][k + t];
+                        db[i][j] += s_part[1][j][k + t];
                     }
         }
         if ((int)threadIdx.x < TPR) {
@@ -357,7 +397,7 @@ __global__ void __launch_bounds__(WIDE) k_ln_fwd_wide(NormArgs p) {
             for (int j = 0; j < V; j++) sq = __builtin_fmaf(f[j] - mean, f[j] - mean, sq);
         }
         row_sum2<WIDE>(sq, b, s_red, 1);
-        const float rstd = 1.0f / sqrtf(sq / (float)p.cols + p.eps);
+        const float rstd = inverse_root(sq / (float)p.cols + p.eps);
         for (int64_t c = threadIdx.x * V; c < p.cols; c += WIDE * V) {
             float w[V], bb[V];
             load_upto(x + c, p.cols - c, 0.0f, f);
@@ -431,21 +471,39 @@ __global__ void __launch_bounds__(64) k_ln_dw_wide(NormArgs p) {
     store_upto(part + p.cols + c, p.cols - c, db);
 }
 
-// ---- which variant: the fewest threads per row that hold it in one vector each; two or four beyond 1024 threads ----
+// ---- which variant: one vector a thread up to a wave, then as many elements a thread as registers allow before more threads:
+// the sums over a row's threads cost about 100 operations a thread and row, as much as four elements do (16384 rows of 4096 in
+// bf16, forward: 512 threads with 8 each 59 us, 256 with 16 each 50 us).  Backward, where a thread also holds its sums of dw and
+// db, 16 elements leave two waves a SIMD, which is enough up to 2048 columns of 16 bits and not beyond (4096 columns: 81 us,
+// with 512 threads of 8 each 72) ----
 struct Shape {
     int tpr, nv, rpb;  // tpr 0: the wide kernels
 };
-Shape shape_for(int64_t cols, int dtype) {
-    const int64_t vecs = cdiv(cols, dtype == EC_F32 ? 4 : 8);
-    for (int tpr : {2, 4, 8, 16, 32, 64, 128, 256, 512, 1024})
-        if (vecs <= tpr) return tpr == 128 ? Shape{64, 2, 4} : Shape{tpr, 1, block_threads(tpr) / tpr};
-    if (vecs <= 2048) return {1024, 2, 1};
-    if (vecs <= 4096 && dtype == EC_F32) return {1024, 4, 1};
+Shape shape_for(int64_t rows, int64_t cols, int dtype, bool bwd) {
+    const bool f32 = dtype == EC_F32;
+    const int64_t vecs = cdiv(cols, f32 ? 4 : 8);
+    if (rows * cols < (f32 ? 4 : 8)) return {0, 0, 1};  // (less than a vector: RowReader)
+    for (int tpr : {2, 4, 8, 16, 32, 64})
+        if (vecs <= tpr) return {tpr, 1, 256 / tpr};
+    if (vecs <= 128) return {64, 2, 4};
+    const int most = f32 ? 4 : 2;
+    for (int tpr : {64, 128, 256, 512, 1024}) {
+        const int nv = bwd && !f32 && tpr >= 256 ? 1 : most;
+        if (vecs <= tpr * nv) return {tpr, nv, block_threads(tpr) / tpr};
+    }
+    if (vecs <= (f32 ? 4096 : 2048)) return {1024, f32 ? 4 : 2, 1};
     return {0, 0, 1};
 }
 
-int bwd_blocks(const Shape& s, int64_t rows) {
-    const int64_t want = cdiv(rows, s.rpb), most = NUM_CU * (s.tpr <= 256 ? 4 : s.tpr == 512 ? 2 : 1);
+// Waves a CU, as swept (1 to 16 blocks a CU over widths from 11 to 16384): what fills the memory's queue, and no more than
+// the registers keep resident; blocks beyond that run behind each other and read their weights again.  4.1 M rows of 64 in
+// fp32: forward 16 waves 967 us, 32 waves 994; backward 12 waves 964 us, 16 waves 997, 8 waves 988 (forward and back each).
+int blocks_for(const Shape& s, int64_t rows, int dtype, bool bwd) {
+    const int elements = s.nv * (dtype == EC_F32 ? 4 : 8);
+    int waves = 16;
+    if (!bwd) waves = s.tpr <= 8 ? 32 : elements > 8 && dtype == EC_F32 ? 12 : 16;
+    else if (s.tpr < 1024 && s.tpr > 8) waves = s.nv > 1 ? 8 : s.tpr < 512 ? 12 : 16;
+    const int64_t want = cdiv(rows, s.rpb), each = waves * 64 / block_threads(s.tpr), most = NUM_CU * (each < 1 ? 1 : each);
     return (int)(want < most ? want : most);
 }
 int wide_parts(int64_t rows) { return (int)(rows < 32 ? rows : 32); }
@@ -470,8 +528,14 @@ template <typename T, bool BWD>
 void dispatch(const NormArgs& a, const Shape& s, unsigned blocks, hipStream_t st) {
 #define EC_LN(TPR, NV) \
     if (s.tpr == TPR && s.nv == NV) return go<T, BWD, TPR, NV>(a, blocks, st);
-    EC_LN(2, 1) EC_LN(4, 1) EC_LN(8, 1) EC_LN(16, 1) EC_LN(32, 1) EC_LN(64, 1) EC_LN(64, 2) EC_LN(256, 1) EC_LN(512, 1) EC_LN(1024, 1) EC_LN(1024, 2)
-    if constexpr (sizeof(T) == 4) { EC_LN(1024, 4) }
+    EC_LN(2, 1) EC_LN(4, 1) EC_LN(8, 1) EC_LN(16, 1) EC_LN(32, 1) EC_LN(64, 1) EC_LN(64, 2)
+    if constexpr (sizeof(T) == 4) {
+        EC_LN(64, 4) EC_LN(128, 4) EC_LN(256, 4) EC_LN(512, 4) EC_LN(1024, 4)
+    } else if constexpr (BWD) {
+        EC_LN(128, 2) EC_LN(512, 1) EC_LN(1024, 1) EC_LN(1024, 2)
+    } else {
+        EC_LN(128, 2) EC_LN(256, 2) EC_LN(512, 2) EC_LN(1024, 2)
+    }
 #undef EC_LN
 }
 
@@ -482,8 +546,10 @@ const char* bad_args(const char* who, const void* x, int64_t x_stride, int32_t d
         snprintf(msg, sizeof msg, "%s: type %d with weights of type %d", who, dtype, wdtype);
     else if (rows < 0 || cols < 1 || cols > (1 << 24))
         snprintf(msg, sizeof msg, "%s: %lld rows of %lld columns (1 .. 2^24)", who, (long long)rows, (long long)cols);
-    else if (rows && (!x || x_stride < 0))
-        snprintf(msg, sizeof msg, "%s: no input, or a negative row stride", who);
+    else if (rows && !x)
+        snprintf(msg, sizeof msg, "%s: no input", who);
+    else if (x_stride < 0 || (rows > 1 && x_stride < cols))
+        snprintf(msg, sizeof msg, "%s: rows of %lld columns %lld apart", who, (long long)cols, (long long)x_stride);
     else
         return nullptr;
     return msg;
@@ -501,15 +567,14 @@ extern "C" int ec_layer_norm_fwd(const void* x, int64_t x_stride, const void* we
     a.x = x, a.w = weight, a.b = bias, a.x_stride = x_stride, a.rows = rows, a.cols = (int)cols, a.wdtype = wdtype;
     a.eps = (float)eps, a.mean = mean, a.rstd = rstd, a.out = y;
     const hipStream_t st = (hipStream_t)stream;
-    const Shape s = shape_for(cols, dtype);
+    const Shape s = shape_for(rows, cols, dtype, false);
     if (s.tpr == 0) {
         const dim3 grid((unsigned)(rows < 1024 ? rows : 1024));
         if (dtype == EC_F32) hipLaunchKernelGGL(k_ln_fwd_wide<float>, grid, dim3(WIDE), 0, st, a);
         if (dtype == EC_BF16) hipLaunchKernelGGL(k_ln_fwd_wide<bf16>, grid, dim3(WIDE), 0, st, a);
         if (dtype == EC_F16) hipLaunchKernelGGL(k_ln_fwd_wide<f16>, grid, dim3(WIDE), 0, st, a);
     } else {
-        const int64_t want = cdiv(rows, s.rpb), most = NUM_CU * (s.tpr <= 256 ? 8 : s.tpr == 512 ? 4 : 2);
-        const unsigned blocks = (unsigned)(want < most ? want : most);
+        const unsigned blocks = (unsigned)blocks_for(s, rows, dtype, false);
         if (dtype == EC_F32) dispatch<float, false>(a, s, blocks, st);
         if (dtype == EC_BF16) dispatch<bf16, false>(a, s, blocks, st);
         if (dtype == EC_F16) dispatch<f16, false>(a, s, blocks, st);
@@ -520,8 +585,8 @@ extern "C" int ec_layer_norm_fwd(const void* x, int64_t x_stride, const void* we
 
 extern "C" int64_t ec_layer_norm_bwd_partials(int64_t rows, int64_t cols, int32_t dtype) {
     if (rows < 1 || cols < 1 || cols > (1 << 24) || !dtype_ok(dtype)) return 0;
-    const Shape s = shape_for(cols, dtype);
-    return s.tpr ? bwd_blocks(s, rows) : wide_parts(rows);
+    const Shape s = shape_for(rows, cols, dtype, true);
+    return s.tpr ? blocks_for(s, rows, dtype, true) : wide_parts(rows);
 }
 
 extern "C" int ec_layer_norm_bwd(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const float* mean,
@@ -531,7 +596,9 @@ extern "C" int ec_layer_norm_bwd(const void* dy, int64_t dy_stride, const void* 
     if (const char* m = bad_args("ec_layer_norm_bwd", x, x_stride, dtype, wdtype, rows, cols)) return ec::fail(EC_EINVAL, "%s", m);
     if (rows < 1) return ec::fail(EC_EINVAL, "ec_layer_norm_bwd: no rows");
     const bool want_w = dweight || dbias;
-    if (!dy || dy_stride < 0 || !mean || !rstd) return ec::fail(EC_EINVAL, "ec_layer_norm_bwd: null argument");
+    if (!dy || !mean || !rstd) return ec::fail(EC_EINVAL, "ec_layer_norm_bwd: null argument");
+    if (dy_stride < 0 || (rows > 1 && dy_stride < cols))
+        return ec::fail(EC_EINVAL, "ec_layer_norm_bwd: rows of %lld columns %lld apart", (long long)cols, (long long)dy_stride);
     const int64_t need = ec_layer_norm_bwd_partials(rows, cols, dtype);
     if (want_w && (!partials || n_partials != need))
         return ec::fail(EC_EINVAL, "ec_layer_norm_bwd: %lld partial rows (%lld are needed)", (long long)(partials ? n_partials : 0),
@@ -542,7 +609,7 @@ extern "C" int ec_layer_norm_bwd(const void* dy, int64_t dy_stride, const void* 
     a.wdtype = wdtype, a.mean = const_cast<float*>(mean), a.rstd = const_cast<float*>(rstd), a.out = dx;
     a.partials = want_w ? partials : nullptr;
     const hipStream_t st = (hipStream_t)stream;
-    const Shape s = shape_for(cols, dtype);
+    const Shape s = shape_for(rows, cols, dtype, true);
     if (s.tpr == 0) {
         if (dx) {
             const dim3 grid((unsigned)(rows < 1024 ? rows : 1024));

@@ -39,7 +39,10 @@ __device__ __forceinline__ void store_raw(T* p, raw_t<T, N> v) {
 typedef uint64_t u64_any __attribute__((aligned(1)));
 typedef uint32_t u32_any __attribute__((aligned(1)));
 typedef uint16_t u16_any __attribute__((aligned(1)));
-__device__ __forceinline__ void load_bytes(const char* p, int bytes, uint64_t (&w)[2]) {
+struct Words {
+    uint64_t lo, hi;
+};
+__device__ __forceinline__ Words load_bytes(const char* p, int bytes) {
     uint64_t r8 = 0;
     uint32_t r4 = 0, r2 = 0, r1 = 0;
     if (bytes & 8) r8 = *(const u64_any*)p;
@@ -48,12 +51,11 @@ __device__ __forceinline__ void load_bytes(const char* p, int bytes, uint64_t (&
     if (bytes & 1) r1 = *(const uint8_t*)(p + (bytes & 14));
     const uint64_t low = (uint64_t)(r2 | ((bytes & 2) ? r1 << 16 : r1));  // the last 2 + 1 bytes
     const uint64_t rest = (bytes & 4) ? low << 32 | r4 : low;             // the last 4 + 2 + 1
-    w[0] = (bytes & 8) ? r8 : rest;
-    w[1] = (bytes & 8) ? rest : 0;
+    return (bytes & 8) ? Words{r8, rest} : Words{rest, 0};
 }
-__device__ __forceinline__ void store_bytes(char* p, int bytes, const uint64_t (&w)[2]) {
-    if (bytes & 8) *(u64_any*)p = w[0];
-    const uint64_t rest = (bytes & 8) ? w[1] : w[0];
+__device__ __forceinline__ void store_bytes(char* p, int bytes, Words w) {
+    if (bytes & 8) *(u64_any*)p = w.lo;
+    const uint64_t rest = (bytes & 8) ? w.hi : w.lo;
     if (bytes & 4) *(u32_any*)(p + (bytes & 8)) = (uint32_t)rest;
     const uint32_t low = (bytes & 4) ? (uint32_t)(rest >> 32) : (uint32_t)rest;
     if (bytes & 2) *(u16_any*)(p + (bytes & 12)) = (uint16_t)low;
@@ -68,9 +70,8 @@ __device__ __forceinline__ raw_t<T, N> load_raw_upto(const T* p, int64_t n) {
     if (n >= N) {
         v = load_raw<NT, T, N>(p);
     } else if (n > 0) {
-        uint64_t w[2];
-        load_bytes((const char*)p, (int)n * (int)sizeof(T), w);
-        __builtin_memcpy(&v, w, N * sizeof(T));
+        const Words w = load_bytes((const char*)p, (int)n * (int)sizeof(T));
+        __builtin_memcpy(&v, &w, N * sizeof(T));
     }
     return v;
 }
@@ -80,8 +81,8 @@ __device__ __forceinline__ void store_raw_upto(T* p, int64_t n, raw_t<T, N> v) {
     if (n >= N) {
         store_raw<NT, T, N>(p, v);
     } else if (n > 0) {
-        uint64_t w[2] = {};
-        __builtin_memcpy(w, &v, N * sizeof(T));
+        Words w{0, 0};
+        __builtin_memcpy(&w, &v, N * sizeof(T));
         store_bytes((char*)p, (int)n * (int)sizeof(T), w);
     }
 }

@@ -54,10 +54,10 @@ def refuse_capture(who, instead):
 
 
 def _rows(t, cols):
-    """[rows, cols] with contiguous columns; a view where the strides allow one"""
+    """[rows, cols] with contiguous columns and rows that do not overlap; a view where the strides allow one"""
     if t.dim() != 2:
         t = t.reshape(-1, cols)
-    return t if cols == 1 or t.stride(1) == 1 else t.contiguous()
+    return t if (cols == 1 or t.stride(1) == 1) and (t.stride(0) >= cols or t.shape[0] <= 1) else t.contiguous()
 
 
 def _check(who, x, weight, bias, eps):

@@ -24,13 +24,13 @@ def test_layer_norm_refuses_bad_arguments():
     fwd = lambda x=PTR, xs=8, dt=0, wdt=0, rows=4, cols=8, eps=1e-5, y=PTR: L.ec_layer_norm_fwd(
         x, xs, PTR, PTR, dt, wdt, rows, cols, eps, y, PTR, PTR, NUL)
     for kw in (dict(dt=3), dict(dt=-1), dict(wdt=1), dict(dt=1, wdt=2), dict(rows=-1), dict(cols=0), dict(cols=(1 << 24) + 1),
-               dict(x=NUL), dict(xs=-1), dict(eps=-1.0), dict(eps=float("nan")), dict(y=NUL)):
+               dict(x=NUL), dict(xs=-1), dict(xs=7), dict(eps=-1.0), dict(eps=float("nan")), dict(y=NUL)):
         assert fwd(**kw) == EINVAL and "ec_layer_norm_fwd" in _message(), kw
     assert fwd(rows=0, x=NUL, y=NUL) == 0
     n = L.ec_layer_norm_bwd_partials(1000, 64, 0)
     bwd = lambda dy=PTR, dys=64, mean=PTR, rows=1000, part=PTR, n_part=n, dw=PTR, dx=PTR: L.ec_layer_norm_bwd(
         dy, dys, PTR, 64, mean, PTR, PTR, 0, 0, rows, 64, dx, part, n_part, dw, NUL, NUL)
-    for kw in (dict(dy=NUL), dict(dys=-2), dict(mean=NUL), dict(rows=0), dict(part=NUL), dict(n_part=n - 1), dict(n_part=n + 1)):
+    for kw in (dict(dy=NUL), dict(dys=-2), dict(dys=63), dict(mean=NUL), dict(rows=0), dict(part=NUL), dict(n_part=n - 1), dict(n_part=n + 1)):
         assert bwd(**kw) == EINVAL and "ec_layer_norm_bwd" in _message(), kw
     assert bwd(part=NUL, n_part=0, dw=NUL, dx=NUL) == 0            # nothing asked for
     assert L.ec_layer_norm_bwd_partials(0, 64, 0) == 0 and L.ec_layer_norm_bwd_partials(5, 0, 0) == 0
