@@ -473,104 +473,136 @@ __global__ void __launch_bounds__(256) k_logp_bwd(LpArgs p) {
 }
 
 // ---- few entries a row (the env's action sets): a lane per row ----
-// 256 rows are staged through LDS as fp32, excluded entries as -inf, at an odd stride (lanes that walk down their rows hit
-// different banks); packed rows come in and gradients leave 16 bytes a lane whatever the row's width.
-constexpr int FEW = 62;  // (64 KB of LDS a block)
+// FEW_ROWS rows are staged through LDS as fp32, excluded entries as -inf; packed rows come in and gradients leave 16 bytes a
+// lane whatever the row's width.  QUADS: widths that are multiples of 4 lie there at an odd multiple of 4, and lanes walk down
+// their rows four entries at a time; other widths at an odd stride, one at a time: different banks for different lanes either
+// way.  (128 rows a block: 64 and 256 are 2 to 12 % slower.)
+constexpr int FEW_ROWS = 128;
+// up to this width (600 000 rows of 60 forward and back: bf16 89 us, with 16 lanes a row 140; fp32 139 and 125)
+constexpr int FEW_16BIT = 62, FEW_FP32 = 52;
+
+__host__ __device__ inline int few_stride(int vocab) { return vocab % 4 ? vocab | 1 : 4 * (vocab / 4 | 1); }
 
 __device__ __forceinline__ int row_in(int i, int vocab, uint32_t by_vocab) {  // i / vocab
     return vocab == 1 ? i : (int)__umulhi((uint32_t)i, by_vocab);
 }
 
-template <typename T, int MASK>
+// f(entry, column) for the entries of a row; WRITE: f may change them
+template <bool QUADS, bool WRITE, typename F>
+__device__ __forceinline__ void each_entry(float* l, int vocab, F f) {
+    if (QUADS) {
+#pragma unroll 2
+        for (int j = 0; j < vocab; j += 4) {
+            float4 v = *(float4*)(l + j);
+            f(v.x, j), f(v.y, j + 1), f(v.z, j + 2), f(v.w, j + 3);
+            if (WRITE) *(float4*)(l + j) = v;
+        }
+    } else {
+#pragma unroll 4
+        for (int j = 0; j < vocab; j++) {
+            float v = l[j];
+            f(v, j);
+            if (WRITE) l[j] = v;
+        }
+    }
+}
+
+template <typename T, int MASK, bool QUADS>
 __device__ __forceinline__ void stage_rows(const LpArgs& p, int64_t r0, int n, int stride, uint32_t by_vocab, bool packed, float* s) {
     constexpr int V = 16 / sizeof(T);
     if (packed) {  // the tile is one run of n * vocab elements, in logits and mask
         const T* l = (const T*)p.logits + r0 * p.vocab;
         const char* av = MASK ? (const char*)p.avail + r0 * p.vocab * (MASK == 1 ? 1 : 4) : nullptr;
         const int all = n * p.vocab;
-        for (int i = threadIdx.x * V; i < all; i += 256 * V) {
+        for (int i = threadIdx.x * V; i < all; i += FEW_ROWS * V) {
             float f1[1][V], (&f)[V] = f1[0];
             if (i + V <= all) load_logits<T, MASK, false, true>(l, av, i, 0, all, f1);
             else load_logits<T, MASK, false, false>(l, av, i, 0, all, f1);
-            if (stride == p.vocab) {  // (an odd width is its own stride: the tile lies in LDS as in memory, which has room for the last)
+            if (QUADS) {  // (four entries in a row are of one row)
+#pragma unroll
+                for (int q = 0; q < V; q += 4) {
+                    const int row = row_in(i + q, p.vocab, by_vocab), col = i + q - row * p.vocab;
+                    if (i + q < all) *(float4*)(s + row * stride + col) = make_float4(f[q], f[q + 1], f[q + 2], f[q + 3]);
+                }
+            } else if (stride == p.vocab) {  // (the tile lies in LDS as in memory, with room for the last vector)
 #pragma unroll
                 for (int q = 0; q < V; q += 4) *(float4*)(s + i + q) = make_float4(f[q], f[q + 1], f[q + 2], f[q + 3]);
-                continue;
-            }
-            int row = row_in(i, p.vocab, by_vocab), col = i - row * p.vocab;
+            } else {
+                int row = row_in(i, p.vocab, by_vocab), col = i - row * p.vocab;
 #pragma unroll
-            for (int j = 0; j < V; j++) {
-                if (i + j < all) s[row * stride + col] = f[j];
-                if (++col == p.vocab) col = 0, row++;
+                for (int j = 0; j < V; j++) {
+                    if (i + j < all) s[row * stride + col] = f[j];
+                    if (++col == p.vocab) col = 0, row++;
+                }
             }
         }
     } else {
-        for (int i = threadIdx.x; i < n * p.vocab; i += 256) {
+        for (int i = threadIdx.x; i < n * p.vocab; i += FEW_ROWS) {
             const int row = row_in(i, p.vocab, by_vocab), col = i - row * p.vocab;
             s[row * stride + col] = logit_at<T, MASK>(row_of<T>(p, r0 + row), MASK ? mask_of<MASK>(p, r0 + row) : nullptr, col);
         }
     }
 }
 
-template <typename T, int MASK>
-__global__ void __launch_bounds__(256) k_logp_few_fwd(LpArgs p, uint32_t by_vocab, bool packed) {
-    extern __shared__ float s_rows[];
-    const int64_t r0 = (int64_t)blockIdx.x * 256, r = r0 + threadIdx.x;
-    const int n = (int)(p.rows - r0 < 256 ? p.rows - r0 : 256), stride = p.vocab | 1;
-    stage_rows<T, MASK>(p, r0, n, stride, by_vocab, packed, s_rows);
+template <typename T, int MASK, bool QUADS>
+__global__ void __launch_bounds__(FEW_ROWS) k_logp_few_fwd(LpArgs p, uint32_t by_vocab, bool packed) {
+    extern __shared__ float4 s_few[];
+    const int64_t r0 = (int64_t)blockIdx.x * FEW_ROWS, r = r0 + threadIdx.x;
+    const int n = (int)(p.rows - r0 < FEW_ROWS ? p.rows - r0 : FEW_ROWS), stride = few_stride(p.vocab);
+    stage_rows<T, MASK, QUADS>(p, r0, n, stride, by_vocab, packed, (float*)s_few);
     __syncthreads();
     if ((int)threadIdx.x >= n) return;
-    const float* l = s_rows + threadIdx.x * stride;
+    float* l = (float*)s_few + threadIdx.x * stride;
     Stat s{-FLT_MAX, 0.0f, 0.0f};
-#pragma unroll 4
-    for (int j = 0; j < p.vocab; j++) s.m = fmaxf(s.m, l[j]);
-#pragma unroll 4
-    for (int j = 0; j < p.vocab; j++) {
-        const float d = (l[j] - s.m) * LOG2E, e = __builtin_amdgcn_exp2f(d);
+    each_entry<QUADS, false>(l, p.vocab, [&](float& x, int) { s.m = fmaxf(s.m, x); });
+    each_entry<QUADS, false>(l, p.vocab, [&](float& x, int) {
+        const float d = (x - s.m) * LOG2E, e = __builtin_amdgcn_exp2f(d);
         s.s1 += e;
         s.s2 = __builtin_fmaf(e, fmaxf(d, -200.0f), s.s2);
-    }
+    });
     const float ln = log_s1(s);
     const int64_t tok = p.tokens[r];
     write_row(p, r, s, ln, logp_of(p, tok, tok >= 0 && tok < p.vocab ? l[tok] : 0.0f, s, ln));
-    float* left = s_rows + threadIdx.x * stride;
     for (int i = 0; i < p.top_k; i++) {  // the largest of what is left, the first of equal ones
         float best = -INF;
         int at = -1;
-#pragma unroll 4
-        for (int j = 0; j < p.vocab; j++) {
-            const bool more = left[j] > best;
-            best = more ? left[j] : best;
+        each_entry<QUADS, false>(l, p.vocab, [&](float& x, int j) {
+            const bool more = x > best;
+            best = more ? x : best;
             at = more ? j : at;
-        }
-        if (at >= 0) left[at] = -INF;
+        });
+        if (at >= 0) l[at] = -INF;
         write_top(p, r, i, s, ln, at >= 0 ? key_of(best, (uint32_t)at) : 0);
     }
 }
 
-template <typename T, int MASK>
-__global__ void __launch_bounds__(256) k_logp_few_bwd(LpArgs p, uint32_t by_vocab, bool packed) {
-    extern __shared__ float s_rows[];
+template <typename T, int MASK, bool QUADS>
+__global__ void __launch_bounds__(FEW_ROWS) k_logp_few_bwd(LpArgs p, uint32_t by_vocab, bool packed) {
+    extern __shared__ float4 s_few[];
     constexpr int V = 16 / sizeof(T);
-    const int64_t r0 = (int64_t)blockIdx.x * 256, r = r0 + threadIdx.x;
-    const int n = (int)(p.rows - r0 < 256 ? p.rows - r0 : 256), stride = p.vocab | 1;
-    stage_rows<T, MASK>(p, r0, n, stride, by_vocab, packed, s_rows);
+    float* const s_rows = (float*)s_few;
+    const int64_t r0 = (int64_t)blockIdx.x * FEW_ROWS, r = r0 + threadIdx.x;
+    const int n = (int)(p.rows - r0 < FEW_ROWS ? p.rows - r0 : FEW_ROWS), stride = few_stride(p.vocab);
+    stage_rows<T, MASK, QUADS>(p, r0, n, stride, by_vocab, packed, s_rows);
     __syncthreads();
     if ((int)threadIdx.x < n) {
         const RowGrad w = row_grad(p, r);
-        float* l = s_rows + threadIdx.x * stride;
-#pragma unroll 4
-        for (int j = 0; j < p.vocab; j++) l[j] = entry_grad(w, l[j], j);
+        each_entry<QUADS, true>(s_rows + threadIdx.x * stride, p.vocab, [&](float& x, int j) { x = entry_grad(w, x, j); });
     }
     __syncthreads();
     T* out = (T*)p.dlogits + r0 * p.vocab;
     const int all = n * p.vocab;
-    for (int i = threadIdx.x * V; i < all; i += 256 * V) {
+    for (int i = threadIdx.x * V; i < all; i += FEW_ROWS * V) {
         float f[V];
-        if (stride == p.vocab) {
+        if (QUADS || stride == p.vocab) {
 #pragma unroll
             for (int q = 0; q < V; q += 4) {
-                const float4 v = *(const float4*)(s_rows + i + q);
+                int at = i + q;
+                if (QUADS) {
+                    const int row = i + q < all ? row_in(i + q, p.vocab, by_vocab) : 0;
+                    at = i + q < all ? i + q + row * (stride - p.vocab) : 0;
+                }
+                const float4 v = *(const float4*)(s_rows + at);
                 f[q] = v.x, f[q + 1] = v.y, f[q + 2] = v.z, f[q + 3] = v.w;
             }
         } else {
@@ -600,12 +632,14 @@ const char* bad(const char* who, const LpArgs& a, int dtype, int mask_dtype) {
     return msg;
 }
 
-// threads that share a row: at most 4 loads of 16 bytes each where 16 or 64 do (0: a lane per row); the alternatives take whole
-// waves
-int threads_for(int64_t vocab, int dtype, bool top) {
-    if (vocab <= FEW) return 0;
+// Threads that share a row (0: a lane per row): 16 or 64 where that is at most 4 loads of 16 bytes each; the alternatives take
+// whole waves.  With rows for every wave of the GPU a wave takes up to 1024 vectors, loop and all: a block has four lists of
+// alternatives to make and join where a wave has one (10000 rows of 5001 in bf16 with 20 of them: 43 us, 75 with a block per
+// row; 5000 rows of 16000: 123 and 109)
+int threads_for(int64_t rows, int64_t vocab, int dtype, bool top) {
+    if (vocab <= (dtype == EC_F32 ? FEW_FP32 : FEW_16BIT)) return 0;
     const int64_t vecs = cdiv(vocab, dtype == EC_F32 ? 4 : 8);
-    return vecs <= 64 && !top ? 16 : vecs <= 256 ? 64 : 256;
+    return vecs <= 64 && !top ? 16 : vecs <= 256 || (rows >= 4096 && vecs <= 1024) ? 64 : 256;
 }
 // vectors a thread then takes at once: as few as hold the row (what is loaded past it is computed with all the same)
 int vectors_for(int64_t vocab, int dtype, int tpr) {
@@ -622,7 +656,7 @@ uint32_t by_vocab(int vocab) { return (uint32_t)((((uint64_t)1 << 32) + vocab - 
 
 // few rows: a row is split over as many blocks as fill the GPU, at least one batch of loads each
 int per_split(int64_t rows, int64_t vocab, int dtype) {
-    if (threads_for(vocab, dtype, true) != 256) return INT32_MAX;
+    if (threads_for(rows, vocab, dtype, true) != 256) return INT32_MAX;
     const int64_t batch = 256 * MOST_U * (dtype == EC_F32 ? 4 : 8), batches = cdiv(vocab, batch), want = cdiv(1024, rows);
     const int64_t splits = want < batches ? (want < MAX_SPLITS ? want : MAX_SPLITS) : (batches < MAX_SPLITS ? batches : MAX_SPLITS);
     const int64_t each = cdiv(batches, splits) * batch;
@@ -630,15 +664,16 @@ int per_split(int64_t rows, int64_t vocab, int dtype) {
 }
 int splits_for(int64_t rows, int64_t vocab, int dtype) { return (int)cdiv(vocab, per_split(rows, vocab, dtype)); }
 
-int few_lds(int vocab) { return (256 * (vocab | 1) + 8) * 4; }  // (the last vector of a tile may be a partial one)
+int few_lds(int vocab) { return (FEW_ROWS * few_stride(vocab) + 8) * 4; }  // (the last vector of a tile may be a partial one)
 
 template <typename T, int MASK>
 void go_fwd(const LpArgs& a, int dtype, hipStream_t st) {
-    const int tpr = threads_for(a.vocab, dtype, a.top_k > 0), u = tpr ? vectors_for(a.vocab, dtype, tpr) : 0;
+    const int tpr = threads_for(a.rows, a.vocab, dtype, a.top_k > 0), u = tpr ? vectors_for(a.vocab, dtype, tpr) : 0;
     const auto blocks = [&](int rows) { return dim3((unsigned)cdiv(a.rows, rows)); };
     const dim3 b(256);
     if (tpr == 0) {
-        hipLaunchKernelGGL((k_logp_few_fwd<T, MASK>), blocks(256), b, few_lds(a.vocab), st, a, by_vocab(a.vocab), is_packed(a));
+        const auto few = a.vocab % 4 ? k_logp_few_fwd<T, MASK, false> : k_logp_few_fwd<T, MASK, true>;
+        hipLaunchKernelGGL(few, blocks(FEW_ROWS), dim3(FEW_ROWS), few_lds(a.vocab), st, a, by_vocab(a.vocab), is_packed(a));
     } else if (tpr == 16) {
         if (u == 1) hipLaunchKernelGGL((k_logp_fwd<T, MASK, false, 16, 1, false>), blocks(16), b, 0, st, a);
         else if (u == 2) hipLaunchKernelGGL((k_logp_fwd<T, MASK, false, 16, 2, false>), blocks(16), b, 0, st, a);
@@ -660,11 +695,12 @@ void go_fwd(const LpArgs& a, int dtype, hipStream_t st) {
 
 template <typename T, int MASK>
 void go_bwd(const LpArgs& a, int dtype, hipStream_t st) {
-    const int tpr = threads_for(a.vocab, dtype, false), u = tpr ? vectors_for(a.vocab, dtype, tpr) : 0;
+    const int tpr = threads_for(a.rows, a.vocab, dtype, false), u = tpr ? vectors_for(a.vocab, dtype, tpr) : 0;
     const auto blocks = [&](int rows) { return dim3((unsigned)cdiv(a.rows, rows)); };
     const dim3 b(256);
+    const auto few = a.vocab % 4 ? k_logp_few_bwd<T, MASK, false> : k_logp_few_bwd<T, MASK, true>;
     if (tpr == 0)
-        hipLaunchKernelGGL((k_logp_few_bwd<T, MASK>), blocks(256), b, few_lds(a.vocab), st, a, by_vocab(a.vocab), is_packed(a));
+        hipLaunchKernelGGL(few, blocks(FEW_ROWS), dim3(FEW_ROWS), few_lds(a.vocab), st, a, by_vocab(a.vocab), is_packed(a));
     else if (tpr == 16 && u == 1)
         hipLaunchKernelGGL((k_logp_bwd<T, MASK, 16, 1, false>), blocks(16), b, 0, st, a);
     else if (tpr == 16 && u == 2)
@@ -736,7 +772,7 @@ extern "C" int ec_token_logprobs_bwd(const void* logits, int64_t inner, int64_t 
     if (!lse || !entropy || !dlogits) return ec::fail(EC_EINVAL, "ec_token_logprobs_bwd: null argument");
     a.lse = const_cast<float*>(lse), a.entropy_in = entropy, a.dlogp = dlogp, a.dentropy = dentropy, a.dlogits = dlogits;
     a.per_split = 256 * MOST_U * (dtype == EC_F32 ? 4 : 8);
-    a.splits = threads_for(vocab, dtype, false) == 256 ? (int)cdiv(vocab, a.per_split) : 1;
+    a.splits = threads_for(rows, vocab, dtype, false) == 256 ? (int)cdiv(vocab, a.per_split) : 1;
     if (rows * a.splits > INT32_MAX) return ec::fail(EC_EINVAL, "ec_token_logprobs_bwd: %lld rows", (long long)rows);
     const hipStream_t st = (hipStream_t)stream;
     EC_LP_TYPES(go_bwd)
