@@ -64,13 +64,21 @@ __device__ __forceinline__ float root_of(float v) {
     return small ? r * 2.3283064365386962890625e-10f : r;
 }
 
-// m, v -> m', v' and p -> p'; root: sqrt(v').  The quotient is a product with v_rcp's inverse (one unit in the last place):
+// m, v -> m', v' and p -> p'; root: sqrt(v').  EXACT, where m' and the root are held in 8 bits afterwards: each operation of
+// the formulas rounded once, so that a value next to a border of its 8 bits falls where the plain formulas in fp32 put it.
+// The quotient is a product with v_rcp's inverse (one unit in the last place):
 // its error is that of the step, far below a rounding of p
+template <bool EXACT>
 __device__ __forceinline__ void adam(const Hyper& h, float coef, float g, float& p, float& m, float& v, float& root) {
     g *= coef;
-    m = __builtin_fmaf(g - m, h.omb1, m);
-    v = __builtin_fmaf(h.omb2 * g, g, v * h.b2);
-    root = root_of(v);
+    if (EXACT) {  // (built without contraction)
+        m = m + (g - m) * h.omb1;
+        v = v * h.b2 + h.omb2 * g * g;
+    } else {
+        m = __builtin_fmaf(g - m, h.omb1, m);
+        v = __builtin_fmaf(h.omb2 * g, g, v * h.b2);
+    }
+    root = EXACT ? sqrtf(v) : root_of(v);
     const float inv = __builtin_amdgcn_rcpf(__builtin_fmaf(root, h.inv_bc2, h.eps));
     p = __builtin_fmaf(-h.step_size * m, inv, p * h.keep);
 }
@@ -99,7 +107,7 @@ __device__ __forceinline__ void adamw32(const Tensor& t, int64_t e0, Hyper& h) {
 #pragma unroll
     for (int i = 0; i < R; i++)
 #pragma unroll
-        for (int j = 0; j < E; j++) adam(h, coef, g[i][j], p[i][j], m[i][j], v[i][j], root);
+        for (int j = 0; j < E; j++) adam<false>(h, coef, g[i][j], p[i][j], m[i][j], v[i][j], root);
 #pragma unroll
     for (int i = 0; i < R; i++) {
         const int64_t e = e0 + i * (CHUNK / R), n = FULL ? E : t.n - e;
@@ -159,7 +167,7 @@ __device__ __forceinline__ Bytes<N> pack8(const float (&f)[N]) {
 __device__ __forceinline__ float scale_of(float most, float& inv) {
     float s = most * (1.0f / QMAX);
     s = s < 1.17549435e-38f ? 0.0f : s;
-    inv = s != 0.0f ? __builtin_amdgcn_rcpf(s) : 0.0f;
+    inv = s != 0.0f ? 1.0f / s : 0.0f;
     return s;
 }
 
@@ -190,7 +198,7 @@ __device__ __forceinline__ void adamw8(const Tensor& t, int64_t b, Hyper& h) {
         for (int j = 0; j < E; j++) {
             float root;
             v[i][j] *= v[i][j];
-            adam(h, coef, g[i][j], p[i][j], m[i][j], v[i][j], root);
+            adam<true>(h, coef, g[i][j], p[i][j], m[i][j], v[i][j], root);
             v[i][j] = root;
             most_m = fmaxf(most_m, fabsf(m[i][j]));
             most_v = fmaxf(most_v, root);
