@@ -240,7 +240,10 @@ __device__ __forceinline__ void write_row(const LpArgs& p, int64_t r, const Stat
         p.lse[2 * r] = none ? -INF : s.m;
         p.lse[2 * r + 1] = ln;
     }
-    if (p.entropy) p.entropy[r] = none ? 0.0f : ln - s.s2 * LN2 / s.s1;
+    if (p.entropy) {
+        const float h = ln - s.s2 * LN2 / s.s1;
+        p.entropy[r] = none || h < 0.0f ? 0.0f : h;  // (a rounding below 0; a NaN stays one)
+    }
     if (p.logp) p.logp[r] = logp;
 }
 __device__ __forceinline__ void write_top(const LpArgs& p, int64_t r, int i, const Stat& s, float ln, uint64_t key) {

@@ -121,6 +121,7 @@ class _TokenLogprobsFn(th.autograd.Function):
     @staticmethod
     @th.autograd.function.once_differentiable
     def backward(ctx, dlogp, dentropy, *_):
+        refuse_capture("token_logprobs", "token_logprobs_fwd and token_logprobs_bwd")
         logits, tokens, avail, lse, entropy = ctx.saved_tensors
         if dlogp is None and dentropy is None:
             return None, None, None, None

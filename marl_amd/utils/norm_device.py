@@ -143,6 +143,7 @@ class _LayerNormFn(th.autograd.Function):
     @staticmethod
     @th.autograd.function.once_differentiable
     def backward(ctx, dy):
+        refuse_capture("layer_norm", "layer_norm_fwd and layer_norm_bwd")
         x, weight, mean, rstd = ctx.saved_tensors
         need = ctx.needs_input_grad
         dx, dw, db = layer_norm_bwd(dy, x, mean, rstd, weight, need[0], need[1], need[2], ctx.param_dtype)

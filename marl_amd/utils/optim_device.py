@@ -188,10 +188,6 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, exp_avg_scale=None, exp_avg_s
     numel = list(map(_NUMEL, params))
     kinds = list(map(_DTYPE, params))
     P = _pointers(who, "params", params, at, numel, _FLOATS)
-    if len(set(P)) != n:
-        live = [a for a, k in zip(P, numel) if k]
-        if len(set(live)) != len(live):
-            raise ValueError("adamw_step: the same parameter twice")
     G = _pointers(who, "grads", grads, at, numel, kinds)
     bits = 8 if exp_avg_scale is not None else 32
     st = {STATE8} if bits == 8 else {th.float32}
@@ -206,6 +202,9 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, exp_avg_scale=None, exp_avg_s
         VS = _pointers(who, "exp_avg_sq_scale", exp_avg_sq_scale, at, blocks, {th.float32})
     elif exp_avg_sq_scale is not None:
         raise ValueError("adamw_step: exp_avg_sq_scale without exp_avg_scale")
+    for name, a in (("parameter", P), ("exp_avg", M), ("exp_avg_sq", V), ("exp_avg_scale", MS), ("exp_avg_sq_scale", VS)):
+        if a is not None and len(set(a)) != n and len({x for x, k in zip(a, numel) if k}) != sum(map(bool, numel)):
+            raise ValueError("adamw_step: the same %s twice" % name)
     for name, t in (("step", step), ("lr", lr), ("coef", coef)):
         if isinstance(t, th.Tensor) and (t.device != dev or t.dtype != th.float32 or t.numel() != 1):
             raise ValueError("adamw_step: %s on the device is one float32 value on %s" % (name, dev))
@@ -233,7 +232,8 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, exp_avg_scale=None, exp_avg_s
     on_dev, lr_dev = dyn is not None, isinstance(lr, th.Tensor)
     launch("ec_adamw_step", dev, n, *map(_address, (P, G, M, V, MS, VS, counts, codes)), bits, ptr(coef), 0.0 if on_dev else step,
            ptr(step if on_dev else None), ptr(dyn), 0.0 if lr_dev else lr, ptr(lr if lr_dev else None), b1, b2, eps, weight_decay)
-    th.autograd.graph.increment_version(params)  # (written through raw pointers: autograd has to know)
+    # (written through raw pointers: autograd has to know; what was made in inference mode counts no versions)
+    th.autograd.graph.increment_version([p for p in params if not p.is_inference()] if params[0].is_inference() else params)
     return norm
 
 
@@ -337,22 +337,30 @@ class AdamW(th.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """torch's load casts states to their parameter's type: here they keep their own, and a capturable group gets its one
-        step count back"""
+        step count back.  Takes torch.optim.AdamW's state_dict too (states in 32 bits)."""
+        for saved in state_dict["param_groups"]:
+            bits = saved.get("state_bits", self.defaults["state_bits"])
+            want = {"step", "exp_avg", "exp_avg_sq"} | ({"exp_avg_scale", "exp_avg_sq_scale"} if bits == 8 else set())
+            for i in saved["params"]:
+                st = state_dict["state"].get(i)
+                if st is not None and (set(st) != want or (bits == 8) != (st["exp_avg"].dtype == STATE8)):
+                    raise ValueError("AdamW.load_state_dict: parameter %s has %s (%s) for states of %d bits"
+                                     % (i, sorted(st), st["exp_avg"].dtype if "exp_avg" in st else None, bits))
         super().load_state_dict(state_dict)
         for saved, group in zip(state_dict["param_groups"], self.param_groups):
+            for k, v in self.defaults.items():
+                group.setdefault(k, v)
+            group["capturable"] = bool(group["capturable"])
             count = None
             for i, p in zip(saved["params"], group["params"]):
                 if i not in state_dict["state"]:
                     continue
-                st = self.state[p]
+                st = self.state[p] = {}
                 for k, v in state_dict["state"][i].items():
-                    if k == "step":
-                        if group["capturable"]:
-                            if count is None:
-                                count = th.as_tensor(float(v), dtype=th.float32).to(p.device)
-                            v = count
-                        else:
-                            v = int(v)
+                    if k != "step":
+                        st[k] = v.detach().to(p.device, STATE8 if v.dtype == STATE8 else th.float32, copy=True).contiguous()
+                    elif group["capturable"]:  # one count for the group
+                        count = count if count is not None else th.tensor(float(v), dtype=th.float32, device=p.device)
+                        st[k] = count
                     else:
-                        v = v.detach().to(p.device, copy=True)
-                    st[k] = v
+                        st[k] = int(v)

@@ -269,6 +269,34 @@ def test_state_dict_round_trip(bits, capturable, tmp_path):
     assert clone.max_norm == 1.0
 
 
+def test_loads_the_state_of_torch_adamw():
+    """a checkpoint of torch.optim.AdamW, and the next step equals torch's; 32-bit states are refused by an 8-bit optimiser"""
+    from marl_amd.utils import optim_device
+    a, b = _net(), _net()
+    ob = th.optim.AdamW(b.parameters(), lr=1e-3)
+    g = th.Generator(device="cuda").manual_seed(5)
+
+    def grads():
+        for pa, pb in zip(a.parameters(), b.parameters()):
+            pa.grad = th.randn(pa.shape, device="cuda", generator=g)
+            pb.grad = pa.grad.clone()
+    grads()
+    ob.step()
+    a.load_state_dict(b.state_dict())
+    oa = optim_device.AdamW(a.parameters(), lr=5.0)
+    oa.load_state_dict(ob.state_dict())
+    grads()
+    oa.step()
+    ob.step()
+    for pa, pb in zip(a.parameters(), b.parameters()):
+        # the step (at most 10 lr) to 40 u on either side, and 4 u of the parameter
+        assert bool(((pa - pb).abs() <= 80 * U * 1e-2 + 8 * U * pb.abs()).all())
+        assert oa.state[pa]["step"] == 2 and th.equal(oa.state[pa]["exp_avg_sq"] > 0, ob.state[pb]["exp_avg_sq"] > 0)
+    q = optim_device.AdamW(a.parameters(), state_bits=8)
+    with pytest.raises(ValueError, match="8 bits"):
+        q.load_state_dict(ob.state_dict())
+
+
 def test_200_steps_stay_finite():
     """a least-squares problem of 4096 unknowns with either kind of state: everything stays finite, the types and the count hold"""
     from marl_amd.utils import optim_device
@@ -333,6 +361,7 @@ def test_refusals():
     bad = [lambda: S(P, G[:1], M, V, step=1, lr=1e-3), lambda: S(P, [g.bfloat16() for g in G], M, V, step=1, lr=1e-3),
            lambda: S(P, G, [m.half() for m in M], V, step=1, lr=1e-3), lambda: S(P, [g[:5] for g in G], M, V, step=1, lr=1e-3),
            lambda: S([P[0], P[0]], [G[0], G[0]], [M[0], M[0]], [V[0], V[0]], step=1, lr=1e-3),
+           lambda: S(P, G, [M[1][:10], M[1]], V, step=1, lr=1e-3), lambda: S(P, G, M, [V[1][:10], V[1]], step=1, lr=1e-3),
            lambda: S([p.double() for p in P], G, M, V, step=1, lr=1e-3), lambda: S(P, G, M, V, step=0, lr=1e-3),
            lambda: S(P, G, M, V, step=1, lr=-1e-3), lambda: S(P, G, M, V, step=1, lr=1e-3, betas=(1.0, 0.9)),
            lambda: S(P, G, M, V, step=1, lr=1e-3, eps=-1.0), lambda: S(P, G, M, V, step=1, lr=1e-3, weight_decay=-1.0),

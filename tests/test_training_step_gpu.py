@@ -74,6 +74,38 @@ def test_ppo_steps_follow_float64(width, n_out):
             assert float((p.detach().cpu().double() - q).abs().mean()) <= (step + 1) * 2e-5
 
 
+def test_on_another_stream_than_the_default():
+    """inputs made, used and read on a side stream behind a long kernel there, from a thread of its own: nothing of a call runs
+    on the default stream"""
+    import threading
+
+    from marl_amd.utils import logprob_device, norm_device, optim_device
+    out = {}
+
+    def work(key, stream):
+        with th.cuda.stream(stream):
+            g = th.Generator(device="cuda").manual_seed(3)
+            a = th.randn(4096, 4096, device="cuda", generator=g)
+            x = th.zeros(500, 700, device="cuda")
+            busy = a
+            for _ in range(4):
+                busy = busy @ a * 1e-3
+            x.copy_(th.randn(500, 700, device="cuda", generator=g))        # (behind the products)
+            w = th.ones(700, device="cuda").requires_grad_(True)
+            tok = th.arange(500, device="cuda")
+            f = logprob_device.token_logprobs(norm_device.layer_norm(x, w), tok, top_k=3)
+            f.logp.sum().backward()
+            opt = optim_device.AdamW([w], lr=0.1, max_norm=1.0)
+            opt.step()
+            out[key] = [t.detach().cpu() for t in (f.logp, f.entropy, f.top_logp, f.top_index, w.grad, w, opt.last_norm)]
+    threads = [threading.Thread(target=work, args=(k, th.cuda.Stream())) for k in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    work("default", th.cuda.default_stream())
+    for k in range(2):
+        assert all(th.equal(p, q) for p, q in zip(out[k], out["default"]))
+
+
 def test_an_update_step_in_a_graph():
     """the passes by hand, with clip and AdamW, recorded once and replayed on new batches: the bits of the eager steps"""
     from marl_amd.utils import logprob_device, norm_device, optim_device
