@@ -22,7 +22,7 @@ namespace {
 using namespace ecs;
 
 constexpr int MAX_TENSORS = 48;          // (the argument block stays under the 4 KB a launch can carry)
-constexpr int CHUNK = 2048;              // elements a block
+constexpr int CHUNK32 = 1024, CHUNK8 = 2048;  // elements a block
 constexpr int QBLOCK = 256;              // elements that share a scale
 constexpr float QMAX = 448.0f, QMIN = 0.001953125f;
 
@@ -83,48 +83,39 @@ __device__ __forceinline__ void adam(const Hyper& h, float coef, float g, float&
     p = __builtin_fmaf(-h.step_size * m, inv, p * h.keep);
 }
 
-// A block takes CHUNK consecutive elements of one tensor, eight a thread, all loads ahead of all stores (a loop with less in
-// flight, or with stores between its loads, runs at 5.2 TB/s against 5.9).  16-bit types: eight in a row; fp32: two runs of
-// four, half a chunk (or, with 8-bit states, half a scale's block) apart.
-template <typename T>
-struct Take {
-    static constexpr int EACH = sizeof(T) == 4 ? 4 : 8, RUNS = 8 / EACH;
-};
-
+// 32 bits: a block takes CHUNK32 consecutive elements of one tensor, four a thread, all loads ahead of all stores (151 M fp32
+// parameters: 737 us, with eight a thread 757; in a loop, with stores between the loads, 816.  bf16: 590 and 619)
 template <typename T, bool NT, bool FULL>
-__device__ __forceinline__ void adamw32(const Tensor& t, int64_t e0, Hyper& h) {
-    constexpr int E = Take<T>::EACH, R = Take<T>::RUNS;
-    float p[R][E], g[R][E], m[R][E], v[R][E], root;
-#pragma unroll
-    for (int i = 0; i < R; i++) {
-        const int64_t e = e0 + i * (CHUNK / R), n = FULL ? E : t.n - e;
-        load_upto<T, E, NT>((const T*)t.g + e, n, 0.0f, g[i]);
-        load_upto<float, E, NT>((const float*)t.m + e, n, 0.0f, m[i]);
-        load_upto<float, E, NT>((const float*)t.v + e, n, 0.0f, v[i]);
-        load_upto<T, E, NT>((const T*)t.p + e, n, 0.0f, p[i]);
-    }
+__device__ __forceinline__ void adamw32(const Tensor& t, int64_t e, Hyper& h) {
+    const int64_t n = FULL ? 4 : t.n - e;
+    float p[4], g[4], m[4], v[4], root;
+    load_upto<T, 4, NT>((const T*)t.g + e, n, 0.0f, g);
+    load_upto<float, 4, NT>((const float*)t.m + e, n, 0.0f, m);
+    load_upto<float, 4, NT>((const float*)t.v + e, n, 0.0f, v);
+    load_upto<T, 4, NT>((const T*)t.p + e, n, 0.0f, p);
     const float coef = read_hyper(h);
 #pragma unroll
-    for (int i = 0; i < R; i++)
-#pragma unroll
-        for (int j = 0; j < E; j++) adam<false>(h, coef, g[i][j], p[i][j], m[i][j], v[i][j], root);
-#pragma unroll
-    for (int i = 0; i < R; i++) {
-        const int64_t e = e0 + i * (CHUNK / R), n = FULL ? E : t.n - e;
-        store_upto<T, E, NT>((T*)t.p + e, n, p[i]);
-        store_upto<float, E, NT>((float*)t.m + e, n, m[i]);
-        store_upto<float, E, NT>((float*)t.v + e, n, v[i]);
-    }
+    for (int j = 0; j < 4; j++) adam<false>(h, coef, g[j], p[j], m[j], v[j], root);
+    store_upto<T, 4, NT>((T*)t.p + e, n, p);
+    store_upto<float, 4, NT>((float*)t.m + e, n, m);
+    store_upto<float, 4, NT>((float*)t.v + e, n, v);
 }
 
 template <typename T, bool NT>
 __global__ void __launch_bounds__(256) k_adamw32(Group a, Hyper h) {
     const int k = tensor_of(a, blockIdx.x);
     const Tensor t = a.t[k];
-    const int64_t b0 = (int64_t)(blockIdx.x - a.first[k]) * CHUNK, e0 = b0 + threadIdx.x * Take<T>::EACH;
-    if (b0 + CHUNK <= t.n) adamw32<T, NT, true>(t, e0, h);
-    else adamw32<T, NT, false>(t, e0, h);
+    const int64_t b0 = (int64_t)(blockIdx.x - a.first[k]) * CHUNK32, e = b0 + threadIdx.x * 4;
+    if (b0 + CHUNK32 <= t.n) adamw32<T, NT, true>(t, e, h);
+    else adamw32<T, NT, false>(t, e, h);
 }
+
+// 8 bits: a block takes CHUNK8 elements, eight a thread: 16-bit types eight in a row, fp32 two runs of four, half a scale's
+// block apart
+template <typename T>
+struct Take {
+    static constexpr int EACH = sizeof(T) == 4 ? 4 : 8, RUNS = 8 / EACH;
+};
 
 // N e4m3 values of N bytes at any address (N = 4, 8), the first n of them; the others 0 / untouched
 template <int N>
@@ -226,8 +217,8 @@ template <typename T, bool NT>
 __global__ void __launch_bounds__(256) k_adamw8(Group a, Hyper h) {
     const int k = tensor_of(a, blockIdx.x);
     const Tensor t = a.t[k];
-    const int64_t c = blockIdx.x - a.first[k], b = c * (CHUNK / QBLOCK) + threadIdx.x / 32;
-    if ((c + 1) * CHUNK <= t.n) adamw8<T, NT, true>(t, b, h);
+    const int64_t c = blockIdx.x - a.first[k], b = c * (CHUNK8 / QBLOCK) + threadIdx.x / 32;
+    if ((c + 1) * CHUNK8 <= t.n) adamw8<T, NT, true>(t, b, h);
     else adamw8<T, NT, false>(t, b, h);
 }
 
@@ -331,7 +322,7 @@ const char* bad_tensors(const char* who, int32_t count, const void* const* grads
         }
         total += numel[i];
     }
-    if (cdiv(total, CHUNK) + count > INT32_MAX) {
+    if (cdiv(total, CHUNK32) + count > INT32_MAX) {
         snprintf(msg, sizeof msg, "%s: %lld elements", who, (long long)total);
         return msg;
     }
@@ -383,7 +374,7 @@ extern "C" int ec_grad_clip_coef(int32_t count, const void* const* grads, const 
         return ec::fail(EC_EINVAL, "ec_grad_clip_coef: workspace of %lld bytes (%lld are needed, at a multiple of 8)",
                         (long long)work_bytes, (long long)need);
     const hipStream_t st = (hipStream_t)stream;
-    const int64_t chunk = total ? norm_chunk(total) : CHUNK;
+    const int64_t chunk = total ? norm_chunk(total) : 1;
     double* partial = (double*)work;
     each_group(count, numel, dtypes, chunk,
                [&](int i) {
@@ -433,7 +424,7 @@ extern "C" int ec_adamw_step(int32_t count, void* const* params, const void* con
         h.keep = (float)(1.0 - lr * weight_decay);
     }
     const bool far = total >= NT_ELEMENTS;
-    each_group(count, numel, dtypes, CHUNK,
+    each_group(count, numel, dtypes, q ? CHUNK8 : CHUNK32,
                [&](int i) {
                    return Tensor{params[i], exp_avg[i], exp_avg_sq[i], grads[i], q ? exp_avg_scale[i] : nullptr,
                                  q ? exp_avg_sq_scale[i] : nullptr, numel[i]};
