@@ -177,14 +177,22 @@ struct TopList {
     }
 };
 
+// (no division where there is nothing to divide by: in 64 bits it costs as much as ten entries)
+__device__ __forceinline__ int64_t row_at(int64_t r, int64_t inner, int64_t s_outer, int64_t s_inner) {
+    if (inner == 1) return r * s_outer;
+    int64_t q;
+    if (((r | inner) >> 32) == 0) q = (uint32_t)r / (uint32_t)inner;
+    else q = r / inner;
+    return q * s_outer + (r - q * inner) * s_inner;
+}
 template <typename T>
 __device__ __forceinline__ const T* row_of(const LpArgs& p, int64_t r) {
-    return (const T*)p.logits + (r / p.inner) * p.s_outer + (r % p.inner) * p.s_inner;
+    return (const T*)p.logits + row_at(r, p.inner, p.s_outer, p.s_inner);
 }
 // MASK 0: none, 1: bytes, 2: int32
 template <int MASK>
 __device__ __forceinline__ const char* mask_of(const LpArgs& p, int64_t r) {
-    return (const char*)p.avail + ((r / p.inner) * p.a_outer + (r % p.inner) * p.a_inner) * (MASK == 1 ? 1 : 4);
+    return (const char*)p.avail + row_at(r, p.inner, p.a_outer, p.a_inner) * (MASK == 1 ? 1 : 4);
 }
 
 // U vectors of N logits from l + c on, `step` apart, those from column c1 on and the excluded as -inf.  FULL: all of them lie
@@ -259,14 +267,20 @@ __device__ __forceinline__ void write_top(const LpArgs& p, int64_t r, int i, con
     p.top_index[r * p.top_k + i] = at;
 }
 
-// what a row's statistics say, by one lane
+// a row's token and its logit: two loads, one behind the other, that a row's lead makes before all others
+struct Taken {
+    int64_t token;
+    float logit;
+};
 template <typename T, int MASK>
-__device__ __forceinline__ void finish_row(const LpArgs& p, int64_t r, bool lead, const Stat& s, float ln) {
+__device__ __forceinline__ Taken taken_of(const LpArgs& p, int64_t r, bool lead) {
+    Taken o{-1, 0.0f};
     if (lead) {
-        const int64_t tok = p.tokens[r];
-        const float l = tok >= 0 && tok < p.vocab ? logit_at<T, MASK>(row_of<T>(p, r), MASK ? mask_of<MASK>(p, r) : nullptr, tok) : 0.0f;
-        write_row(p, r, s, ln, logp_of(p, tok, l, s, ln));
+        o.token = p.tokens[r];
+        if (o.token >= 0 && o.token < p.vocab)
+            o.logit = logit_at<T, MASK>(row_of<T>(p, r), MASK ? mask_of<MASK>(p, r) : nullptr, o.token);
     }
+    return o;
 }
 
 // U vectors a thread from column b on into the row's statistics and alternatives (the same rounds for every thread: the lists
@@ -318,6 +332,7 @@ __global__ void __launch_bounds__(256) k_logp_fwd(LpArgs p) {
     const int64_t c0 = (int64_t)split * p.per_split;
     const int64_t c1 = c0 + p.per_split < p.vocab ? c0 + p.per_split : p.vocab;
     Stat s{-FLT_MAX, 0.0f, 0.0f};
+    const Taken taken = taken_of<T, MASK>(p, r, t == 0 && on && (TPR < 256 || p.splits == 1));
     TopList top;
     top.clear(p.top_k);
     int64_t b = c0;
@@ -326,7 +341,7 @@ __global__ void __launch_bounds__(256) k_logp_fwd(LpArgs p) {
     s = lanes_join<W>(s);
     if (TPR < 256) {
         const float ln = log_s1(s);
-        if (on) finish_row<T, MASK>(p, r, t == 0, s, ln);
+        if (on && t == 0) write_row(p, r, s, ln, logp_of(p, taken.token, taken.logit, s, ln));
         if (TOP && on && t < p.top_k) write_top(p, r, t, s, ln, top.mine);
         return;
     }
@@ -338,8 +353,10 @@ __global__ void __launch_bounds__(256) k_logp_fwd(LpArgs p) {
     for (int w = 1; w < 4; w++) s = join(s, s_stat[w]);
     const float ln = log_s1(s);
     char* to = p.splits > 1 ? p.work + (r * p.splits + split) * part_bytes(p.top_k) : nullptr;
-    if (p.splits == 1) finish_row<T, MASK>(p, r, threadIdx.x == 0, s, ln);
-    else if (threadIdx.x == 0) ((float*)to)[0] = s.m, ((float*)to)[1] = s.s1, ((float*)to)[2] = s.s2;
+    if (threadIdx.x == 0) {
+        if (p.splits == 1) write_row(p, r, s, ln, logp_of(p, taken.token, taken.logit, s, ln));
+        else ((float*)to)[0] = s.m, ((float*)to)[1] = s.s1, ((float*)to)[2] = s.s2;
+    }
     if (TOP) {
         // a key's place among the four waves' lists: its place in its own and the number of larger ones in the others (the
         // places behind the last key, each wave its share of them, take "none")
@@ -372,6 +389,7 @@ __global__ void __launch_bounds__(256) k_logp_join(LpArgs p) {
     const char* from = p.work + r * p.splits * part_bytes(k);
     // (every wave joins the statistics for itself; what is loaded is loaded first: this kernel is a chain of waits)
     Stat s{-FLT_MAX, 0.0f, 0.0f};
+    const Taken taken = taken_of<T, MASK>(p, r, threadIdx.x == 255);
     if (lane < p.splits) {
         const float* f = (const float*)(from + lane * part_bytes(k));
         s = Stat{f[0], f[1], f[2]};
@@ -384,7 +402,7 @@ __global__ void __launch_bounds__(256) k_logp_join(LpArgs p) {
     for (int i = threadIdx.x; i < all; i += 256) s_keys[i] = ((const uint64_t*)(from + (i / k) * part_bytes(k) + 16))[i % k];
     s = lanes_join<64>(s);
     const float ln = log_s1(s);
-    finish_row<T, MASK>(p, r, threadIdx.x == 255, s, ln);
+    if (threadIdx.x == 255) write_row(p, r, s, ln, logp_of(p, taken.token, taken.logit, s, ln));
     if (k == 0) return;
     __syncthreads();
     // nothing below the k-th of one split can be among the best, nor below the k-th largest of the splits' largest (TopList)

@@ -14,7 +14,6 @@ template <typename T, int N>
 struct vec_of {
     typedef T raw __attribute__((ext_vector_type(N)));
     typedef raw type __attribute__((aligned(sizeof(T))));
-    typedef float fraw __attribute__((ext_vector_type(N)));
 };
 
 template <typename T, int N>
@@ -103,11 +102,6 @@ __device__ __forceinline__ raw_t<T, N> narrow(const float (&f)[N]) {
     for (int j = 0; j < N; j++) v[j] = (T)f[j];
     return v;
 }
-template <typename T, int N, bool NT = false>
-__device__ __forceinline__ void store_n(T* p, const float (&f)[N]) {
-    store_raw<NT, T, N>(p, narrow<T, N>(f));
-}
-
 // the same for the first n of N, which may be several vectors of 16 bytes
 template <typename T, int N, bool NT = false>
 __device__ __forceinline__ void load_upto(const T* p, int64_t n, float fill, float (&f)[N]) {
