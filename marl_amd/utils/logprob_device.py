@@ -78,7 +78,8 @@ def token_logprobs_fwd(logits, tokens, avail=None, top_k=0):
         raise ValueError("token_logprobs_fwd: top_k %d (0 .. %d)" % (top_k, MAX_TOP))
     lead = tuple(tokens.shape)
     rows, vocab, code = head[-2], head[-1], head[-3]
-    logp, entropy = th.empty((2,) + lead, dtype=th.float32, device=dev).unbind(0)
+    # (memory of its own for each: views of one tensor could not be changed in place under autograd)
+    logp, entropy = (th.empty(lead, dtype=th.float32, device=dev) for _ in range(2))
     lse = th.empty(lead + (2,), dtype=th.float32, device=dev)
     top_logp = th.empty(lead + (top_k,), dtype=th.float32, device=dev) if top_k else None
     top_index = th.empty(lead + (top_k,), dtype=th.int64, device=dev) if top_k else None

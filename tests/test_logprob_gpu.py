@@ -232,6 +232,23 @@ def test_autograd_and_differences():
     assert not logprob_device.token_logprobs(l, t).logp.requires_grad
 
 
+def test_outputs_changed_in_place():
+    from marl_amd.utils.logprob_device import token_logprobs
+    l, t, _, g1, g2 = _inputs(40, 9, th.float32, None)
+    grads = []
+    for in_place in (False, True):
+        x = l.clone().requires_grad_()
+        f = token_logprobs(x, t)
+        (f.logp.mul_(g1) if in_place else f.logp * g1).sum().backward()
+        grads.append(x.grad)
+    assert th.equal(*grads)
+    with th.no_grad():
+        f = token_logprobs(l, t)
+    w = g1.clone().requires_grad_()
+    f.logp.mul_(w).add_(f.entropy.mul_(g2)).sum().backward()   # (no gradient of logits: plain tensors)
+    assert w.grad is not None
+
+
 def test_matches_the_learners_own_evaluation():
     """PPOAgent.evaluate_actions' formulas (masked_fill, softmax, Categorical) on the env's int32 masks"""
     from torch.distributions import Categorical

@@ -168,6 +168,22 @@ def test_autograd_and_differences():
     assert ws.grad is not None and not norm_device.layer_norm(x, w, b).requires_grad
 
 
+def test_outputs_changed_in_place():
+    from marl_amd.utils.norm_device import layer_norm, layer_norm_fwd
+    x, w, b, dy = _inputs(21, 64, th.float32, th.float32)
+    grads = []
+    for in_place in (False, True):
+        a = x.clone().requires_grad_()
+        y = layer_norm(a, w, b)
+        (y.relu_() if in_place else y.relu()).backward(dy)
+        grads.append(a.grad)
+    assert th.equal(*grads)
+    _, mean, rstd = layer_norm_fwd(x, w, b)
+    s = rstd.clone().requires_grad_()
+    mean.mul_(s).sum().backward()
+    assert s.grad is not None
+
+
 def test_refusals():
     from marl_amd.utils import norm_device
     x, w, b, dy = _inputs(4, 32, th.bfloat16, th.float32)
