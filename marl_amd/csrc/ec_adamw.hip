@@ -103,9 +103,10 @@ __device__ __forceinline__ void adamw32(const Tensor& t, int64_t e, Hyper& h) {
 
 template <typename T, bool NT>
 __global__ void __launch_bounds__(256) k_adamw32(Group a, Hyper h) {
-    const int k = tensor_of(a, blockIdx.x);
+    const uint32_t block = block_index();  // (those behind the last tensor's end do nothing)
+    const int k = tensor_of(a, block);
     const Tensor t = a.t[k];
-    const int64_t b0 = (int64_t)(blockIdx.x - a.first[k]) * CHUNK32, e = b0 + threadIdx.x * 4;
+    const int64_t b0 = (int64_t)(block - a.first[k]) * CHUNK32, e = b0 + threadIdx.x * 4;
     if (b0 + CHUNK32 <= t.n) adamw32<T, NT, true>(t, e, h);
     else adamw32<T, NT, false>(t, e, h);
 }
@@ -215,9 +216,10 @@ __device__ __forceinline__ void adamw8(const Tensor& t, int64_t b, Hyper& h) {
 
 template <typename T, bool NT>
 __global__ void __launch_bounds__(256) k_adamw8(Group a, Hyper h) {
-    const int k = tensor_of(a, blockIdx.x);
+    const uint32_t block = block_index();
+    const int k = tensor_of(a, block);
     const Tensor t = a.t[k];
-    const int64_t c = blockIdx.x - a.first[k], b = c * (CHUNK8 / QBLOCK) + threadIdx.x / 32;
+    const int64_t c = block - a.first[k], b = c * (CHUNK8 / QBLOCK) + threadIdx.x / 32;
     if ((c + 1) * CHUNK8 <= t.n) adamw8<T, NT, true>(t, b, h);
     else adamw8<T, NT, false>(t, b, h);
 }
@@ -296,7 +298,7 @@ constexpr int64_t NT_ELEMENTS = 8 << 20;
 
 template <typename T>
 void go_step(const Group& a, const Hyper& h, uint32_t blocks, bool q, bool far, hipStream_t st) {
-    const dim3 g(blocks), b(256);
+    const dim3 g = grid_of(blocks), b(256);
     if (q) {
         if (far) hipLaunchKernelGGL((k_adamw8<T, true>), g, b, 0, st, a, h);
         else hipLaunchKernelGGL((k_adamw8<T, false>), g, b, 0, st, a, h);

@@ -323,10 +323,12 @@ __global__ void __launch_bounds__(256) k_logp_fwd(LpArgs p) {
     __shared__ uint64_t s_pool[TOP ? 4 : 1][TOP ? POOL : 1];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, t = threadIdx.x % TPR;
     // (every thread makes every round: a group of rows past the last reads the last and writes nothing)
-    const int64_t r0 = TPR == 256 ? blockIdx.x / p.splits : (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+    const uint32_t block = block_index();
+    const int64_t r0 = TPR == 256 ? block / (uint32_t)p.splits : (int64_t)block * (256 / TPR) + threadIdx.x / TPR;
     const bool on = r0 < p.rows;
+    if (TPR == 256 && !on) return;
     const int64_t r = on ? r0 : p.rows - 1;
-    const int split = TPR == 256 ? (int)(blockIdx.x % p.splits) : 0;
+    const int split = TPR == 256 ? (int)(block % (uint32_t)p.splits) : 0;
     const T* l = row_of<T>(p, r);
     const char* av = MASK ? mask_of<MASK>(p, r) : nullptr;
     const int64_t c0 = (int64_t)split * p.per_split;
@@ -479,9 +481,10 @@ __device__ __forceinline__ void grad_batch(const RowGrad& w, const T* l, const c
 template <typename T, int MASK, int TPR, int U, bool NT>
 __global__ void __launch_bounds__(256) k_logp_bwd(LpArgs p) {
     constexpr int V = 16 / sizeof(T);
-    const int64_t r = TPR == 256 ? blockIdx.x / p.splits : (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+    const uint32_t block = block_index();
+    const int64_t r = TPR == 256 ? block / (uint32_t)p.splits : (int64_t)block * (256 / TPR) + threadIdx.x / TPR;
     if (r >= p.rows) return;
-    const int64_t c0 = TPR == 256 ? (int64_t)(blockIdx.x % p.splits) * p.per_split : 0;
+    const int64_t c0 = TPR == 256 ? (int64_t)(block % (uint32_t)p.splits) * p.per_split : 0;
     const int64_t c1 = TPR == 256 && c0 + p.per_split < p.vocab ? c0 + p.per_split : p.vocab;
     const T* l = row_of<T>(p, r);
     const char* av = MASK ? mask_of<MASK>(p, r) : nullptr;
@@ -568,7 +571,8 @@ __device__ __forceinline__ void stage_rows(const LpArgs& p, int64_t r0, int n, i
 template <typename T, int MASK, bool QUADS, bool NT>
 __global__ void __launch_bounds__(FEW_ROWS) k_logp_few_fwd(LpArgs p, uint32_t by_vocab, bool packed) {
     extern __shared__ float4 s_few[];
-    const int64_t r0 = (int64_t)blockIdx.x * FEW_ROWS, r = r0 + threadIdx.x;
+    const int64_t r0 = (int64_t)block_index() * FEW_ROWS, r = r0 + threadIdx.x;
+    if (r0 >= p.rows) return;
     const int n = (int)(p.rows - r0 < FEW_ROWS ? p.rows - r0 : FEW_ROWS), stride = few_stride(p.vocab);
     stage_rows<T, MASK, QUADS, NT>(p, r0, n, stride, by_vocab, packed, (float*)s_few);
     __syncthreads();
@@ -602,7 +606,8 @@ __global__ void __launch_bounds__(FEW_ROWS) k_logp_few_bwd(LpArgs p, uint32_t by
     extern __shared__ float4 s_few[];
     constexpr int V = 16 / sizeof(T);
     float* const s_rows = (float*)s_few;
-    const int64_t r0 = (int64_t)blockIdx.x * FEW_ROWS, r = r0 + threadIdx.x;
+    const int64_t r0 = (int64_t)block_index() * FEW_ROWS, r = r0 + threadIdx.x;
+    if (r0 >= p.rows) return;
     const int n = (int)(p.rows - r0 < FEW_ROWS ? p.rows - r0 : FEW_ROWS), stride = few_stride(p.vocab);
     stage_rows<T, MASK, QUADS, NT>(p, r0, n, stride, by_vocab, packed, s_rows);
     __syncthreads();
@@ -698,7 +703,7 @@ template <typename T, int MASK>
 void go_fwd(const LpArgs& a, int dtype, hipStream_t st) {
     const int tpr = threads_for(a.rows, a.vocab, dtype, a.top_k > 0), u = tpr ? vectors_for(a.vocab, dtype, tpr) : 0;
     const bool far = is_far(a, dtype, MASK);
-    const auto blocks = [&](int rows) { return dim3((unsigned)cdiv(a.rows, rows)); };
+    const auto blocks = [&](int rows) { return grid_of(cdiv(a.rows, rows)); };
     const dim3 b(256);
     if (tpr == 0) {
         const auto few = a.vocab % 4 ? far ? k_logp_few_fwd<T, MASK, false, true> : k_logp_few_fwd<T, MASK, false, false>
@@ -716,7 +721,7 @@ void go_fwd(const LpArgs& a, int dtype, hipStream_t st) {
         if (u == 2) hipLaunchKernelGGL((k_logp_fwd<T, MASK, false, 64, 2, false>), blocks(4), b, 0, st, a);
         else hipLaunchKernelGGL((k_logp_fwd<T, MASK, false, 64, 4, false>), blocks(4), b, 0, st, a);
     } else {
-        const dim3 grid((unsigned)(a.rows * a.splits));
+        const dim3 grid = grid_of(a.rows * a.splits);
         const auto k = a.top_k ? far ? k_logp_fwd<T, MASK, true, 256, MOST_U, true> : k_logp_fwd<T, MASK, true, 256, MOST_U, false>
                                : far ? k_logp_fwd<T, MASK, false, 256, MOST_U, true> : k_logp_fwd<T, MASK, false, 256, MOST_U, false>;
         hipLaunchKernelGGL(k, grid, b, 0, st, a);
@@ -728,7 +733,7 @@ template <typename T, int MASK>
 void go_bwd(const LpArgs& a, int dtype, hipStream_t st) {
     const int tpr = threads_for(a.rows, a.vocab, dtype, false), u = tpr ? vectors_for(a.vocab, dtype, tpr) : 0;
     const bool far = is_far(a, dtype, MASK);
-    const auto blocks = [&](int rows) { return dim3((unsigned)cdiv(a.rows, rows)); };
+    const auto blocks = [&](int rows) { return grid_of(cdiv(a.rows, rows)); };
     const dim3 b(256);
     const auto few = a.vocab % 4 ? far ? k_logp_few_bwd<T, MASK, false, true> : k_logp_few_bwd<T, MASK, false, false>
                                  : far ? k_logp_few_bwd<T, MASK, true, true> : k_logp_few_bwd<T, MASK, true, false>;
@@ -746,7 +751,7 @@ void go_bwd(const LpArgs& a, int dtype, hipStream_t st) {
         hipLaunchKernelGGL((k_logp_bwd<T, MASK, 64, 4, false>), blocks(4), b, 0, st, a);
     else
         hipLaunchKernelGGL((far ? k_logp_bwd<T, MASK, 256, MOST_U, true> : k_logp_bwd<T, MASK, 256, MOST_U, false>),
-                           dim3((unsigned)(a.rows * a.splits)), b, 0, st, a);
+                           grid_of(a.rows * a.splits), b, 0, st, a);
 }
 
 #define EC_LP_GO(GO, T)                                  \

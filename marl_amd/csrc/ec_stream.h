@@ -5,6 +5,13 @@
 
 namespace ecs {
 
+// A launch takes fewer than 2^32 threads along x: blocks from the 2^22nd on stand along y, and a few may be too many
+inline dim3 grid_of(int64_t blocks) {
+    const int64_t most = 1 << 22;
+    return blocks <= most ? dim3((unsigned)blocks) : dim3((unsigned)most, (unsigned)((blocks + most - 1) / most));
+}
+__device__ __forceinline__ uint32_t block_index() { return blockIdx.y << 22 | blockIdx.x; }
+
 using bf16 = __bf16;
 using f16 = _Float16;
 

@@ -325,3 +325,25 @@ def test_offsets_past_32_bits():
         assert th.equal(logprob_device.token_logprobs_bwd(l, t, a.lse, a.entropy, g, h, av),
                         logprob_device.token_logprobs_bwd(src, t, b.lse, b.entropy, g, h, on))
         del flat, mask, l, av
+
+
+def test_more_rows_than_a_launch_has_threads_along_x():
+    """2^26 + 3 rows with alternatives take a wave each: 2^32 + 192 threads.  All rows hold the same 64 logits, so each has
+    what a call of 64 rows, one per token, gives (the same kernel: the same bits)"""
+    from marl_amd.utils.logprob_device import token_logprobs_bwd, token_logprobs_fwd
+    rows, vocab = 2 ** 26 + 3, 64
+    one = th.randn(1, vocab, device="cuda").bfloat16()
+    each = th.arange(vocab, device="cuda")
+    few = token_logprobs_fwd(one.expand(vocab, vocab), each, top_k=1)
+    tokens = th.randint(0, vocab, (rows,), device="cuda")
+    all_rows = one.expand(rows, vocab)
+    f = token_logprobs_fwd(all_rows, tokens, top_k=1)
+    assert th.equal(f.logp, few.logp[tokens])
+    for name in ("entropy", "lse", "top_logp", "top_index"):
+        got, want = getattr(f, name), getattr(few, name)
+        assert bool((got == want[0]).all()), name
+    g = th.ones(rows, device="cuda")
+    d = token_logprobs_bwd(all_rows, tokens, f.lse, f.entropy, g)
+    few_d = token_logprobs_bwd(one.expand(vocab, vocab), each, few.lse, few.entropy, g[:vocab])
+    for a in range(0, rows, 2 ** 22):
+        assert th.equal(d[a:a + 2 ** 22], few_d[tokens[a:a + 2 ** 22]]), a
