@@ -684,15 +684,20 @@ bool is_packed(const LpArgs& a) {
 // i / vocab = umulhi(i, by_vocab) for i < 2^16 and 2 <= vocab < 2^16: the excess over 2^32 / vocab is below 1
 uint32_t by_vocab(int vocab) { return (uint32_t)((((uint64_t)1 << 32) + vocab - 1) / vocab); }
 
-// few rows: a row is split over as many blocks as fill the GPU, at least one batch of loads each
-int per_split(int64_t rows, int64_t vocab, int dtype) {
+// Few rows: a row is split over as many blocks as fill the GPU, at least one batch of loads each, and a second launch joins them.
+// Not where a block is through in few batches: the second launch is 4 us of the host's time, and of the GPU's 1 us or, with
+// alternatives to join, 5 (one row of 32000 in bf16, 4 batches: 17.4 us a call split, 13.1 whole, both 4.7 in a graph; with 20
+// alternatives 21.0 and 16.6, but 11.0 and 15.5 in a graph; 2 batches: 20.9 and 16.5, 9.7 and 9.2).
+int per_split(int64_t rows, int64_t vocab, int dtype, bool top) {
     if (threads_for(rows, vocab, dtype, true) != 256) return INT32_MAX;
-    const int64_t batch = 256 * MOST_U * (dtype == EC_F32 ? 4 : 8), batches = cdiv(vocab, batch), want = cdiv(1024, rows);
+    const int64_t batch = 256 * MOST_U * (dtype == EC_F32 ? 4 : 8), batches = cdiv(vocab, batch);
+    // (to the nearest: 900 rows of 65536 45.9 us by two blocks each, 40.7 by one; 600 of 200000 71.6 and 89.4)
+    const int64_t want = batches <= (top ? 2 : 4) || rows > 1024 ? 1 : (1024 + rows / 2) / rows;
     const int64_t splits = want < batches ? (want < MAX_SPLITS ? want : MAX_SPLITS) : (batches < MAX_SPLITS ? batches : MAX_SPLITS);
     const int64_t each = cdiv(batches, splits) * batch;
     return (int)(each < INT32_MAX ? each : INT32_MAX);
 }
-int splits_for(int64_t rows, int64_t vocab, int dtype) { return (int)cdiv(vocab, per_split(rows, vocab, dtype)); }
+int splits_for(int64_t rows, int64_t vocab, int dtype, bool top) { return (int)cdiv(vocab, per_split(rows, vocab, dtype, top)); }
 
 // The streaming hint for what the caches do not hold from one pass to the next.  (4.1 M rows of 11 under int32 masks 207 us
 // without it, 170 with; 8192 x 65536 in bf16 553 and 505; 3200 x 10000 44 and 47.  Not for 16 and 64 threads a row, which
@@ -774,7 +779,7 @@ void go_bwd(const LpArgs& a, int dtype, hipStream_t st) {
 
 extern "C" int64_t ec_token_logprobs_workspace(int64_t rows, int64_t vocab, int32_t dtype, int32_t top_k) {
     if (rows < 1 || vocab < 1 || vocab > INT32_MAX || !dtype_ok(dtype) || top_k < 0 || top_k > MAX_TOP) return 0;
-    const int s = splits_for(rows, vocab, dtype);
+    const int s = splits_for(rows, vocab, dtype, top_k > 0);
     return s > 1 ? rows * s * part_bytes(top_k) : 0;
 }
 
@@ -795,8 +800,8 @@ extern "C" int ec_token_logprobs_fwd(const void* logits, int64_t inner, int64_t 
                         (long long)work_bytes, (long long)need);
     a.top_k = top_k, a.logp = logp, a.entropy = entropy, a.lse = lse, a.top_logp = top_logp, a.top_index = top_index;
     a.work = (char*)work;
-    a.splits = splits_for(rows, vocab, dtype);
-    a.per_split = per_split(rows, vocab, dtype);
+    a.splits = splits_for(rows, vocab, dtype, top_k > 0);
+    a.per_split = per_split(rows, vocab, dtype, top_k > 0);
     if (rows * a.splits > INT32_MAX) return ec::fail(EC_EINVAL, "ec_token_logprobs_fwd: %lld rows", (long long)rows);
     const hipStream_t st = (hipStream_t)stream;
     EC_LP_TYPES(go_fwd)
