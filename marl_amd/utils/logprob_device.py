@@ -79,7 +79,8 @@ def token_logprobs_fwd(logits, tokens, avail=None, top_k=0):
     lead = tuple(tokens.shape)
     rows, vocab, code = head[-2], head[-1], head[-3]
     # (memory of its own for each: views of one tensor could not be changed in place under autograd)
-    logp, entropy = (th.empty(lead, dtype=th.float32, device=dev) for _ in range(2))
+    logp = th.empty_like(tokens, dtype=th.float32, memory_format=th.contiguous_format)
+    entropy = th.empty_like(logp)
     lse = th.empty(lead + (2,), dtype=th.float32, device=dev)
     top_logp = th.empty(lead + (top_k,), dtype=th.float32, device=dev) if top_k else None
     top_index = th.empty(lead + (top_k,), dtype=th.int64, device=dev) if top_k else None

@@ -90,7 +90,8 @@ def layer_norm_fwd(x, weight=None, bias=None, eps=1e-5, want_stats=True):
     y = th.empty_like(x, memory_format=th.contiguous_format)
     mean = rstd = None
     if want_stats:
-        mean, rstd = (th.empty(x.shape[:-1], dtype=th.float32, device=dev) for _ in range(2))
+        mean = th.empty(x.shape[:-1], dtype=th.float32, device=dev)
+        rstd = th.empty_like(mean)
     weight = weight.contiguous() if weight is not None else None
     bias = bias.contiguous() if bias is not None else None
     launch("ec_layer_norm_fwd", dev, x2.data_ptr(), x2.stride(0), ptr(weight), ptr(bias), code, wcode, rows, cols, eps, y.data_ptr(),
