@@ -352,6 +352,30 @@ def test_captured_and_replayed():
                 optim_device.adamw_step(ps, ps, ps, ps, step=1, lr=1e-3)
 
 
+@pytest.mark.parametrize("sizes,dtypes", [
+    ([1], [th.float32]), ([32768], [th.float32]), ([32769], [th.float32]), ([1023, 0, 1025, 7, 5000], [th.float32]),
+    ([5, 2049, 4097], [th.bfloat16]), ([300, 4001], [th.float16]), ([300, 4001], [th.float32, th.bfloat16]), ([17] * 48, [th.float32]),
+    ([17] * 49, [th.bfloat16]), ([8191, 8193, 70001], [th.float16])])
+def test_the_norm_of_few_and_of_many(sizes, dtypes):
+    """one block's sum (few elements of one type) and the joined ones; gradients at odd addresses.  The squares are exact in
+    double, their sum is off by less than 2^-36 of itself: what is left are the rounding of the norm to fp32, and for the
+    coefficient those of the sum and the quotient too"""
+    from marl_amd.utils.optim_device import clip_coef
+    gen = th.Generator(device="cuda").manual_seed(sum(sizes))
+    grads = [th.randn(n + 1, device="cuda", generator=gen).to(dtypes[i % len(dtypes)])[1:] for i, n in enumerate(sizes)]
+    want = float(th.cat([g.double() for g in grads]).norm())
+    for max_norm in (0.5 * want, 2 * want + 1):
+        norm, coef = (float(t) for t in clip_coef(grads, max_norm))
+        assert abs(norm - want) <= 1.01 * U * want
+        exact = min(1.0, max_norm / (want + 1e-6))
+        assert abs(coef - exact) <= 5 * U * exact, (coef, exact)
+        assert (norm, coef) == tuple(float(t) for t in clip_coef(grads, max_norm))
+    grads[-1][-1] = float("nan")
+    norm, coef = clip_coef(grads, 1.0)
+    assert norm.isnan() and coef.isnan()
+
+
+
 def test_refusals():
     from marl_amd.utils import optim_device
     S = optim_device.adamw_step
