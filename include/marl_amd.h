@@ -600,7 +600,8 @@ int ec_grad_clip_coef(int32_t count, const void* const* grads, const int64_t* nu
                       float* norm, float* coef, void* work, int64_t work_bytes, void* stream);
 /* One AdamW step (decoupled weight decay) over `count` tensors of any size; dtypes[i]: the type of params[i] and grads[i].
  * state_bits 32: exp_avg, exp_avg_sq f32 (scales NULL).  state_bits 8: exp_avg [numel] e4m3 with exp_avg_scale
- * [ceil(numel / 256)] f32: m = q * scale over each 256 consecutive elements; exp_avg_sq likewise holds sqrt(v).
+ * [ceil(numel / 256)] f32: m = q * scale over each 256 consecutive elements; exp_avg_sq likewise holds sqrt(v).  An
+ * infinite m or v makes its scale infinite, and NaN of those 256 from the next step on (a NaN stays one element's).
  * coef (optional, on the device) scales the gradients as they are read.  The step count is step_host (this step's, from 1
  * on), or *step_dev f32, which the call advances (dyn: scratch of 3 f32); with it lr may come from *lr_dev.  Pointers need
  * no alignment beyond their element's. */

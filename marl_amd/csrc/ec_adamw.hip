@@ -8,11 +8,15 @@
 // s = max |m| / 448, and v as (q s)^2, the root being what the step divides by and having half the range of v in exponents.
 // q is rounded to the nearest e4m3 value (relative step 2^-3 .. 2^-4, the states' only loss: the step itself uses m' and v'
 // before they are rounded), except that the q of a v' > 0 is never 0, which would turn a rounding into a step of lr m / eps.
+// A NaN stays its own element's; an infinite m' or v' makes its scale infinite, and NaN of the 256 from the next step on.
 //
 // Bound by HBM: every operand once, 28 bytes an element in fp32 (16 with 8-bit moments), no intermediate.  A launch takes
 // up to MAX_TENSORS tensors in its argument block, so nothing is copied to the device; a block finds its tensor by the
 // first block of each.  The clip reads g once more: per-block sums in double, added in a fixed order by one block, so that
 // the coefficient is the same every run; it stays on the device.
+//
+// Measured: 151 M fp32 parameters 737 us (5.7 TB/s); 201 M in bf16 with 8-bit moments 314 to 385 us (6.5 to 5.3 TB/s), the
+// norm 70 us (5.7) and the coefficient 5.
 #include <cmath>
 
 #include "ec_stream.h"

@@ -8,6 +8,12 @@
 // exact second pass over (x - mean) at no traffic; a thread keeps its columns from row to row, so that weight, bias and
 // the sums of dw and db stay in registers over all rows of a block.  dw and db leave as one partial row per block, added
 // up in a fixed order by a second kernel (no atomics: the same bits every run).  All sums are fp32.
+//
+// Measured (a copy runs at 6.4 TB/s at best): 4.1 M rows of 64 in fp32 388 us forward (5.5 TB/s) and 543 us backward (5.9);
+// 16384 rows of 4096 in bf16 48 us (5.6) and 77 us (5.2), dw and db of which 5 us more.  Rows that just miss a power of two
+// of vectors leave threads idle: 16384 rows of 2053 in fp16 43 us, of 4096 48.  (Not faster: as many waves as a row needs, a
+// number known at run time, 119 -> 145 us for 30000 rows of 1601; three vectors a thread instead of twice the threads, 43 ->
+// 44 us; idle vectors skipped by a branch, 43 -> 42 us there, but 126 -> 150 us where there are none.)
 #include "ec_stream.h"
 
 namespace {

@@ -177,7 +177,7 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, exp_avg_scale=None, exp_avg_s
     parameter's type.
     States in 32 bits: exp_avg, exp_avg_sq float32.  In 8 bits: exp_avg, exp_avg_sq float8_e4m3fn with exp_avg_scale,
     exp_avg_sq_scale [scale_count(p)] float32, where exp_avg * scale is m and exp_avg_sq * scale is sqrt(v), one scale for each
-    256 consecutive elements.
+    256 consecutive elements (an infinite gradient is lost to all of them, a NaN only to its own).
     step: this step's count, from 1 on; or a float32 scalar on the device (what a HIP graph needs), which the call advances
     first, and with which lr may be such a scalar too.
     max_norm: the gradients enter scaled by clip_coef(grads, max_norm)'s coef, and its norm is returned; coef: scaled by that
