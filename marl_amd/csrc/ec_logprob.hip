@@ -34,6 +34,7 @@ struct LpArgs {
     const void *logits, *avail;
     const int64_t* tokens;
     int64_t rows, inner, s_outer, s_inner, a_outer, a_inner;  // row r is at (r / inner) * s_outer + (r % inner) * s_inner
+    uint32_t by_inner;                                        // i / inner = umulhi(i, by_inner) for i < 2^16; 0: inner >= 2^15
     int vocab, top_k, splits, per_split;                      // per_split: columns of one split
     float *lse, *logp, *entropy;                              // lse [rows][2]: m, log S1
     float* top_logp;
@@ -509,7 +510,8 @@ __global__ void __launch_bounds__(256) k_logp_bwd(LpArgs p) {
 // FEW_ROWS rows are staged through LDS as fp32, excluded entries as -inf; packed rows come in and gradients leave 16 bytes a
 // lane whatever the row's width.  QUADS: widths that are multiples of 4 lie there at an odd multiple of 4, and lanes walk down
 // their rows four entries at a time; other widths at an odd stride, one at a time: different banks for different lanes either
-// way.  (128 rows a block: 64 and 256 are 2 to 12 % slower.)
+// way.  (128 rows a block: 64 and 256 are 2 to 12 % slower.)  GAPS: rows that are not packed, by a kernel of their own (in one
+// kernel with them packed rows take 3 % longer).
 constexpr int FEW_ROWS = 128;
 // up to this width (600 000 rows of 60 forward and back: bf16 89 us, with 16 lanes a row 140; fp32 139 and 125)
 constexpr int FEW_16BIT = 62, FEW_FP32 = 52;
@@ -540,50 +542,104 @@ __device__ __forceinline__ void each_entry(float* l, int vocab, F f) {
     }
 }
 
-template <typename T, int MASK, bool QUADS, bool NT>
-__device__ __forceinline__ void stage_rows(const LpArgs& p, int64_t r0, int n, int stride, uint32_t by_vocab, bool packed, float* s) {
+// where the rows of a tile are, from r0 on
+struct Tile {
+    int64_t at_l, at_a;  // of the group that r0 is in
+    uint32_t rem;        // r0's place in it
+    __device__ __forceinline__ Tile(const LpArgs& p, int64_t r0) {
+        int64_t q = r0;
+        if (p.inner != 1) q = ((r0 | p.inner) >> 32) == 0 ? (uint32_t)r0 / (uint32_t)p.inner : r0 / p.inner;
+        at_l = q * p.s_outer, at_a = q * p.a_outer, rem = (uint32_t)(r0 - q * p.inner);
+    }
+    __device__ __forceinline__ void find(const LpArgs& p, int row, int col, int64_t& l, int64_t& a) const {
+        const uint32_t x = rem + row;
+        const uint32_t q = p.inner == 1 ? x : p.by_inner ? __umulhi(x, p.by_inner) : x >= p.inner;
+        const uint32_t i = p.inner == 1 ? 0 : x - q * (uint32_t)p.inner;
+        l = at_l + q * p.s_outer + i * p.s_inner + col;
+        a = at_a + q * p.a_outer + i * p.a_inner + col;
+    }
+};
+
+// V entries of a tile from its i-th on: at once where they are of one row, or of rows in ORDER and V - 1 apart from first to
+// last; else one by one, with no branch between the loads.  (4.1 M rows of 11 in fp32 under int32 masks, both slices of wider
+// buffers: forward and back 83 and 107 us, an element at a time 148 and 167, packed 72 and 97)
+template <typename T, int MASK, bool NT, int V>
+__device__ __forceinline__ void load_apart(const LpArgs& p, const Tile& t, int i, int all, uint32_t by_vocab, bool order,
+                                           float (&f1)[1][V]) {
+    constexpr int S = MASK == 1 ? 1 : 4;
+    const T* l = (const T*)p.logits;
+    const char* av = (const char*)p.avail;
+    const int last = i + V <= all ? i + V - 1 : all - 1;
+    int row = row_in(i, p.vocab, by_vocab), col = i - row * p.vocab;
+    const int end = row_in(last, p.vocab, by_vocab);
+    int64_t l0, a0, l1, a1;
+    t.find(p, row, col, l0, a0);
+    t.find(p, end, last - end * p.vocab, l1, a1);
+    if (i + V <= all && (row == end || (order && l1 - l0 == V - 1 && (!MASK || a1 - a0 == V - 1)))) {
+        load_logits<T, MASK, NT, true>(l + l0, MASK ? av + a0 * S : nullptr, 0, 0, V, f1);
+    } else {
+        T x[V];
+        int32_t on[V];
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            t.find(p, row, col, l0, a0);
+            x[j] = l[l0];
+            on[j] = MASK == 0 ? 1 : MASK == 1 ? (int32_t)av[a0] : ((const int32_t*)av)[a0];
+            if (i + j < last && ++col == p.vocab) col = 0, row++;
+        }
+#pragma unroll
+        for (int j = 0; j < V; j++) f1[0][j] = i + j <= last && on[j] ? (float)x[j] : -INF;
+    }
+}
+
+template <typename T, int MASK, bool QUADS, bool NT, bool GAPS>
+__device__ __forceinline__ void stage_rows(const LpArgs& p, int64_t r0, int n, int stride, uint32_t by_vocab, bool order, float* s) {
     constexpr int V = 16 / sizeof(T);
-    if (packed) {  // the tile is one run of n * vocab elements, in logits and mask
-        const T* l = (const T*)p.logits + r0 * p.vocab;
-        const char* av = MASK ? (const char*)p.avail + r0 * p.vocab * (MASK == 1 ? 1 : 4) : nullptr;
-        const int all = n * p.vocab;
-        for (int i = threadIdx.x * V; i < all; i += FEW_ROWS * V) {
-            float f1[1][V], (&f)[V] = f1[0];
-            if (i + V <= all) load_logits<T, MASK, NT, true>(l, av, i, 0, all, f1);
-            else load_logits<T, MASK, false, false>(l, av, i, 0, all, f1);
-            if (QUADS) {  // (four entries in a row are of one row)
+    const int all = n * p.vocab;
+    const auto put = [&](int i, const float(&f)[V]) {
+        if (QUADS) {  // (four entries in a row are of one row)
 #pragma unroll
-                for (int q = 0; q < V; q += 4) {
-                    const int row = row_in(i + q, p.vocab, by_vocab), col = i + q - row * p.vocab;
-                    if (i + q < all) *(float4*)(s + row * stride + col) = make_float4(f[q], f[q + 1], f[q + 2], f[q + 3]);
-                }
-            } else if (stride == p.vocab) {  // (the tile lies in LDS as in memory, with room for the last vector)
+            for (int q = 0; q < V; q += 4) {
+                const int row = row_in(i + q, p.vocab, by_vocab), col = i + q - row * p.vocab;
+                if (i + q < all) *(float4*)(s + row * stride + col) = make_float4(f[q], f[q + 1], f[q + 2], f[q + 3]);
+            }
+        } else if (stride == p.vocab) {  // (the tile lies in LDS as in memory, with room for the last vector)
 #pragma unroll
-                for (int q = 0; q < V; q += 4) *(float4*)(s + i + q) = make_float4(f[q], f[q + 1], f[q + 2], f[q + 3]);
-            } else {
-                int row = row_in(i, p.vocab, by_vocab), col = i - row * p.vocab;
+            for (int q = 0; q < V; q += 4) *(float4*)(s + i + q) = make_float4(f[q], f[q + 1], f[q + 2], f[q + 3]);
+        } else {
+            int row = row_in(i, p.vocab, by_vocab), col = i - row * p.vocab;
 #pragma unroll
-                for (int j = 0; j < V; j++) {
-                    if (i + j < all) s[row * stride + col] = f[j];
-                    if (++col == p.vocab) col = 0, row++;
-                }
+            for (int j = 0; j < V; j++) {
+                if (i + j < all) s[row * stride + col] = f[j];
+                if (++col == p.vocab) col = 0, row++;
             }
         }
+    };
+    float f1[1][V];
+    if (!GAPS) {  // the tile is one run of n * vocab elements, in logits and mask
+        const T* l = (const T*)p.logits + r0 * p.vocab;
+        const char* av = MASK ? (const char*)p.avail + r0 * p.vocab * (MASK == 1 ? 1 : 4) : nullptr;
+        for (int i = threadIdx.x * V; i < all; i += FEW_ROWS * V) {
+            if (i + V <= all) load_logits<T, MASK, NT, true>(l, av, i, 0, all, f1);
+            else load_logits<T, MASK, false, false>(l, av, i, 0, all, f1);
+            put(i, f1[0]);
+        }
     } else {
-        for (int i = threadIdx.x; i < n * p.vocab; i += FEW_ROWS) {
-            const int row = row_in(i, p.vocab, by_vocab), col = i - row * p.vocab;
-            s[row * stride + col] = logit_at<T, MASK>(row_of<T>(p, r0 + row), MASK ? mask_of<MASK>(p, r0 + row) : nullptr, col);
+        const Tile t(p, r0);
+        for (int i = threadIdx.x * V; i < all; i += FEW_ROWS * V) {
+            load_apart<T, MASK, NT, V>(p, t, i, all, by_vocab, order, f1);
+            put(i, f1[0]);
         }
     }
 }
 
-template <typename T, int MASK, bool QUADS, bool NT>
-__global__ void __launch_bounds__(FEW_ROWS) k_logp_few_fwd(LpArgs p, uint32_t by_vocab, bool packed) {
+template <typename T, int MASK, bool QUADS, bool NT, bool GAPS>
+__global__ void __launch_bounds__(FEW_ROWS) k_logp_few_fwd(LpArgs p, uint32_t by_vocab, bool order) {
     extern __shared__ float4 s_few[];
     const int64_t r0 = (int64_t)block_index() * FEW_ROWS, r = r0 + threadIdx.x;
     if (r0 >= p.rows) return;
     const int n = (int)(p.rows - r0 < FEW_ROWS ? p.rows - r0 : FEW_ROWS), stride = few_stride(p.vocab);
-    stage_rows<T, MASK, QUADS, NT>(p, r0, n, stride, by_vocab, packed, (float*)s_few);
+    stage_rows<T, MASK, QUADS, NT, GAPS>(p, r0, n, stride, by_vocab, order, (float*)s_few);
     __syncthreads();
     if ((int)threadIdx.x >= n) return;
     float* l = (float*)s_few + threadIdx.x * stride;
@@ -610,15 +666,15 @@ __global__ void __launch_bounds__(FEW_ROWS) k_logp_few_fwd(LpArgs p, uint32_t by
     }
 }
 
-template <typename T, int MASK, bool QUADS, bool NT>
-__global__ void __launch_bounds__(FEW_ROWS) k_logp_few_bwd(LpArgs p, uint32_t by_vocab, bool packed) {
+template <typename T, int MASK, bool QUADS, bool NT, bool GAPS>
+__global__ void __launch_bounds__(FEW_ROWS) k_logp_few_bwd(LpArgs p, uint32_t by_vocab, bool order) {
     extern __shared__ float4 s_few[];
     constexpr int V = 16 / sizeof(T);
     float* const s_rows = (float*)s_few;
     const int64_t r0 = (int64_t)block_index() * FEW_ROWS, r = r0 + threadIdx.x;
     if (r0 >= p.rows) return;
     const int n = (int)(p.rows - r0 < FEW_ROWS ? p.rows - r0 : FEW_ROWS), stride = few_stride(p.vocab);
-    stage_rows<T, MASK, QUADS, NT>(p, r0, n, stride, by_vocab, packed, s_rows);
+    stage_rows<T, MASK, QUADS, NT, GAPS>(p, r0, n, stride, by_vocab, order, s_rows);
     __syncthreads();
     if ((int)threadIdx.x < n) {
         const RowGrad w = row_grad(p, r);
@@ -681,10 +737,19 @@ int vectors_for(int64_t vocab, int dtype, int tpr) {
     const int64_t each = cdiv(cdiv(vocab, dtype == EC_F32 ? 4 : 8), tpr);
     return each <= 1 ? 1 : each <= 2 ? 2 : MOST_U;
 }
-// rows that lie one behind the other, mask and logits
-bool is_packed(const LpArgs& a) {
-    const bool l = a.s_outer == a.inner * a.vocab && (a.inner == 1 || a.s_inner == a.vocab);
-    return l && (!a.avail || (a.a_outer == a.inner * a.vocab && (a.inner == 1 || a.a_inner == a.vocab)));
+// how rows of few entries lie in memory, logits and mask: one behind the other; in order, with gaps; anyhow (a mask for all)
+enum Layout { PACKED, APART, ANYHOW };
+
+// (APART takes rows in order that do not overlap: what lies V - 1 apart is then V in a row)
+Layout layout_of(const LpArgs& a) {
+    const auto one = [&](int64_t outer, int64_t inner) {
+        const bool packed = outer == a.inner * a.vocab && (a.inner == 1 || inner == a.vocab);
+        if (packed || a.rows == 1) return PACKED;
+        if (a.inner == 1) return outer >= a.vocab ? APART : ANYHOW;
+        return inner >= a.vocab && (a.inner >= a.rows || outer >= (a.inner - 1) * inner + a.vocab) ? APART : ANYHOW;
+    };
+    const Layout l = one(a.s_outer, a.s_inner), m = a.avail ? one(a.a_outer, a.a_inner) : PACKED;
+    return l > m ? l : m;
 }
 // i / vocab = umulhi(i, by_vocab) for i < 2^16 and 2 <= vocab < 2^16: the excess over 2^32 / vocab is below 1
 uint32_t by_vocab(int vocab) { return (uint32_t)((((uint64_t)1 << 32) + vocab - 1) / vocab); }
@@ -714,16 +779,25 @@ bool is_far(const LpArgs& a, int dtype, int mask) {
 int few_lds(int vocab) { return (FEW_ROWS * few_stride(vocab) + 8) * 4; }  // (the last vector of a tile may be a partial one)
 
 template <typename T, int MASK>
+auto few_fwd(bool quads, bool far, bool gaps) {
+    if (gaps)
+        return quads ? far ? k_logp_few_fwd<T, MASK, true, true, true> : k_logp_few_fwd<T, MASK, true, false, true>
+                     : far ? k_logp_few_fwd<T, MASK, false, true, true> : k_logp_few_fwd<T, MASK, false, false, true>;
+    return quads ? far ? k_logp_few_fwd<T, MASK, true, true, false> : k_logp_few_fwd<T, MASK, true, false, false>
+                 : far ? k_logp_few_fwd<T, MASK, false, true, false> : k_logp_few_fwd<T, MASK, false, false, false>;
+}
+
+template <typename T, int MASK>
 void go_fwd(LpArgs a, int dtype, hipStream_t st) {
     const int tpr = threads_for(a.rows, a.vocab, dtype, a.top_k > 0), u = tpr ? vectors_for(a.vocab, dtype, tpr) : 0;
     const bool far = is_far(a, dtype, MASK);
+    const Layout layout = layout_of(a);
     const auto blocks = [&](int rows) { return grid_of(cdiv(a.rows, rows)); };
     const dim3 b(256);
     a.ahead = a.splits == 1 && cdiv(a.rows, tpr ? 256 / tpr : 1) <= AT_ONCE;
     if (tpr == 0) {
-        const auto few = a.vocab % 4 ? far ? k_logp_few_fwd<T, MASK, false, true> : k_logp_few_fwd<T, MASK, false, false>
-                                     : far ? k_logp_few_fwd<T, MASK, true, true> : k_logp_few_fwd<T, MASK, true, false>;
-        hipLaunchKernelGGL(few, blocks(FEW_ROWS), dim3(FEW_ROWS), few_lds(a.vocab), st, a, by_vocab(a.vocab), is_packed(a));
+        const auto few = few_fwd<T, MASK>(a.vocab % 4 == 0, far, layout != PACKED);
+        hipLaunchKernelGGL(few, blocks(FEW_ROWS), dim3(FEW_ROWS), few_lds(a.vocab), st, a, by_vocab(a.vocab), layout == APART);
     } else if (tpr == 16) {
         if (u == 1) hipLaunchKernelGGL((k_logp_fwd<T, MASK, false, 16, 1, false>), blocks(16), b, 0, st, a);
         else if (u == 2) hipLaunchKernelGGL((k_logp_fwd<T, MASK, false, 16, 2, false>), blocks(16), b, 0, st, a);
@@ -745,15 +819,24 @@ void go_fwd(LpArgs a, int dtype, hipStream_t st) {
 }
 
 template <typename T, int MASK>
+auto few_bwd(bool quads, bool far, bool gaps) {
+    if (gaps)
+        return quads ? far ? k_logp_few_bwd<T, MASK, true, true, true> : k_logp_few_bwd<T, MASK, true, false, true>
+                     : far ? k_logp_few_bwd<T, MASK, false, true, true> : k_logp_few_bwd<T, MASK, false, false, true>;
+    return quads ? far ? k_logp_few_bwd<T, MASK, true, true, false> : k_logp_few_bwd<T, MASK, true, false, false>
+                 : far ? k_logp_few_bwd<T, MASK, false, true, false> : k_logp_few_bwd<T, MASK, false, false, false>;
+}
+
+template <typename T, int MASK>
 void go_bwd(const LpArgs& a, int dtype, hipStream_t st) {
     const int tpr = threads_for(a.rows, a.vocab, dtype, false), u = tpr ? vectors_for(a.vocab, dtype, tpr) : 0;
     const bool far = is_far(a, dtype, MASK);
+    const Layout layout = layout_of(a);
     const auto blocks = [&](int rows) { return grid_of(cdiv(a.rows, rows)); };
     const dim3 b(256);
-    const auto few = a.vocab % 4 ? far ? k_logp_few_bwd<T, MASK, false, true> : k_logp_few_bwd<T, MASK, false, false>
-                                 : far ? k_logp_few_bwd<T, MASK, true, true> : k_logp_few_bwd<T, MASK, true, false>;
+    const auto few = few_bwd<T, MASK>(a.vocab % 4 == 0, far, layout != PACKED);
     if (tpr == 0)
-        hipLaunchKernelGGL(few, blocks(FEW_ROWS), dim3(FEW_ROWS), few_lds(a.vocab), st, a, by_vocab(a.vocab), is_packed(a));
+        hipLaunchKernelGGL(few, blocks(FEW_ROWS), dim3(FEW_ROWS), few_lds(a.vocab), st, a, by_vocab(a.vocab), layout == APART);
     else if (tpr == 16 && u == 1)
         hipLaunchKernelGGL((k_logp_bwd<T, MASK, 16, 1, false>), blocks(16), b, 0, st, a);
     else if (tpr == 16 && u == 2)
@@ -795,6 +878,7 @@ extern "C" int ec_token_logprobs_fwd(const void* logits, int64_t inner, int64_t 
     LpArgs a{};
     a.logits = logits, a.avail = avail, a.tokens = tokens, a.rows = rows, a.inner = inner, a.s_outer = s_outer;
     a.s_inner = s_inner, a.a_outer = a_outer, a.a_inner = a_inner, a.vocab = (int)(vocab > INT32_MAX || vocab < 1 ? 0 : vocab);
+    a.by_inner = inner >= 2 && inner < 1 << 15 ? by_vocab((int)inner) : 0;
     if (const char* m = bad("ec_token_logprobs_fwd", a, dtype, mask_dtype)) return ec::fail(EC_EINVAL, "%s", m);
     if (top_k < 0 || top_k > MAX_TOP || (top_k && rows && (!top_logp || !top_index)))
         return ec::fail(EC_EINVAL, "ec_token_logprobs_fwd: %d alternatives (0 .. %d, with both outputs)", top_k, MAX_TOP);
@@ -821,6 +905,7 @@ extern "C" int ec_token_logprobs_bwd(const void* logits, int64_t inner, int64_t 
     LpArgs a{};
     a.logits = logits, a.avail = avail, a.tokens = tokens, a.rows = rows, a.inner = inner, a.s_outer = s_outer;
     a.s_inner = s_inner, a.a_outer = a_outer, a.a_inner = a_inner, a.vocab = (int)(vocab > INT32_MAX || vocab < 1 ? 0 : vocab);
+    a.by_inner = inner >= 2 && inner < 1 << 15 ? by_vocab((int)inner) : 0;
     if (const char* m = bad("ec_token_logprobs_bwd", a, dtype, mask_dtype)) return ec::fail(EC_EINVAL, "%s", m);
     if (rows == 0) return EC_OK;
     if (!lse || !entropy || !dlogits) return ec::fail(EC_EINVAL, "ec_token_logprobs_bwd: null argument");

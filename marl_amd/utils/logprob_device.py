@@ -15,19 +15,40 @@ MAX_TOP = 64  # EC_TOKEN_LOGPROBS_MAX_TOP
 TokenLogprobs = namedtuple("TokenLogprobs", "logp entropy top_logp top_index lse")
 
 
-def _layout(t, vocab):
-    """(tensor, inner, outer stride, inner stride): the rows of t [..., vocab] as [outer, inner] of them, a view where the
-    strides allow one (a slice of steps out of [batch, steps, vocab] does)"""
-    if t.dim() == 2:
-        t = t if vocab == 1 or t.stride(1) == 1 else t.contiguous()
-        return t, 1, t.stride(0), 0
-    lead = t.shape[:-1]
-    inner = lead[-1] if len(lead) >= 2 else 1
-    outer = lead[:-1].numel() if len(lead) >= 2 else lead.numel()
-    t = t.reshape(outer, inner, vocab)
-    if vocab > 1 and t.stride(2) != 1:
-        t = t.contiguous()
-    return t, max(1, inner), t.stride(0), t.stride(1)
+def _breaks(t):
+    """leading dimensions of t [..., vocab] that do not continue the one behind them (by stride): where its rows stop lying one
+    stride apart.  Each as the number of dimensions up to and with it"""
+    shape, stride = t.shape, t.stride()
+    dims = [d for d in range(len(shape) - 1) if shape[d] != 1]
+    return {a + 1 for a, b in zip(dims, dims[1:]) if stride[a] != stride[b] * shape[b]}
+
+
+def _steps(t, at):
+    """(outer, inner) stride of t's rows as [shape[:at], shape[at:-1]] (a part of one row: any)"""
+    shape, stride = t.shape, t.stride()
+    last = lambda lo, hi: next((stride[d] for d in range(hi - 1, lo - 1, -1) if shape[d] != 1), 0)
+    return last(0, at), last(at, len(shape) - 1)
+
+
+def _layout(logits, avail):
+    """(logits, avail, inner, logits' outer and inner stride, avail's): rows as [outer, inner] of them, of both tensors alike,
+    and in place wherever their strides allow one such split (a slice of steps out of [batch, steps, agents, vocab] does)"""
+    vocab = logits.shape[-1]
+    if vocab > 1 and logits.stride(-1) != 1:
+        logits = logits.contiguous()
+    if avail is not None and vocab > 1 and avail.stride(-1) != 1:
+        avail = avail.contiguous()
+    at = _breaks(logits) if logits.dim() > 2 else set()
+    if avail is not None and logits.dim() > 2:
+        both = at | _breaks(avail)
+        if len(both) > 1:
+            avail = avail.contiguous()
+        else:
+            at = both
+    if len(at) > 1:
+        logits, at = logits.contiguous(), set()
+    at = at.pop() if at else logits.dim() - 1
+    return (logits, avail, max(1, logits.shape[at:-1].numel()), *_steps(logits, at), *(_steps(avail, at) if avail is not None else (0, 0)))
 
 
 def _inputs(who, logits, tokens, avail):
@@ -52,10 +73,7 @@ def _inputs(who, logits, tokens, avail):
         if avail.dtype not in (th.bool, th.uint8, th.int8, th.int32):
             avail = avail != 0
         kind = 2 if avail.dtype == th.int32 else 1
-        avail, _, ao, ai = _layout(avail, vocab)
-    else:
-        ao = ai = 0
-    logits, inner, so, si = _layout(logits, vocab)
+    logits, avail, inner, so, si, ao, ai = _layout(logits, avail)
     tokens = tokens.to(th.int64).contiguous()
     # (the tensors are kept by the caller until the launch is made)
     head = (logits.data_ptr(), inner, so, si, tokens.data_ptr(), ptr(avail), kind, ao, ai, code, tokens.numel(), vocab)

@@ -203,6 +203,39 @@ def test_views_and_broadcast_masks(vocab):
     assert th.equal(a.logp[0], F(base[:, :-1, :vocab], t, on).logp) and a.logp.shape == (1, 3, 5)
 
 
+@pytest.mark.parametrize("dtype", [th.float32, th.bfloat16])
+@pytest.mark.parametrize("vocab", [1, 3, 8, 11, 30, 40, 130])
+def test_rows_with_gaps(vocab, dtype):
+    """logits and masks as views of wider buffers, in one order and in different ones: the bits of the packed call"""
+    from marl_amd.utils import logprob_device
+    gen = th.Generator(device="cuda").manual_seed(vocab)
+    big = th.randn(9, 8, 7, vocab + 3, device="cuda", generator=gen).to(dtype)
+    on = th.rand(9, 8, 7, vocab + 3, device="cuda", generator=gen) < 0.6
+    views = [lambda x: x[:, :-1, :, :vocab], lambda x: x[:8, 1:, :, 3:], lambda x: x[:8, :7, :, 1:vocab + 1].contiguous(),
+             lambda x: x[..., :vocab].contiguous()[:, :-1], lambda x: x[..., :vocab].contiguous()[1:, 1:],
+             lambda x: x[..., :vocab].contiguous()[:, :, 1:], lambda x: x[:7, :8, :, :vocab].transpose(0, 1),
+             lambda x: x[:1, :1, :, 2:vocab + 2].expand(8, 7, 7, vocab), lambda x: x[:1, :7, :1, 2:vocab + 2].expand(8, 7, 7, vocab)]
+    for i, lv in enumerate(views):
+        for k, mv in enumerate([None, views[i], *views[:5], *views[7:]]):
+            l = lv(big)
+            a = mv(on) if mv else None
+            if a is not None:                                # (what both have)
+                n, m, o = (min(x, y) for x, y in zip(l.shape[:3], a.shape[:3]))
+                l, a = l[:n, :m, :o], a[:n, :m, :o]
+            a = a.to((th.int32, th.bool, th.int64)[(i + k) % 3]) if a is not None and k % 2 else a
+            t = th.randint(0, vocab, l.shape[:-1], device="cuda", generator=gen)
+            g = th.randn(l.shape[:-1], device="cuda", generator=gen)
+            plain = a.contiguous() if a is not None else None
+            f = logprob_device.token_logprobs_fwd(l, t, a, min(3, vocab))
+            e = logprob_device.token_logprobs_fwd(l.contiguous(), t, plain, min(3, vocab))
+            assert all(th.equal(p, q) for p, q in zip(f, e)), (i, k)
+            assert th.equal(logprob_device.token_logprobs_bwd(l, t, f.lse, f.entropy, g, g, a),
+                            logprob_device.token_logprobs_bwd(l.contiguous(), t, e.lse, e.entropy, g, g, plain)), (i, k)
+    for shape in ((2, 0, vocab), (0, 3, vocab), (0, vocab)):
+        f = logprob_device.token_logprobs_fwd(big.new_empty(shape), th.zeros(shape[:-1], dtype=th.int64, device="cuda"))
+        assert f.logp.shape == shape[:-1]
+
+
 def test_autograd_and_differences():
     """token_logprobs' gradient is token_logprobs_bwd's, also through either output alone, and the slope of the loss"""
     from marl_amd.utils import logprob_device
