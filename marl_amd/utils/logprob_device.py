@@ -38,8 +38,10 @@ def _layout(logits, avail):
         logits = logits.contiguous()
     if avail is not None and vocab > 1 and avail.stride(-1) != 1:
         avail = avail.contiguous()
-    at = _breaks(logits) if logits.dim() > 2 else set()
-    if avail is not None and logits.dim() > 2:
+    if logits.dim() == 2:
+        return logits, avail, 1, logits.stride(0), 0, avail.stride(0) if avail is not None else 0, 0
+    at = _breaks(logits)
+    if avail is not None:
         both = at | _breaks(avail)
         if len(both) > 1:
             avail = avail.contiguous()
