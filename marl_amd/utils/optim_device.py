@@ -237,6 +237,15 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, exp_avg_scale=None, exp_avg_s
     return norm
 
 
+def _need_options(group):
+    """torch's optimisers share their group's options by state_dict: one under which the update is another is refused"""
+    for k in ("maximize", "amsgrad", "differentiable"):
+        if group.get(k):
+            raise ValueError("AdamW: %s=%r (only False)" % (k, group[k]))
+    if not group.get("decoupled_weight_decay", True) and group["weight_decay"]:
+        raise ValueError("AdamW: weight_decay %r with decoupled_weight_decay=False" % (group["weight_decay"],))
+
+
 class AdamW(th.optim.Optimizer):
     """torch.optim.AdamW's update (decoupled weight decay, no amsgrad) over all tensors in a few launches, with moments in 32
     bits or in 8 (state_bits, per group), and clip_grad_norm_ over all groups on the way (max_norm; the gradients stay as
@@ -261,6 +270,7 @@ class AdamW(th.optim.Optimizer):
         super().add_param_group(param_group)
         g = self.param_groups[-1]
         try:
+            _need_options(g)
             if g["state_bits"] not in (8, 32):
                 raise ValueError("AdamW: state_bits %r (8 or 32)" % (g["state_bits"],))
             if isinstance(g["lr"], th.Tensor) and not g["capturable"]:
@@ -305,6 +315,7 @@ class AdamW(th.optim.Optimizer):
                 loss = closure()
         calls, every = [], []
         for group in self.param_groups:
+            _need_options(group)
             by_step = {}
             for p in group["params"]:
                 g = p.grad
@@ -337,8 +348,9 @@ class AdamW(th.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """torch's load casts states to their parameter's type: here they keep their own, and a capturable group gets its one
-        step count back.  Takes torch.optim.AdamW's state_dict too (states in 32 bits)."""
+        step count back.  Takes torch.optim.AdamW's state_dict too (states in 32 bits, no amsgrad, not maximize)."""
         for saved in state_dict["param_groups"]:
+            _need_options(saved)
             bits = saved.get("state_bits", self.defaults["state_bits"])
             want = {"step", "exp_avg", "exp_avg_sq"} | ({"exp_avg_scale", "exp_avg_sq_scale"} if bits == 8 else set())
             for i in saved["params"]:

@@ -1,0 +1,73 @@
+"""What optim_device.AdamW takes into its state and its groups: nothing is launched, so all of it is checked without a GPU."""
+import copy
+
+import pytest
+import torch as th
+
+
+def _params(*shapes):
+    g = th.Generator().manual_seed(0)
+    return [th.nn.Parameter(th.randn(s, generator=g)) for s in shapes or ((3, 4), (7,))]
+
+
+def _stepped(opt, steps=1):
+    """a torch optimiser after `steps` steps"""
+    for _ in range(steps):
+        for g in opt.param_groups:
+            for p in g["params"]:
+                p.grad = th.ones_like(p)
+        opt.step()
+    return opt
+
+
+def _snapshot(opt):
+    return copy.deepcopy(opt.state_dict())
+
+
+def _same(a, b):
+    if isinstance(a, dict):
+        return a.keys() == b.keys() and all(_same(a[k], b[k]) for k in a)
+    if isinstance(a, (list, tuple)):
+        return len(a) == len(b) and all(map(_same, a, b))
+    if isinstance(a, th.Tensor):
+        return a.dtype == b.dtype and a.shape == b.shape and th.equal(a.reshape(-1).view(th.uint8), b.reshape(-1).view(th.uint8))
+    return a == b
+
+
+@pytest.mark.parametrize("option", ["maximize", "amsgrad", "differentiable"])
+@pytest.mark.parametrize("steps", [0, 1])
+def test_options_of_another_update_are_refused(option, steps):
+    """torch's AdamW with an option that changes the step: its state_dict, a group made with it, and a group that got it later
+    are refused; the optimiser stays as it was"""
+    from marl_amd.utils.optim_device import AdamW
+    ps = _params()
+    if option == "differentiable" and steps:
+        pytest.skip("torch steps a leaf in place under this option only where no gradient is recorded")
+    saved = _stepped(th.optim.AdamW(ps, **{option: True}), steps).state_dict()
+    opt = AdamW(_params())
+    before = _snapshot(opt)
+    with pytest.raises(ValueError, match=option if option != "amsgrad" or not steps else "amsgrad|max_exp_avg_sq"):
+        opt.load_state_dict(saved)
+    assert _same(opt.state_dict(), before)
+    with pytest.raises(ValueError, match=option):
+        AdamW([{"params": _params(), option: True}])
+    with pytest.raises(ValueError, match=option):
+        opt.add_param_group({"params": _params(), option: True})
+    assert len(opt.param_groups) == 1
+    opt.param_groups[0][option] = True
+    with pytest.raises(ValueError, match=option):
+        opt.step()
+
+
+def test_a_decay_that_is_part_of_the_gradient_is_refused():
+    """torch.optim.Adam's weight decay enters the moments; without one its states continue here, as does its group"""
+    from marl_amd.utils.optim_device import AdamW
+    opt = AdamW(_params())
+    with pytest.raises(ValueError, match="decoupled_weight_decay"):
+        opt.load_state_dict(_stepped(th.optim.Adam(_params(), weight_decay=0.1)).state_dict())
+    assert not opt.state and opt.param_groups[0]["weight_decay"] == 1e-2
+    opt.load_state_dict(_stepped(th.optim.Adam(_params()), 3).state_dict())
+    assert [st["step"] for st in opt.state.values()] == [3, 3]
+    opt.param_groups[0]["weight_decay"] = 0.1
+    with pytest.raises(ValueError, match="decoupled_weight_decay"):
+        opt.step()
