@@ -252,19 +252,21 @@ class AdamW(th.optim.Optimizer):
     they are; `last_norm` holds the norm).  Parameters: contiguous, on one device, float32, bfloat16 or float16.
 
     State: state[p] = {"step", "exp_avg", "exp_avg_sq"} and, with 8 bits, {"exp_avg_scale", "exp_avg_sq_scale"} (see
-    adamw_step); state_dict / load_state_dict keep their types.  capturable: the step count lives on the device, one for the
-    parameters of a group, and lr may be a device scalar -- for steps recorded into a HIP graph."""
+    adamw_step); state_dict / load_state_dict keep their types.  capturable: step counts live on the device, and lr may be a
+    device scalar -- for steps recorded into a HIP graph.  Parameters of a group that have taken the same steps share one
+    count; where a gradient is missing for some of them they get one of their own.  Not while a graph is recorded, and not
+    once a graph has recorded the shared one, which it would go on advancing for all (RuntimeError)."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, max_norm=None, state_bits=32,
                  capturable=False):
         if max_norm is not None and not max_norm > 0:
             raise ValueError("AdamW: max_norm %r" % (max_norm,))
-        self.max_norm, self.last_norm = max_norm, None
+        self.max_norm, self.last_norm, self._recorded = max_norm, None, []
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       capturable=capturable))
 
     def __getstate__(self):  # (torch's names three attributes: what a copy or a pickle keeps)
-        return dict(super().__getstate__(), max_norm=self.max_norm, last_norm=None)
+        return dict(super().__getstate__(), max_norm=self.max_norm, last_norm=None, _recorded=[])
 
     def add_param_group(self, param_group):
         super().add_param_group(param_group)
@@ -288,7 +290,8 @@ class AdamW(th.optim.Optimizer):
             self.param_groups.pop()
             raise
 
-    def _init(self, group, p):
+    def _init(self, group, p, count):
+        """p's state; count: the step count of a capturable group's parameters that take their first step together"""
         if th.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW: the first step of a parameter makes its state; take it before a HIP graph is recorded")
         st = self.state[p]
@@ -302,10 +305,25 @@ class AdamW(th.optim.Optimizer):
             st["exp_avg_sq"] = th.zeros(p.shape, dtype=th.float32, **kw)
         if not group["capturable"]:
             st["step"] = 0
-        else:  # one count for the group
-            have = [self.state[q]["step"] for q in group["params"] if "step" in self.state.get(q, ())]
-            st["step"] = have[0] if have else th.zeros((), dtype=th.float32, **kw)
+        else:
+            st["step"] = count if count is not None else th.zeros((), dtype=th.float32, **kw)
         return st
+
+    def _split(self, calls, idle):
+        """a count of their own, as it stands, for parameters without a gradient (`idle`: their states) that share one which
+        this step advances"""
+        live = {id(step): step for _, step, _ in calls if isinstance(step, th.Tensor)}
+        apart = {}
+        for st in idle:
+            if id(st["step"]) in live:
+                apart.setdefault(id(st["step"]), []).append(st)
+        if apart and (th.cuda.is_current_stream_capturing() or any(id(t) in apart for t in self._recorded)):
+            raise RuntimeError("AdamW: parameters with and without a gradient share a step count that a HIP graph records; take a "
+                               "step with the same gradients missing before it is recorded")
+        for at, sts in apart.items():
+            own = live[at].clone()
+            for st in sts:
+                st["step"] = own
 
     @th.no_grad()
     def step(self, closure=None):
@@ -313,42 +331,51 @@ class AdamW(th.optim.Optimizer):
         if closure is not None:
             with th.enable_grad():
                 loss = closure()
-        calls, every = [], []
+        calls, every, idle = [], [], []
         for group in self.param_groups:
             _need_options(group)
-            by_step = {}
+            by_step, count = {}, None
             for p in group["params"]:
                 g = p.grad
                 if g is None:
+                    if p in self.state:
+                        idle.append(self.state[p])
                     continue
                 if g.is_sparse:
                     raise RuntimeError("AdamW: sparse gradients are not supported")
                 if not g.is_contiguous():
                     g = g.contiguous()
-                st = self.state[p] if p in self.state else self._init(group, p)
+                if p in self.state:
+                    st = self.state[p]
+                else:
+                    st = self._init(group, p, count)
+                    count = st["step"]
                 step = st["step"]
-                by_step.setdefault(None if group["capturable"] else step, []).append((p, g, st))
+                by_step.setdefault((id(step),) if isinstance(step, th.Tensor) else step, []).append((p, g, st))
                 every.append(g)
-            calls += [(group, step, ts) for step, ts in by_step.items()]
+            calls += [(group, ts[0][2]["step"], ts) for ts in by_step.values()]
         if not every:
             return loss
+        self._split(calls, idle)
         coef = None
         if self.max_norm is not None:
             self.last_norm, coef = clip_coef(every, self.max_norm)
         for group, step, ts in calls:
+            on_dev = isinstance(step, th.Tensor)
             cols = lambda k: [st[k] for _, _, st in ts]
             scales = [cols("exp_avg_scale"), cols("exp_avg_sq_scale")] if group["state_bits"] == 8 else []
             adamw_step([p for p, _, _ in ts], [g for _, g, _ in ts], cols("exp_avg"), cols("exp_avg_sq"), *scales,
-                       step=ts[0][2]["step"] if step is None else step + 1, lr=group["lr"], betas=group["betas"], eps=group["eps"],
+                       step=step if on_dev else step + 1, lr=group["lr"], betas=group["betas"], eps=group["eps"],
                        weight_decay=group["weight_decay"], coef=coef)
-            if step is not None:  # (after the call: a refused one has counted nothing)
+            if not on_dev:  # (after the call: a refused one has counted nothing)
                 for _, _, st in ts:
                     st["step"] = step + 1
+            elif th.cuda.is_current_stream_capturing():
+                self._recorded.append(step)
         return loss
 
     def load_state_dict(self, state_dict):
-        """torch's load casts states to their parameter's type: here they keep their own, and a capturable group gets its one
-        step count back.  Takes torch.optim.AdamW's state_dict too (states in 32 bits, no amsgrad, not maximize)."""
+        """torch's load casts states to their parameter's type: here they keep their own.  Takes torch.optim.AdamW's state_dict too (states in 32 bits, no amsgrad, not maximize)."""
         for saved in state_dict["param_groups"]:
             _need_options(saved)
             bits = saved.get("state_bits", self.defaults["state_bits"])
@@ -363,7 +390,7 @@ class AdamW(th.optim.Optimizer):
             for k, v in self.defaults.items():
                 group.setdefault(k, v)
             group["capturable"] = bool(group["capturable"])
-            count = None
+            counts = {}  # (of a capturable group: one for each value)
             for i, p in zip(saved["params"], group["params"]):
                 if i not in state_dict["state"]:
                     continue
@@ -371,8 +398,9 @@ class AdamW(th.optim.Optimizer):
                 for k, v in state_dict["state"][i].items():
                     if k != "step":
                         st[k] = v.detach().to(p.device, STATE8 if v.dtype == STATE8 else th.float32, copy=True).contiguous()
-                    elif group["capturable"]:  # one count for the group
-                        count = count if count is not None else th.tensor(float(v), dtype=th.float32, device=p.device)
-                        st[k] = count
+                    elif group["capturable"]:
+                        if float(v) not in counts:
+                            counts[float(v)] = th.tensor(float(v), dtype=th.float32, device=p.device)
+                        st[k] = counts[float(v)]
                     else:
                         st[k] = int(v)

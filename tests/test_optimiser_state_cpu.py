@@ -71,3 +71,23 @@ def test_a_decay_that_is_part_of_the_gradient_is_refused():
     opt.param_groups[0]["weight_decay"] = 0.1
     with pytest.raises(ValueError, match="decoupled_weight_decay"):
         opt.step()
+
+
+def test_a_capturable_group_keeps_each_parameters_count():
+    """torch's states hold a count per parameter: loaded, each parameter has its own back, equal ones share one tensor"""
+    from marl_amd.utils.optim_device import AdamW
+    src = th.optim.AdamW(_params((4,), (5,), (6,)))
+    ps = src.param_groups[0]["params"]
+    for step in range(3):
+        for i, p in enumerate(ps):
+            p.grad = th.ones_like(p) if i != 1 or step == 2 else None
+        src.step()
+    saved = src.state_dict()
+    saved["param_groups"][0]["capturable"] = True
+    opt = AdamW(_params((4,), (5,), (6,)), capturable=True)
+    opt.load_state_dict(saved)
+    steps = [opt.state[p]["step"] for p in opt.param_groups[0]["params"]]
+    assert [float(s) for s in steps] == [3, 1, 3] and steps[0] is steps[2] and steps[0] is not steps[1]
+    again = AdamW(_params((4,), (5,), (6,)), capturable=True)
+    again.load_state_dict(opt.state_dict())
+    assert _same(again.state_dict(), opt.state_dict())
