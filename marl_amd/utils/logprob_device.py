@@ -8,7 +8,7 @@ from collections import namedtuple
 import torch as th
 
 from marl_amd import _abi
-from marl_amd.utils.norm_device import launch, need_device, need_dtype, ptr, refuse_capture
+from marl_amd.utils.norm_device import launch, need_device, need_dtype, ptr, refuse_capture, refuse_tangent
 
 MAX_TOP = 64  # EC_TOKEN_LOGPROBS_MAX_TOP
 
@@ -153,7 +153,8 @@ class _TokenLogprobsFn(th.autograd.Function):
 def token_logprobs(logits, tokens, avail=None, top_k=0):
     """token_logprobs_fwd with gradients of logp and entropy for logits (the alternatives and lse carry none).  Not while a
     HIP graph is recorded (RuntimeError, unless logits need no gradient): record token_logprobs_fwd and token_logprobs_bwd
-    there."""
+    there.  No forward-mode derivative (RuntimeError)."""
+    refuse_tangent("token_logprobs", logits)
     if th.is_grad_enabled() and logits.requires_grad:
         refuse_capture("token_logprobs", "token_logprobs_fwd and token_logprobs_bwd")
         return TokenLogprobs(*_TokenLogprobsFn.apply(logits, tokens, avail, top_k))

@@ -3,6 +3,7 @@
 `layer_norm` is the autograd form; `layer_norm_fwd` and `layer_norm_bwd` are the two passes by hand, for update steps that
 keep no autograd graph and for recording into a HIP graph."""
 import torch as th
+from torch.autograd import forward_ad
 
 from marl_amd import _abi
 
@@ -51,6 +52,12 @@ def refuse_capture(who, instead):
     process -- refused before anything is recorded"""
     if th.cuda.is_current_stream_capturing():
         raise RuntimeError("%s: no autograd while a HIP graph is recorded; record %s" % (who, instead))
+
+
+def refuse_tangent(who, *tensors):
+    """a forward-mode tangent would be dropped and the result pass for a constant: such a tensor has requires_grad False"""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("%s: no forward-mode derivative" % who)
 
 
 def _rows(t, cols):
@@ -153,7 +160,8 @@ class _LayerNormFn(th.autograd.Function):
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """layer_norm_fwd's y, with gradients for x, weight and bias.  Not while a HIP graph is recorded (RuntimeError, unless
-    nothing needs a gradient): record layer_norm_fwd and layer_norm_bwd there."""
+    nothing needs a gradient): record layer_norm_fwd and layer_norm_bwd there.  No forward-mode derivative (RuntimeError)."""
+    refuse_tangent("layer_norm", x, weight, bias)
     if th.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
         refuse_capture("layer_norm", "layer_norm_fwd and layer_norm_bwd")
         return _LayerNormFn.apply(x, weight, bias, eps)
