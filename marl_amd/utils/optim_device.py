@@ -246,6 +246,22 @@ def _need_options(group):
         raise ValueError("AdamW: weight_decay %r with decoupled_weight_decay=False" % (group["weight_decay"],))
 
 
+def _need_state(i, p, st, bits):
+    """a saved state of parameter p, the i-th: its names, shapes and types"""
+    float_of = lambda t: t.is_floating_point() and t.dtype != STATE8
+    moment = lambda t: t.shape == p.shape and (t.dtype == STATE8 if bits == 8 else float_of(t))
+    want = dict(exp_avg=moment, exp_avg_sq=moment)
+    if bits == 8:
+        want["exp_avg_scale"] = want["exp_avg_sq_scale"] = lambda t: t.shape == (scale_count(p),) and float_of(t)
+    bad = sorted(set(st) ^ set(want) ^ {"step"}) or [k for k, ok in want.items() if not isinstance(st[k], th.Tensor) or not ok(st[k])]
+    if not bad and not (st["step"].numel() == 1 if isinstance(st["step"], th.Tensor) else isinstance(st["step"], (int, float))):
+        bad = ["step"]
+    if bad:
+        is_ = lambda v: "%s %s" % (v.dtype, tuple(v.shape)) if isinstance(v, th.Tensor) else repr(v)
+        raise ValueError("AdamW.load_state_dict: parameter %s %s has %s for states of %d bits"
+                         % (i, tuple(p.shape), ", ".join("%s %s" % (k, is_(st[k]) if k in st else "missing") for k in bad), bits))
+
+
 class AdamW(th.optim.Optimizer):
     """torch.optim.AdamW's update (decoupled weight decay, no amsgrad) over all tensors in a few launches, with moments in 32
     bits or in 8 (state_bits, per group), and clip_grad_norm_ over all groups on the way (max_norm; the gradients stay as
@@ -375,16 +391,14 @@ class AdamW(th.optim.Optimizer):
         return loss
 
     def load_state_dict(self, state_dict):
-        """torch's load casts states to their parameter's type: here they keep their own.  Takes torch.optim.AdamW's state_dict too (states in 32 bits, no amsgrad, not maximize)."""
-        for saved in state_dict["param_groups"]:
+        """torch's load casts states to their parameter's type: here they keep their own.  Takes torch.optim.AdamW's state_dict
+        too (states in 32 bits, no amsgrad, not maximize).  What does not fit is refused before anything is replaced."""
+        for saved, group in zip(state_dict["param_groups"], self.param_groups):
             _need_options(saved)
             bits = saved.get("state_bits", self.defaults["state_bits"])
-            want = {"step", "exp_avg", "exp_avg_sq"} | ({"exp_avg_scale", "exp_avg_sq_scale"} if bits == 8 else set())
-            for i in saved["params"]:
-                st = state_dict["state"].get(i)
-                if st is not None and (set(st) != want or (bits == 8) != (st["exp_avg"].dtype == STATE8)):
-                    raise ValueError("AdamW.load_state_dict: parameter %s has %s (%s) for states of %d bits"
-                                     % (i, sorted(st), st["exp_avg"].dtype if "exp_avg" in st else None, bits))
+            for i, p in zip(saved["params"], group["params"]):
+                if i in state_dict["state"]:
+                    _need_state(i, p, state_dict["state"][i], bits)
         super().load_state_dict(state_dict)
         for saved, group in zip(state_dict["param_groups"], self.param_groups):
             for k, v in self.defaults.items():

@@ -91,3 +91,43 @@ def test_a_capturable_group_keeps_each_parameters_count():
     again = AdamW(_params((4,), (5,), (6,)), capturable=True)
     again.load_state_dict(opt.state_dict())
     assert _same(again.state_dict(), opt.state_dict())
+
+
+def _saved(bits, opt=None):
+    """a state_dict of one step, of parameters (3, 4) and (7,)"""
+    from marl_amd.utils.optim_device import STATE8, AdamW
+    opt = opt or AdamW(_params(), state_bits=bits)
+    for p in opt.param_groups[0]["params"]:
+        n = p.numel()
+        st = opt.state[p] = dict(step=1, exp_avg=th.ones(p.shape), exp_avg_sq=th.ones(p.shape))
+        if bits == 8:
+            st.update(exp_avg=th.ones(p.shape).to(STATE8), exp_avg_sq=th.ones(p.shape).to(STATE8))
+            st.update(exp_avg_scale=th.ones(-(-n // 256)), exp_avg_sq_scale=th.ones(-(-n // 256)))
+    return opt.state_dict()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("key", ["exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale", "step"])
+def test_states_of_other_sizes_and_types_are_refused(key, bits):
+    """before anything of the optimiser is replaced"""
+    from marl_amd.utils.optim_device import AdamW
+    if bits == 32 and key.endswith("_scale"):
+        pytest.skip("no scales")
+    good = _saved(bits)
+    opt = AdamW(_params(), state_bits=bits, lr=0.25)
+    opt.load_state_dict(_saved(bits, AdamW(_params(), state_bits=bits, lr=0.25)))
+    before = _snapshot(opt)
+    old = good["state"][1][key]
+    bad = [th.ones(3), "1"] if key == "step" else [th.ones(8).to(old.dtype), th.ones(1, 7).to(old.dtype), [1.0] * 7]
+    if key in ("exp_avg", "exp_avg_sq"):
+        bad += [old.to(th.float32 if bits == 8 else th.float8_e4m3fn), old.to(th.int32)]
+    for value in bad:
+        saved = copy.deepcopy(good)
+        saved["state"][1][key] = value
+        with pytest.raises(ValueError, match="parameter 1"):
+            opt.load_state_dict(saved)
+        assert _same(opt.state_dict(), before)
+    del good["state"][1][key]
+    with pytest.raises(ValueError, match="parameter 1"):
+        opt.load_state_dict(good)
+    assert _same(opt.state_dict(), before)
