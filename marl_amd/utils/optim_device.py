@@ -395,13 +395,16 @@ class AdamW(th.optim.Optimizer):
         too (states in 32 bits, no amsgrad, not maximize).  What does not fit is refused before anything is replaced."""
         for saved, group in zip(state_dict["param_groups"], self.param_groups):
             _need_options(saved)
-            bits = saved.get("state_bits", self.defaults["state_bits"])
+            bits = saved.get("state_bits", group["state_bits"])
+            if bits not in (8, 32):
+                raise ValueError("AdamW.load_state_dict: state_bits %r (8 or 32)" % (bits,))
             for i, p in zip(saved["params"], group["params"]):
                 if i in state_dict["state"]:
                     _need_state(i, p, state_dict["state"][i], bits)
+        own = [{k: group[k] for k in self.defaults} for group in self.param_groups]
         super().load_state_dict(state_dict)
-        for saved, group in zip(state_dict["param_groups"], self.param_groups):
-            for k, v in self.defaults.items():
+        for saved, group, options in zip(state_dict["param_groups"], self.param_groups, own):
+            for k, v in options.items():  # (what the state_dict does not name stays as it was)
                 group.setdefault(k, v)
             group["capturable"] = bool(group["capturable"])
             counts = {}  # (of a capturable group: one for each value)

@@ -131,3 +131,43 @@ def test_states_of_other_sizes_and_types_are_refused(key, bits):
     with pytest.raises(ValueError, match="parameter 1"):
         opt.load_state_dict(good)
     assert _same(opt.state_dict(), before)
+
+
+@pytest.mark.parametrize("default", [32, 8])
+def test_a_groups_own_bits_outlast_a_load_that_names_none(default):
+    """torch's state_dict names no state_bits: each group keeps its own, whatever the constructor's default was"""
+    from marl_amd.utils.optim_device import AdamW
+    make = lambda: AdamW([dict(params=_params(), state_bits=40 - default), dict(params=_params((5,)))], state_bits=default)
+    torchs = lambda: th.optim.AdamW([dict(params=_params()), dict(params=_params((5,)))])
+    opt = make()
+    opt.load_state_dict(torchs().state_dict())
+    assert [g["state_bits"] for g in opt.param_groups] == [40 - default, default]
+    # states only for the group of 32 bits: taken; for that of 8: refused
+    wide, narrow = (0, 1) if default == 8 else (1, 0)
+    for k in (wide, narrow):
+        src = torchs()
+        for p in src.param_groups[k]["params"]:
+            p.grad = th.ones_like(p)
+        src.step()
+        opt = make()
+        if k == wide:
+            opt.load_state_dict(src.state_dict())
+            assert all(opt.state[p]["exp_avg"].dtype == th.float32 for p in opt.param_groups[k]["params"])
+            assert [g["state_bits"] for g in opt.param_groups] == [40 - default, default]
+        else:
+            with pytest.raises(ValueError, match="8 bits"):
+                opt.load_state_dict(src.state_dict())
+    with pytest.raises(ValueError, match="state_bits"):
+        saved = make().state_dict()
+        saved["param_groups"][1]["state_bits"] = 16
+        make().load_state_dict(saved)
+
+
+def test_options_that_a_state_dict_lacks_are_the_groups_own():
+    from marl_amd.utils.optim_device import AdamW
+    opt = AdamW([dict(params=_params(), capturable=True, eps=1e-5)])
+    saved = opt.state_dict()
+    for k in ("capturable", "eps"):
+        del saved["param_groups"][0][k]
+    opt.load_state_dict(saved)
+    assert opt.param_groups[0]["capturable"] is True and opt.param_groups[0]["eps"] == 1e-5
