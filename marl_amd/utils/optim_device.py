@@ -398,6 +398,8 @@ class AdamW(th.optim.Optimizer):
             bits = saved.get("state_bits", group["state_bits"])
             if bits not in (8, 32):
                 raise ValueError("AdamW.load_state_dict: state_bits %r (8 or 32)" % (bits,))
+            if isinstance(saved["lr"], th.Tensor) and not saved.get("capturable", group["capturable"]):
+                raise ValueError("AdamW.load_state_dict: a learning rate on the device needs capturable=True")
             for i, p in zip(saved["params"], group["params"]):
                 if i in state_dict["state"]:
                     _need_state(i, p, state_dict["state"][i], bits)

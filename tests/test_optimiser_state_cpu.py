@@ -171,3 +171,12 @@ def test_options_that_a_state_dict_lacks_are_the_groups_own():
         del saved["param_groups"][0][k]
     opt.load_state_dict(saved)
     assert opt.param_groups[0]["capturable"] is True and opt.param_groups[0]["eps"] == 1e-5
+
+
+def test_a_learning_rate_on_the_device_needs_capturable_at_load_too():
+    from marl_amd.utils.optim_device import AdamW
+    opt = AdamW(_params(), lr=0.5)
+    before = _snapshot(opt)
+    with pytest.raises(ValueError, match="capturable"):
+        opt.load_state_dict(th.optim.AdamW(_params(), lr=th.tensor(1e-3), foreach=False).state_dict())
+    assert _same(opt.state_dict(), before)
