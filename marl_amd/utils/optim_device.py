@@ -409,6 +409,8 @@ class AdamW(th.optim.Optimizer):
             for k, v in options.items():  # (what the state_dict does not name stays as it was)
                 group.setdefault(k, v)
             group["capturable"] = bool(group["capturable"])
+            if isinstance(group["lr"], th.Tensor) and group["params"]:  # (a checkpoint's may have come by the host)
+                group["lr"] = group["lr"].detach().to(group["params"][0].device, th.float32)
             counts = {}  # (of a capturable group: one for each value)
             for i, p in zip(saved["params"], group["params"]):
                 if i not in state_dict["state"]:

@@ -93,3 +93,33 @@ def test_a_count_that_a_graph_advances_is_not_split():
     a[3].grad = None                    # neither of those two: nothing is split
     oa.step()
     assert [float(oa.state[p]["step"]) for p in a] == [6] * 3 + [4] * 2
+
+
+def test_a_checkpoint_on_the_host_continues_with_a_learning_rate_on_the_device(tmp_path):
+    """saved, loaded with map_location="cpu" and continued, recorded into a HIP graph: the bits of the optimiser that went on"""
+    from marl_amd.utils.optim_device import AdamW
+    a, b = _params(), _params()
+    oa, ob = (AdamW(ps, lr=th.full((), 1e-2, device="cuda"), capturable=True) for ps in (a, b))
+    _grads(a, 0)
+    oa.step()
+    th.save([[p.detach() for p in a], oa.state_dict()], tmp_path / "o.th")
+    ps, saved = th.load(tmp_path / "o.th", map_location="cpu", weights_only=True)
+    for p, q in zip(b, ps):
+        p.data.copy_(q)
+    ob.load_state_dict(saved)
+    lr = ob.param_groups[0]["lr"]
+    assert lr.device == b[0].device and lr.dtype == th.float32
+    _grads(b, 1)
+    graph = th.cuda.CUDAGraph()
+    with th.cuda.graph(graph):
+        ob.step()
+    for k in range(1, 5):
+        _grads(a, k)
+        for p, q in zip(a, b):
+            q.grad.copy_(p.grad)
+        oa.param_groups[0]["lr"].fill_(1e-2 / k)
+        lr.fill_(1e-2 / k)
+        graph.replay()
+        oa.step()
+        th.cuda.synchronize()
+        assert all(th.equal(p, q) for p, q in zip(a, b)), k
