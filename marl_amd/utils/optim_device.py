@@ -297,7 +297,7 @@ class AdamW(th.optim.Optimizer):
             if not (0 <= b1 < 1 and 0 <= b2 < 1 and g["eps"] >= 0 and g["weight_decay"] >= 0
                     and (isinstance(g["lr"], th.Tensor) or g["lr"] >= 0)):
                 raise ValueError("AdamW: lr %r, betas %r, eps %r, weight_decay %r" % (g["lr"], g["betas"], g["eps"], g["weight_decay"]))
-            dev = self.param_groups[0]["params"][0].device
+            dev = next((p.device for group in self.param_groups for p in group["params"]), None)
             for p in g["params"]:
                 if p.dtype not in DTYPES or not p.is_contiguous() or p.device != dev:
                     raise ValueError("AdamW: a parameter of type %s, strides %s on %s (contiguous float32, bfloat16 or float16 on one "

@@ -180,3 +180,14 @@ def test_a_learning_rate_on_the_device_needs_capturable_at_load_too():
     with pytest.raises(ValueError, match="capturable"):
         opt.load_state_dict(th.optim.AdamW(_params(), lr=th.tensor(1e-3), foreach=False).state_dict())
     assert _same(opt.state_dict(), before)
+
+
+def test_groups_without_parameters():
+    """as torch takes them (a net without biases, say): first, last and filled by none"""
+    from marl_amd.utils.optim_device import AdamW
+    opt = AdamW([dict(params=[]), dict(params=_params()), dict(params=[], lr=1.0)])
+    assert [len(g["params"]) for g in opt.param_groups] == [0, 2, 0]
+    AdamW([dict(params=[]), dict(params=_params()), dict(params=[], lr=1.0)]).load_state_dict(opt.state_dict())
+    with pytest.raises(ValueError, match="on one device"):
+        opt.add_param_group(dict(params=[th.nn.Parameter(th.zeros(3, device="meta"))]))
+    assert len(opt.param_groups) == 3
