@@ -393,6 +393,22 @@ class AdamW(th.optim.Optimizer):
     def load_state_dict(self, state_dict):
         """torch's load casts states to their parameter's type: here they keep their own.  Takes torch.optim.AdamW's state_dict
         too (states in 32 bits, no amsgrad, not maximize).  What does not fit is refused before anything is replaced."""
+        own = []
+
+        def check(_, saved):
+            self._need_state_dict(saved)
+            own[:] = saved, [{k: group[k] for k in self.defaults} for group in self.param_groups]
+
+        # (behind the last of the user's hooks in front of a load, and ahead of the first behind it)
+        hooks = [self.register_load_state_dict_pre_hook(check),
+                 self.register_load_state_dict_post_hook(lambda _: self._take_states(*own), prepend=True)]
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for h in hooks:
+                h.remove()
+
+    def _need_state_dict(self, state_dict):
         for saved, group in zip(state_dict["param_groups"], self.param_groups):
             _need_options(saved)
             bits = saved.get("state_bits", group["state_bits"])
@@ -403,8 +419,9 @@ class AdamW(th.optim.Optimizer):
             for i, p in zip(saved["params"], group["params"]):
                 if i in state_dict["state"]:
                     _need_state(i, p, state_dict["state"][i], bits)
-        own = [{k: group[k] for k in self.defaults} for group in self.param_groups]
-        super().load_state_dict(state_dict)
+
+    def _take_states(self, state_dict, own):
+        """what torch's load has cast, as it was saved; own: each group's options before"""
         for saved, group, options in zip(state_dict["param_groups"], self.param_groups, own):
             for k, v in options.items():  # (what the state_dict does not name stays as it was)
                 group.setdefault(k, v)

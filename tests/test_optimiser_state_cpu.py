@@ -191,3 +191,33 @@ def test_groups_without_parameters():
     with pytest.raises(ValueError, match="on one device"):
         opt.add_param_group(dict(params=[th.nn.Parameter(th.zeros(3, device="meta"))]))
     assert len(opt.param_groups) == 3
+
+
+def test_load_state_dict_hooks():
+    """a pre-hook's state_dict is the one that is checked and loaded; a post-hook sees, and may change, the loaded states"""
+    from marl_amd.utils.optim_device import AdamW
+    ps = [p.bfloat16() for p in _params()]
+    opt = AdamW([th.nn.Parameter(p.detach()) for p in ps])
+
+    def pre(o, state_dict):
+        return dict(state_dict, state={i: {k: v * 2 if k == "exp_avg" else v for k, v in st.items()}
+                                       for i, st in state_dict["state"].items()})
+    seen = []
+
+    def post(o):
+        seen.extend(st["exp_avg"].dtype for st in o.state.values())
+        for st in o.state.values():
+            st["step"] = 7
+    opt.register_load_state_dict_pre_hook(pre)
+    opt.register_load_state_dict_post_hook(post)
+    opt.load_state_dict(_saved(32))
+    assert seen == [th.float32, th.float32]
+    assert all(st["step"] == 7 and bool((st["exp_avg"] == 2).all()) for st in opt.state.values())
+    opt.register_load_state_dict_pre_hook(lambda o, s: dict(s, state={0: {"step": 1}}))
+    with pytest.raises(ValueError, match="parameter 0"):
+        opt.load_state_dict(_saved(32))
+    assert all(st["step"] == 7 for st in opt.state.values())
+    opt = AdamW(_params())
+    for _ in range(2):                                        # (nothing of a load is left behind)
+        opt.load_state_dict(_saved(32))
+    assert not opt._optimizer_load_state_dict_pre_hooks and not opt._optimizer_load_state_dict_post_hooks
