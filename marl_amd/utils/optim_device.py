@@ -397,7 +397,7 @@ class AdamW(th.optim.Optimizer):
 
         def check(_, saved):
             self._need_state_dict(saved)
-            own[:] = saved, [{k: group[k] for k in self.defaults} for group in self.param_groups]
+            own[:] = saved, [{k: group[k] for k in self.defaults if k in group} for group in self.param_groups]
 
         # (behind the last of the user's hooks in front of a load, and ahead of the first behind it)
         hooks = [self.register_load_state_dict_pre_hook(check),

@@ -221,3 +221,14 @@ def test_load_state_dict_hooks():
     for _ in range(2):                                        # (nothing of a load is left behind)
         opt.load_state_dict(_saved(32))
     assert not opt._optimizer_load_state_dict_pre_hooks and not opt._optimizer_load_state_dict_post_hooks
+
+
+def test_loaded_again_and_copied():
+    """a load after a load, and after a copy (torch adds an option to the defaults there that no group has)"""
+    from marl_amd.utils.optim_device import AdamW
+    opt = AdamW(_params(), state_bits=8)
+    saved = _saved(8)
+    for o in (opt, copy.deepcopy(opt)):
+        for _ in range(3):
+            o.load_state_dict(saved)
+            assert _same(o.state_dict()["state"], saved["state"])
