@@ -9,6 +9,7 @@ ec_grad_clip_coef, ec_adamw_step: AdamW over any number of tensors of any size, 
 import array
 import ctypes as C
 import operator
+from collections import namedtuple
 
 import torch as th
 
@@ -182,6 +183,24 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, exp_avg_scale=None, exp_avg_s
     first, and with which lr may be such a scalar too.
     max_norm: the gradients enter scaled by clip_coef(grads, max_norm)'s coef, and its norm is returned; coef: scaled by that
     device scalar (one clip over several calls).  The gradients are only read."""
+    work = _checked_step(params, grads, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, step, lr, betas, eps, weight_decay, coef)
+    norm = None
+    if max_norm is not None:
+        if coef is not None:
+            raise ValueError("adamw_step: max_norm and coef")
+        if not max_norm > 0:
+            raise ValueError("adamw_step: max_norm %r" % (max_norm,))
+        norm, coef = _clip_coef(work.dev, work.grads, work.counts, work.codes, max_norm)
+    _launch_step(work, coef)
+    return norm
+
+
+# a step's arguments once they are checked: arrays of addresses, sizes and type codes, and what they were made from
+_Step = namedtuple("_Step", "dev tensors pointers grads counts codes bits step lr betas eps weight_decay")
+
+
+def _checked_step(params, grads, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, step, lr, betas, eps, weight_decay, coef=None):
+    """all that adamw_step refuses, ahead of all that it launches"""
     who = "adamw_step"
     dev = _device_of(who, params)
     n, at = len(params), dev.index
@@ -208,9 +227,8 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, exp_avg_scale=None, exp_avg_s
     for name, t in (("step", step), ("lr", lr), ("coef", coef)):
         if isinstance(t, th.Tensor) and (t.device != dev or t.dtype != th.float32 or t.numel() != 1):
             raise ValueError("adamw_step: %s on the device is one float32 value on %s" % (name, dev))
-    dyn = None
     if isinstance(step, th.Tensor):
-        dyn = th.empty(3, dtype=th.float32, device=dev)
+        pass
     elif isinstance(lr, th.Tensor):
         raise ValueError("adamw_step: a learning rate on the device needs a step count there")
     elif not step >= 1:
@@ -220,21 +238,18 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, exp_avg_scale=None, exp_avg_s
     b1, b2 = (float(b) for b in betas)
     if not (0 <= b1 < 1 and 0 <= b2 < 1 and eps >= 0 and weight_decay >= 0 and (isinstance(lr, th.Tensor) or lr >= 0)):
         raise ValueError("adamw_step: lr %r, betas %r, eps %r, weight_decay %r" % (lr, betas, eps, weight_decay))
-    norm = None
-    if max_norm is not None:
-        if coef is not None:
-            raise ValueError("adamw_step: max_norm and coef")
-        if not max_norm > 0:
-            raise ValueError("adamw_step: max_norm %r" % (max_norm,))
     counts, codes = array.array("q", numel), array.array("i", map(DTYPES.get, kinds))
-    if max_norm is not None:
-        norm, coef = _clip_coef(dev, G, counts, codes, max_norm)
-    on_dev, lr_dev = dyn is not None, isinstance(lr, th.Tensor)
-    launch("ec_adamw_step", dev, n, *map(_address, (P, G, M, V, MS, VS, counts, codes)), bits, ptr(coef), 0.0 if on_dev else step,
-           ptr(step if on_dev else None), ptr(dyn), 0.0 if lr_dev else lr, ptr(lr if lr_dev else None), b1, b2, eps, weight_decay)
+    return _Step(dev, params, (P, G, M, V, MS, VS, counts, codes), G, counts, codes, bits, step, lr, (b1, b2), eps, weight_decay)
+
+
+def _launch_step(w, coef):
+    on_dev, lr_dev, params = isinstance(w.step, th.Tensor), isinstance(w.lr, th.Tensor), w.tensors
+    dyn = th.empty(3, dtype=th.float32, device=w.dev) if on_dev else None
+    launch("ec_adamw_step", w.dev, len(params), *map(_address, w.pointers), w.bits, ptr(coef), 0.0 if on_dev else w.step,
+           ptr(w.step if on_dev else None), ptr(dyn), 0.0 if lr_dev else w.lr, ptr(w.lr if lr_dev else None), *w.betas, w.eps,
+           w.weight_decay)
     # (written through raw pointers: autograd has to know; what was made in inference mode counts no versions)
     th.autograd.graph.increment_version([p for p in params if not p.is_inference()] if params[0].is_inference() else params)
-    return norm
 
 
 def _need_options(group):
@@ -372,18 +387,21 @@ class AdamW(th.optim.Optimizer):
             calls += [(group, ts[0][2]["step"], ts) for ts in by_step.values()]
         if not every:
             return loss
+        # (all calls are checked before the first is launched: what is refused has changed nothing)
+        checked = []
+        for group, step, ts in calls:
+            cols = lambda k: [st[k] for _, _, st in ts]
+            scales = [cols("exp_avg_scale"), cols("exp_avg_sq_scale")] if group["state_bits"] == 8 else [None, None]
+            checked.append(_checked_step([p for p, _, _ in ts], [g for _, g, _ in ts], cols("exp_avg"), cols("exp_avg_sq"), *scales,
+                                         step if isinstance(step, th.Tensor) else step + 1, group["lr"], group["betas"], group["eps"],
+                                         group["weight_decay"]))
         self._split(calls, idle)
         coef = None
         if self.max_norm is not None:
             self.last_norm, coef = clip_coef(every, self.max_norm)
-        for group, step, ts in calls:
-            on_dev = isinstance(step, th.Tensor)
-            cols = lambda k: [st[k] for _, _, st in ts]
-            scales = [cols("exp_avg_scale"), cols("exp_avg_sq_scale")] if group["state_bits"] == 8 else []
-            adamw_step([p for p, _, _ in ts], [g for _, g, _ in ts], cols("exp_avg"), cols("exp_avg_sq"), *scales,
-                       step=step if on_dev else step + 1, lr=group["lr"], betas=group["betas"], eps=group["eps"],
-                       weight_decay=group["weight_decay"], coef=coef)
-            if not on_dev:  # (after the call: a refused one has counted nothing)
+        for (_, step, ts), work in zip(calls, checked):
+            _launch_step(work, coef)
+            if not isinstance(step, th.Tensor):
                 for _, _, st in ts:
                     st["step"] = step + 1
             elif th.cuda.is_current_stream_capturing():

@@ -123,3 +123,48 @@ def test_a_checkpoint_on_the_host_continues_with_a_learning_rate_on_the_device(t
         oa.step()
         th.cuda.synchronize()
         assert all(th.equal(p, q) for p, q in zip(a, b)), k
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("what", ["lr", "betas", "state", "parameter", "gradient", "option"])
+def test_a_step_that_is_refused_has_done_nothing(what, bits):
+    """something wrong in the last of two groups: no parameter, state, count or norm changes in either; put right, the step is
+    the one of an optimiser that met no refusal"""
+    from marl_amd.utils.optim_device import AdamW
+    a, b = _params(), _params()
+    oa, ob = (AdamW([dict(params=ps[:2]), dict(params=ps[2:])], max_norm=1.0, state_bits=bits) for ps in (a, b))
+    for ps, o in ((a, oa), (b, ob)):
+        _grads(ps, 0)
+        o.step()
+        _grads(ps, 1)
+    before = copy.deepcopy(oa.state_dict()), [p.detach().clone() for p in a], oa.last_norm
+    group, st = oa.param_groups[1], oa.state[a[4]]
+    kept = dict(group), dict(st), a[4].data, a[4].grad
+    if what == "lr":
+        group["lr"] = -1.0
+    elif what == "betas":
+        group["betas"] = (0.9, 1.0)
+    elif what == "state":
+        st["exp_avg_sq"] = st["exp_avg_sq"][:-1].clone()
+    elif what == "parameter":
+        a[4].data = th.zeros(600, device="cuda")[::2]
+    elif what == "gradient":
+        a[4].grad = None
+        a[4].grad_dtype = None
+        a[4].grad = kept[3].bfloat16()
+    else:
+        group["maximize"] = True
+    with pytest.raises(ValueError):
+        oa.step()
+    a[4].data = kept[2]
+    a[4].grad = kept[3]
+    st.update(kept[1])
+    group.update(kept[0])
+    group.pop("maximize", None) if what == "option" else None
+    assert oa.last_norm is before[2] and all(th.equal(p, q) for p, q in zip(a, before[1]))
+    for i, s in oa.state_dict()["state"].items():
+        assert all(th.equal(v.view(-1).view(th.uint8), w.view(-1).view(th.uint8)) if isinstance(v, th.Tensor) else v == w
+                   for v, w in zip(s.values(), before[0]["state"][i].values()))
+    oa.step()
+    ob.step()
+    assert all(th.equal(p, q) for p, q in zip(a, b)) and th.equal(oa.last_norm, ob.last_norm)
