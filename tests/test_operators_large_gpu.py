@@ -20,7 +20,9 @@ U = 2.0 ** -24
 # rows: past one round of all blocks and no multiple of it (waves a CU times 256 CUs, as blocks_for has them)
 NORM = [(270001, 11), (70003, 29), (20011, 61), (10007, 125), (9001, 250), (9001, 300), (5003, 1003), (2503, 1601), (2503, 2048),
         (1100, 4093), (700, 8191), (300, 16384), (1027, 16391), (40, 40003)]
-NORM_FAR = [(3100001, 11), (600001, 61), (8301, 4099), (2053, 16384)]       # from 2^25 elements on: the streaming hint
+# past 2^25 elements: the streaming hint
+NORM_FAR = [(4800001, 7), (3100001, 11), (1200001, 29), (600001, 61), (280001, 125), (140001, 250), (70001, 500), (34001, 1003),
+            (16501, 2047), (8301, 4093), (8301, 4099), (2053, 16384)]
 
 
 @pytest.mark.parametrize("dtype,wdtype", [(th.float32, th.float32), (th.bfloat16, th.float32), (th.float16, th.float16)])
@@ -43,8 +45,10 @@ def test_layer_norm(rows, cols, dtype, wdtype):
 @pytest.mark.parametrize("mask", [None, th.bool, th.int32])
 @pytest.mark.parametrize("rows,vocab,dtype", [
     (4099, 1203, th.float32), (4099, 4001, th.float32), (4099, 2100, th.bfloat16), (4099, 8001, th.float16),  # a wave a row, batch by batch
-    (4099, 4101, th.float32), (1009, 50021, th.float32), (601, 100003, th.bfloat16)])                        # a block a row; the last two far
-def test_token_logprobs_of_wide_rows(rows, vocab, dtype, mask):
+    (4099, 4101, th.float32), (1009, 50021, th.float32), (601, 100003, th.bfloat16), (601, 100003, th.float16),  # a block; the last three far
+    (307, 200, th.bfloat16), (307, 400, th.bfloat16), (307, 200, th.float16), (307, 400, th.float16), (307, 120, th.float32),  # 16
+    (307, 200, th.float32), (307, 400, th.float32)])                          # lanes a row, and a wave
+def test_token_logprobs_of_middle_and_wide_rows(rows, vocab, dtype, mask):
     from marl_amd.utils import logprob_device
     l, t, avail, g, h = L._inputs(rows, vocab, dtype, mask)
     lp, want, tol = L._reference(l, t, avail, g, h)
@@ -79,13 +83,14 @@ def test_ties_over_the_batches_of_a_wave(vocab, dtype):
 
 
 @pytest.mark.parametrize("gaps", [False, True])
-@pytest.mark.parametrize("rows,vocab,dtype,mask", [(1300003, 11, th.float32, th.int32), (2300003, 11, th.float32, None),
-                                                   (1100001, 12, th.float32, th.int32), (1500001, 23, th.bfloat16, th.bool),
-                                                   (2000003, 28, th.float16, None)])
-def test_token_logprobs_of_few_entries_with_the_streaming_hint(rows, vocab, dtype, mask, gaps):
+@pytest.mark.parametrize("mask", [None, th.bool, th.int32])
+@pytest.mark.parametrize("dtype", [th.float32, th.bfloat16, th.float16])
+@pytest.mark.parametrize("vocab", [11, 20, 26])
+def test_token_logprobs_of_few_entries_with_the_streaming_hint(vocab, dtype, mask, gaps):
     """more than 96 MiB of logits and mask: the bits of calls on parts of the rows, which have no hint, and the formulas there"""
     from marl_amd.utils import logprob_device
     F, B = logprob_device.token_logprobs_fwd, logprob_device.token_logprobs_bwd
+    rows = (100 << 20) // (vocab * (th.finfo(dtype).bits // 8 + {None: 0, th.bool: 1, th.int32: 4}[mask])) + 3
     l, t, avail, g, h = L._inputs(rows, vocab, dtype, mask)
     if gaps:
         wide = lambda x: th.nn.functional.pad(x.view(th.uint8) if x.dtype == th.bool else x, (1, 2))[:, 1:vocab + 1]
@@ -104,7 +109,7 @@ def test_token_logprobs_of_few_entries_with_the_streaming_hint(rows, vocab, dtyp
 
 
 @pytest.mark.parametrize("bits", [32, 8])
-@pytest.mark.parametrize("dtype", [th.float32, th.bfloat16])
+@pytest.mark.parametrize("dtype", [th.float32, th.bfloat16, th.float16])
 def test_adamw_with_the_streaming_hint(dtype, bits):
     """9.5 M elements in one call against the formulas, and tensor by tensor (under the 8 M of the hint): the same bits"""
     from marl_amd.utils import optim_device
