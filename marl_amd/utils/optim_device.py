@@ -9,7 +9,6 @@ ec_grad_clip_coef, ec_adamw_step: AdamW over any number of tensors of any size, 
 import array
 import ctypes as C
 import operator
-from collections import namedtuple
 
 import torch as th
 
@@ -190,17 +189,14 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, exp_avg_scale=None, exp_avg_s
             raise ValueError("adamw_step: max_norm and coef")
         if not max_norm > 0:
             raise ValueError("adamw_step: max_norm %r" % (max_norm,))
-        norm, coef = _clip_coef(work.dev, work.grads, work.counts, work.codes, max_norm)
-    _launch_step(work, coef)
+        dev, _, (_, G, _, _, _, _, counts, codes) = work[:3]
+        norm, coef = _clip_coef(dev, G, counts, codes, max_norm)
+    _launch_step(coef, *work)
     return norm
 
 
-# a step's arguments once they are checked: arrays of addresses, sizes and type codes, and what they were made from
-_Step = namedtuple("_Step", "dev tensors pointers grads counts codes bits step lr betas eps weight_decay")
-
-
 def _checked_step(params, grads, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, step, lr, betas, eps, weight_decay, coef=None):
-    """all that adamw_step refuses, ahead of all that it launches"""
+    """all that adamw_step refuses, ahead of all that it launches; what _launch_step takes behind coef"""
     who = "adamw_step"
     dev = _device_of(who, params)
     n, at = len(params), dev.index
@@ -239,25 +235,25 @@ def _checked_step(params, grads, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_
     if not (0 <= b1 < 1 and 0 <= b2 < 1 and eps >= 0 and weight_decay >= 0 and (isinstance(lr, th.Tensor) or lr >= 0)):
         raise ValueError("adamw_step: lr %r, betas %r, eps %r, weight_decay %r" % (lr, betas, eps, weight_decay))
     counts, codes = array.array("q", numel), array.array("i", map(DTYPES.get, kinds))
-    return _Step(dev, params, (P, G, M, V, MS, VS, counts, codes), G, counts, codes, bits, step, lr, (b1, b2), eps, weight_decay)
+    return dev, params, (P, G, M, V, MS, VS, counts, codes), bits, step, lr, b1, b2, eps, weight_decay
 
 
-def _launch_step(w, coef):
-    on_dev, lr_dev, params = isinstance(w.step, th.Tensor), isinstance(w.lr, th.Tensor), w.tensors
-    dyn = th.empty(3, dtype=th.float32, device=w.dev) if on_dev else None
-    launch("ec_adamw_step", w.dev, len(params), *map(_address, w.pointers), w.bits, ptr(coef), 0.0 if on_dev else w.step,
-           ptr(w.step if on_dev else None), ptr(dyn), 0.0 if lr_dev else w.lr, ptr(w.lr if lr_dev else None), *w.betas, w.eps,
-           w.weight_decay)
+def _launch_step(coef, dev, params, pointers, bits, step, lr, b1, b2, eps, weight_decay):
+    """pointers: addresses of parameters, gradients and states, sizes and types, an array (or None) each"""
+    on_dev, lr_dev = isinstance(step, th.Tensor), isinstance(lr, th.Tensor)
+    dyn = th.empty(3, dtype=th.float32, device=dev) if on_dev else None
+    launch("ec_adamw_step", dev, len(params), *map(_address, pointers), bits, ptr(coef), 0.0 if on_dev else step,
+           ptr(step if on_dev else None), ptr(dyn), 0.0 if lr_dev else lr, ptr(lr if lr_dev else None), b1, b2, eps, weight_decay)
     # (written through raw pointers: autograd has to know; what was made in inference mode counts no versions)
     th.autograd.graph.increment_version([p for p in params if not p.is_inference()] if params[0].is_inference() else params)
 
 
 def _need_options(group):
     """torch's optimisers share their group's options by state_dict: one under which the update is another is refused"""
-    for k in ("maximize", "amsgrad", "differentiable"):
-        if group.get(k):
-            raise ValueError("AdamW: %s=%r (only False)" % (k, group[k]))
-    if not group.get("decoupled_weight_decay", True) and group["weight_decay"]:
+    get = group.get
+    if get("maximize") or get("amsgrad") or get("differentiable"):
+        raise ValueError("AdamW: %s (only False)" % ", ".join("%s=%r" % (k, get(k)) for k in ("maximize", "amsgrad", "differentiable")))
+    if not get("decoupled_weight_decay", True) and group["weight_decay"]:
         raise ValueError("AdamW: weight_decay %r with decoupled_weight_decay=False" % (group["weight_decay"],))
 
 
@@ -362,27 +358,28 @@ class AdamW(th.optim.Optimizer):
         if closure is not None:
             with th.enable_grad():
                 loss = closure()
-        calls, every, idle = [], [], []
+        calls, every, idle, state = [], [], [], self.state
         for group in self.param_groups:
             _need_options(group)
-            by_step, count = {}, None
+            by_step, count, last = {}, None, None
             for p in group["params"]:
                 g = p.grad
                 if g is None:
-                    if p in self.state:
-                        idle.append(self.state[p])
+                    if p in state:
+                        idle.append(state[p])
                     continue
                 if g.is_sparse:
                     raise RuntimeError("AdamW: sparse gradients are not supported")
                 if not g.is_contiguous():
                     g = g.contiguous()
-                if p in self.state:
-                    st = self.state[p]
-                else:
+                st = state.get(p)
+                if st is None:
                     st = self._init(group, p, count)
                     count = st["step"]
                 step = st["step"]
-                by_step.setdefault((id(step),) if isinstance(step, th.Tensor) else step, []).append((p, g, st))
+                if step is not last:  # (tensors by identity)
+                    last, ts = step, by_step.setdefault((id(step),) if isinstance(step, th.Tensor) else step, [])
+                ts.append((p, g, st))
                 every.append(g)
             calls += [(group, ts[0][2]["step"], ts) for ts in by_step.values()]
         if not every:
@@ -395,15 +392,17 @@ class AdamW(th.optim.Optimizer):
             checked.append(_checked_step([p for p, _, _ in ts], [g for _, g, _ in ts], cols("exp_avg"), cols("exp_avg_sq"), *scales,
                                          step if isinstance(step, th.Tensor) else step + 1, group["lr"], group["betas"], group["eps"],
                                          group["weight_decay"]))
-        self._split(calls, idle)
+        if idle:
+            self._split(calls, idle)
         coef = None
         if self.max_norm is not None:
             self.last_norm, coef = clip_coef(every, self.max_norm)
         for (_, step, ts), work in zip(calls, checked):
-            _launch_step(work, coef)
+            _launch_step(coef, *work)
             if not isinstance(step, th.Tensor):
+                step += 1
                 for _, _, st in ts:
-                    st["step"] = step + 1
+                    st["step"] = step
             elif th.cuda.is_current_stream_capturing():
                 self._recorded.append(step)
         return loss
