@@ -295,6 +295,10 @@ class AdamW(th.optim.Optimizer):
     def __getstate__(self):  # (torch's names three attributes: what a copy or a pickle keeps)
         return dict(super().__getstate__(), max_norm=self.max_norm, last_norm=None, _recorded=[])
 
+    def __setstate__(self, state):  # (a pickle may be older than the list)
+        super().__setstate__(state)
+        self.__dict__.setdefault("_recorded", [])
+
     def add_param_group(self, param_group):
         super().add_param_group(param_group)
         g = self.param_groups[-1]

@@ -232,3 +232,13 @@ def test_loaded_again_and_copied():
         for _ in range(3):
             o.load_state_dict(saved)
             assert _same(o.state_dict()["state"], saved["state"])
+
+
+def test_pickled_before_it_kept_recorded_counts():
+    """a pickle without the list of counts that graphs advance: unpickled it has an empty one"""
+    from marl_amd.utils.optim_device import AdamW
+    old = AdamW(_params(), capturable=True, max_norm=2.0).__getstate__()
+    del old["_recorded"]
+    opt = AdamW.__new__(AdamW)
+    opt.__setstate__(old)
+    assert opt._recorded == [] and opt.max_norm == 2.0
