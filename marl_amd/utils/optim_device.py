@@ -418,7 +418,7 @@ class AdamW(th.optim.Optimizer):
 
         def check(_, saved):
             self._need_state_dict(saved)
-            own[:] = saved, [{k: group[k] for k in self.defaults if k in group} for group in self.param_groups]
+            own[:] = saved, self._options()
 
         # (behind the last of the user's hooks in front of a load, and ahead of the first behind it)
         hooks = [self.register_load_state_dict_pre_hook(check),
@@ -429,13 +429,17 @@ class AdamW(th.optim.Optimizer):
             for h in hooks:
                 h.remove()
 
+    def _options(self):
+        return [{k: group[k] for k in self.defaults if k in group} for group in self.param_groups]
+
     def _need_state_dict(self, state_dict):
-        for saved, group in zip(state_dict["param_groups"], self.param_groups):
+        for saved, group, own in zip(state_dict["param_groups"], self.param_groups, self._options()):
+            saved = {**own, **saved}
             _need_options(saved)
-            bits = saved.get("state_bits", group["state_bits"])
+            bits = saved["state_bits"]
             if bits not in (8, 32):
                 raise ValueError("AdamW.load_state_dict: state_bits %r (8 or 32)" % (bits,))
-            if isinstance(saved["lr"], th.Tensor) and not saved.get("capturable", group["capturable"]):
+            if isinstance(saved["lr"], th.Tensor) and not saved["capturable"]:
                 raise ValueError("AdamW.load_state_dict: a learning rate on the device needs capturable=True")
             for i, p in zip(saved["params"], group["params"]):
                 if i in state_dict["state"]:

@@ -242,3 +242,17 @@ def test_pickled_before_it_kept_recorded_counts():
     opt = AdamW.__new__(AdamW)
     opt.__setstate__(old)
     assert opt._recorded == [] and opt.max_norm == 2.0
+
+
+@pytest.mark.parametrize("missing", ["lr", "weight_decay", "betas"])
+def test_options_that_are_checked_at_load_may_be_missing(missing):
+    from marl_amd.utils.optim_device import AdamW
+    opt = AdamW(_params(), lr=0.5, weight_decay=0.0)
+    saved = th.optim.Adam(_params()).state_dict()
+    del saved["param_groups"][0][missing]
+    opt.load_state_dict(saved)
+    assert opt.param_groups[0]["lr"] == (0.5 if missing == "lr" else 1e-3) and opt.param_groups[0]["betas"] == (0.9, 0.999)
+    opt.param_groups[0]["weight_decay"] = 0.1
+    del saved["param_groups"][0]["weight_decay" if missing != "weight_decay" else "lr"]
+    with pytest.raises(ValueError, match="decoupled"):   # (with the weight decay that the group would then have)
+        opt.load_state_dict(saved)
