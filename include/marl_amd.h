@@ -577,7 +577,8 @@ int ec_layer_norm_bwd(const void* dy, int64_t dy_stride, const void* x, int64_t 
  *   entropy [rows];  lse [rows][2]: the largest logit and log(sum exp(logit - largest)), their sum is the log-sum-exp
  *   top_logp f32, top_index i64 [rows][top_k]: in falling order, equal ones by index; -inf / -1 where there are fewer
  * A row with everything excluded: logp -inf, entropy 0, lse (-inf, 0).  A NaN or +inf among the entries makes the row NaN
- * (top_index -1).  Outputs are optional; top_k <= 64.  work: scratch, ec_token_logprobs_workspace bytes, 8-byte aligned. */
+ * (top_index -1).  Outputs are optional; top_k <= 64; fewer than 2^31 rows (of each split, where a row is taken by several
+ * blocks).  work: scratch, ec_token_logprobs_workspace bytes, 8-byte aligned. */
 #define EC_TOKEN_LOGPROBS_MAX_TOP 64
 int64_t ec_token_logprobs_workspace(int64_t rows, int64_t vocab, int32_t dtype, int32_t top_k);
 int ec_token_logprobs_fwd(const void* logits, int64_t inner, int64_t s_outer, int64_t s_inner, const int64_t* tokens,

@@ -3,9 +3,9 @@
 //   mean = sum x / C;  var = sum (x - mean)^2 / C;  rstd = 1 / sqrt(var + eps);  xhat = (x - mean) rstd;  y = xhat w + b
 //   dx = rstd (dy w - mean_c(dy w) - xhat mean_c(dy w xhat));  dw = sum_r dy xhat;  db = sum_r dy
 //
-// Bound by HBM: 8 and 14 operations an element against 2 and 3 elements moved.  So every element is read once: a row stays
-// in the registers of the TPR threads that share it (16 bytes a thread and load, NV loads), which makes the variance an
-// exact second pass over (x - mean) at no traffic; a thread keeps its columns from row to row, so that weight, bias and
+// Bound by HBM: 8 and 14 operations an element against 2 and 3 elements moved.  So up to 16384 columns every element is read
+// once: a row stays in the registers of the TPR threads that share it (16 bytes a thread and load, NV loads), which makes the
+// variance an exact second pass over (x - mean) at no traffic; a thread keeps its columns from row to row, so that weight, bias and
 // the sums of dw and db stay in registers over all rows of a block.  dw and db leave as one partial row per block, added
 // up in a fixed order by a second kernel (no atomics: the same bits every run).  All sums are fp32.
 //
@@ -13,7 +13,9 @@
 // 16384 rows of 4096 in bf16 48 us (5.6) and 77 us (5.2), dw and db of which 5 us more.  Rows that just miss a power of two
 // of vectors leave threads idle: 16384 rows of 2053 in fp16 43 us, of 4096 48.  (Not faster: as many waves as a row needs, a
 // number known at run time, 119 -> 145 us for 30000 rows of 1601; three vectors a thread instead of twice the threads, 43 ->
-// 44 us; idle vectors skipped by a branch, 43 -> 42 us there, but 126 -> 150 us where there are none.)
+// 44 us; idle vectors skipped by a branch, 43 -> 42 us there, but 126 -> 150 us where there are none.)  Narrow rows that end
+// inside a vector: 4 M of 11 in fp32 99 us (3.9 TB/s) and 127 us (4.4).  Long ones: 4096 rows of 16384 in fp32 98 us (5.5) and
+// 212 us (3.8: spills, see k_ln_bwd), 8192 of 10240 118 us (5.7) and 533 us (1.9), 8192 of 16384 in bf16 98 us (5.5) and 160 us (5.0).
 #include "ec_stream.h"
 
 namespace {
@@ -246,7 +248,8 @@ __global__ void __launch_bounds__(block_threads(TPR)) k_ln_bwd(NormArgs p) {
     int slot = 0;
     const RowReader<T, V, TPR, NV, NT> in_x(p.x, p.x_stride, p.rows, p.cols), in_dy(p.dy, p.dy_stride, p.rows, p.cols);
     // (a block of 1024 threads has 128 registers a thread: no room for the next row with two vectors or more; the row then
-    // stays as it was read, and xhat and dy w are made from it twice)
+    // stays as it was read, and xhat and dy w are made from it twice.  Weights, both sums and the row are more than 128 even
+    // so: 99 registers a thread go to scratch in fp32, 16 to 18 in 16 bits)
     constexpr bool AHEAD = TPR < 1024 || NV == 1;
     raw_t<T, V> x[NV], dy[NV], next_x[NV], next_dy[NV];
     float mean = 0.0f, rstd = 0.0f, next_mean = 0.0f, next_rstd = 0.0f;
@@ -377,7 +380,9 @@ __global__ void __launch_bounds__(1024) k_ln_wgrad(const float* partials, int n,
     }
 }
 
-// ---- rows too long for the registers of a block: a block of 1024 threads reads its row again for each pass (from L2) ----
+// ---- rows too long for the registers of a block: a block of 1024 threads reads its row again for each pass, three times
+// forward, x and dy twice for dx and once more for dw and db (2048 rows of 32768 in bf16: 84 us forward, 105 + 57 + 5 back,
+// against 42 and 63 for each element moved once at 6.4 TB/s; 1024 in fp32: 84 and 101 + 49 + 5) ----
 constexpr int WIDE = 1024;
 
 template <typename T>
